@@ -37,6 +37,7 @@ extern "C" {
 #define KB200_FP16 0
 #define KB200_BF16 1
 #define KB200_FP8_E4M3 2   /* KV caches of the decode calls only, see kb200_kv_layout */
+#define KB200_INT4 3       /* KV caches of the decode calls and of kb200_kv_write / kb200_kv_read, see kb200_kv_layout */
 
 #define KB200_HEAD_DIM 128
 #define KB200_GROUP_SIZE 4
@@ -113,7 +114,7 @@ typedef struct kb200_kv_layout {
   int32_t page_size;          /* power of two, >= 1 */
   int32_t dtype;              /* KB200_FP16 / KB200_BF16: type of the cache, of q and of the output of a decode call;
                                  KB200_FP8_E4M3: the cache holds e4m3 bytes (strides in bytes, multiples of 16), q and
-                                 the output are fp16 */
+                                 the output are fp16; KB200_INT4: see below */
   /* FP8 caches: value = stored e4m3 value x scale, one fp32 scale per (page, KV head), K and V separately:
    *   k_scale[b * scale_stride_batch + page * scale_stride_page + g * scale_stride_head]   (page as in the address
    * rule above: physical page with a block table).  The kernels turn the stored bytes into fp16 exactly and
@@ -124,6 +125,25 @@ typedef struct kb200_kv_layout {
   int64_t scale_stride_batch;
   int64_t scale_stride_page;
   int64_t scale_stride_head;
+  /* INT4 caches.  A row of 128 values is four groups of 32; a group keeps a scale s and a zero z in fp16 and a value as a
+   * code c of 0..15, which stands for  s * c + z.  The 128 codes of a row are 64 bytes (strides of the cache in bytes,
+   * multiples of 16), two per byte, the low nibble first; counted so, nibble n of
+   *   a K row is value 32 g + 8 q + i  with n = 32 q + 8 g + i   (q, g = 0..3, i = 0..7),
+   *   a V row is value 32 g + 4 r + i  with n = 16 r + 4 g + i   (r = 0..7, g, i = 0..3):
+   * the orders in which the lanes of a matrix operand hold them.  The parameters of the row of (token, head) are eight
+   * fp16, s of groups 0..3 and z of groups 0..3, at
+   *   k_param[b * param_stride_batch + page * param_stride_page + slot * param_stride_token + g * param_stride_head]
+   * (strides in elements, multiples of 8, the same for v_param; lay the two rows' parameters beside each other, so that
+   * one 32-byte sector holds both).  A row is complete in itself, so rows can move between pages (kb200_evict_move).
+   * act_dtype: KB200_FP16 or KB200_BF16, the type of q and of the output of a decode call, and of the rows that
+   * kb200_kv_write takes and kb200_kv_read gives.  The reference has no quantised cache. */
+  const void* k_param;
+  const void* v_param;
+  int64_t param_stride_batch;
+  int64_t param_stride_page;
+  int64_t param_stride_token;
+  int64_t param_stride_head;
+  int32_t act_dtype;
 } kb200_kv_layout;
 
 /* Workspace for kb200_decode_sparse_paged / kb200_decode_anchor_paged (split-K partials). */
@@ -365,7 +385,10 @@ int kb200_prefill_budgets(int32_t* n_valid, int32_t* k_row, int batch, int num_k
  *   kv          the cache (written): paged with a block table that already covers the new positions, or contiguous;
  *               or an FP8 cache (dtype KB200_FP8_E4M3, k_scale / v_scale given by the caller, e.g. calibrated per
  *               layer): a row is stored as value / scale of its page and KV head (fp32 division, saturating at
- *               +-448, round to nearest even) - the bytes the decode entry points read back as byte x scale
+ *               +-448, round to nearest even) - the bytes the decode entry points read back as byte x scale;
+ *               or an INT4 cache: per group of 32 values  z = fp16(min), s = fp16((max - z) / 15 in fp32) and the codes
+ *               round((x - z) / s), half to even, clamped to 0..15.  What fp16 cannot hold saturates; a group with a value
+ *               that is not finite gets z = NaN
  *   q_norm_gain / k_norm_gain  [D] in the same type, or NULL (no norm);  norm_eps
  *   inv_freq    [D/2] fp32 inverse frequencies of the model's rotary embedding (device memory), or NULL
  *               (no rotary);  rope_scale multiplies cos and sin (1 for the default rope type)
@@ -375,6 +398,86 @@ int kb200_kv_write(const kb200_act_layout* q_in, void* q_out, const kb200_act_la
                    const kb200_kv_layout* kv, const void* q_norm_gain, const void* k_norm_gain,
                    float norm_eps, const float* inv_freq, float rope_scale, int batch, int max_new,
                    int num_q_heads, int num_kv_heads, void* stream);
+
+/* kb200_kv_write for tokens whose rotary positions are not their places in the cache: a cache that rows have left
+ * (kb200_evict_plan), images and video with positions on several axes (time, height, width).
+ * Pair i of a head (elements i and i + 64) turns by positions[pair_axis[i]] * inv_freq[i].  The angle is formed in 64 bits,
+ * norm and rotation are computed in fp32 and rounded once (kb200_kv_write repeats the modules' roundings instead).
+ *   positions  [axes, B, T] int32: element (axis, b, t) at axis * stride_axis + b * stride_batch + t
+ *   pair_axis  [64] int32 with values in [0, axes) (others are clamped), or NULL: the first axis for all
+ *   token_positions  [B, token_rows] int32 (rows token_stride apart), or NULL: receives positions[0] of every token at its
+ *              row of the cache, start_pos[b] + t; rows beyond token_rows are not noted
+ * All other arguments as kb200_kv_write; start_pos is the place in the cache only. */
+typedef struct kb200_positions {
+  const int32_t* positions;
+  int64_t stride_axis;
+  int64_t stride_batch;
+  const int32_t* pair_axis;
+  int32_t axes;
+  int32_t* token_positions;
+  int64_t token_stride;
+  int32_t token_rows;
+} kb200_positions;
+int kb200_kv_write_at(const kb200_act_layout* q_in, void* q_out, const kb200_act_layout* k_new,
+                      const kb200_act_layout* v_new, const int32_t* start_pos, const int32_t* n_new,
+                      const kb200_kv_layout* kv, const void* q_norm_gain, const void* k_norm_gain,
+                      float norm_eps, const float* inv_freq, float rope_scale, const kb200_positions* at,
+                      int batch, int max_new, int num_q_heads, int num_kv_heads, void* stream);
+
+/* Rows 0 .. seq_lens[b] - 1 of an INT4 cache in 16 bits (act_dtype of the layout), for a prompt that arrives in pieces: the
+ * prefill kernels take fp16 / bf16.
+ *   k_out / v_out  [B, max_len, G, 128] contiguous; rows behind a sequence are written as zeros */
+int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens, void* k_out, void* v_out, int batch, int max_len,
+                  int num_kv_heads, void* stream);
+
+/* ---- eviction from a cache by accumulated attention weight -------------------------------------
+ * The weight of a cache row is the attention that later queries paid to it, summed over the query heads and over whatever
+ * layers and steps the caller adds up: what the anchor layers' pooled scores hold anyway.  It is kept per sequence, not per
+ * head, because anchor layers hand their index rows to the reuse layers of other heads: a row has to mean the same token
+ * in every layer and head.  The reference has no eviction. */
+
+/* Weight of a decode step (pooled [B, G, row_stride] of kb200_decode_anchor_paged), for the rows j < seq_lens[b] and j < max_len:
+ *   mass_out[b, j] = mass_in[b, j] + sum_g pooled[b, g, j]        (added up in the order of g)
+ * mass_out may be mass_in (rows mass_stride apart, both of them). */
+int kb200_mass_add(const float* pooled, int64_t row_stride, const int32_t* seq_lens, const float* mass_in, float* mass_out,
+                   int64_t mass_stride, int batch, int num_kv_heads, int max_len, void* stream);
+
+/* Weight of a prompt (pooled [B, G, num_tiles, row_stride] of kb200_prefill_pool_scores[_ragged]):
+ *   mass_out[b, j] = mass_in[b, j] + sum_g sum_{t : 32 t > j} pooled[b, g, t, j]     for 0 <= j < n_rows
+ * over the tiles t < ceil(seq_len[b] / 32) (NULL: num_tiles for every sequence).  What a tile's queries pay to the tile's own
+ * keys is not part of the pooled scores.  n_rows >= 32 * (num_tiles - 1), row_stride >= that; mass_out may be mass_in. */
+int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t* seq_len, const float* mass_in,
+                          float* mass_out, int64_t mass_in_stride, int64_t mass_out_stride, int batch, int num_kv_heads,
+                          int num_tiles, int n_rows, void* stream);
+
+/* What eviction ranks the rows of a cache by, for kb200_topk_select with k_max = budget:
+ *   keys[b, j] = +inf for protected rows, else mass[b, j] (a NaN counts as 0)        for j < seq_lens[b]
+ * Protected are the rows whose token position is below `sinks` or within the last `recent` of the sequence's positions.
+ *   token_positions  [B, rows] int32 (pos_stride apart), or NULL: the row's number (a cache that no row has left yet) */
+int kb200_evict_keys(const float* mass, int64_t mass_stride, const int32_t* seq_lens, const int32_t* token_positions,
+                     int64_t pos_stride, int sinks, int recent, float* keys, int64_t key_stride, int batch, int n_rows,
+                     void* stream);
+
+/* Turns the kept rows of every sequence (kb200_topk_select's output over the keys: ascending, keep_count[b] of them) into the
+ * moves that bring them together in rows 0 .. keep_count[b] - 1.  Kept rows below keep_count[b] stay where they are; those behind
+ * fill the rows that were let go, the lowest into the lowest.  That is the smallest number of moves, and no row is both
+ * source and target, so the moves have no order.  (The order of rows in a cache has no meaning to attention: positions
+ * are in the keys' rotation.)
+ *   moves      [B, move_stride] pairs (source row, target row) int32, move_stride >= budget (in pairs); move_count [B]
+ *   new_lens   [B] receives keep_count
+ *   mass_out / pos_out  [B, n_rows] (out_stride apart): the rows' weight and token position after the moves, 0 and -1 behind
+ *              new_lens[b]; neither may be its input.  pos_out may be NULL; pos_in may be NULL (the row's number) */
+int kb200_evict_plan(const int32_t* keep, int64_t keep_stride, const int32_t* keep_count, const float* mass_in,
+                     int64_t mass_stride, const int32_t* pos_in, int64_t pos_stride, int32_t* moves, int64_t move_stride,
+                     int32_t* move_count, int32_t* new_lens, float* mass_out, int32_t* pos_out,
+                     int64_t out_stride, int batch, int n_rows, void* stream);
+
+/* Moves rows inside the caches of several layers.  All layers share the block table; fp16 / bf16 or INT4 caches (an FP8
+ * cache has one scale per page, so its rows cannot leave their page: refused), one type and one set of strides per call.
+ *   layers     host array of n_layers layouts
+ *   max_moves  the most moves of a sequence (the grid's size) */
+int kb200_evict_move(const kb200_kv_layout* layers, int n_layers, const int32_t* moves, int64_t move_stride,
+                     const int32_t* move_count, int max_moves, int batch, int num_kv_heads, void* stream);
 
 /* ---- diagnostics ----------------------------------------------------------------------------- */
 

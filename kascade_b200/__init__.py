@@ -4,6 +4,7 @@
 kernels live in ``libkascade_b200.so`` (C ABI in ``include/kascade_b200.h``), built in-tree by
 ``python -m kascade_b200.build``.
 """
-from .strategy import EfficientKascadeStrategy, Strategy, topk_budget  # noqa: F401
+from .strategy import (  # noqa: F401
+    EfficientKascadeStrategy, Strategy, int4_kv_cache, rope_axis_map, topk_budget)
 
 __version__ = "0.1.0"

@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libkascade_b200.so")
 HEAD_DIM = 128
 GROUP_SIZE = 4
 TILE = 32
-FP16, BF16, FP8_E4M3 = 0, 1, 2        # KB200_FP16 / KB200_BF16 / KB200_FP8_E4M3
+FP16, BF16, FP8_E4M3, INT4 = 0, 1, 2, 3        # KB200_FP16 / KB200_BF16 / KB200_FP8_E4M3 / KB200_INT4
 DTYPES = {torch.float16: FP16, torch.bfloat16: BF16}
 FP8_TORCH = (torch.float8_e4m3fn, torch.uint8)   # an FP8 cache may be handed over as raw bytes
 
@@ -30,6 +30,8 @@ EXPORTS = [
     "kb200_decode_sparse_paged_noalloc", "kb200_prefill_dense_fanout", "kb200_prefill_sparse_fanout",
     "kb200_kv_write", "kb200_prefill_dense_ragged", "kb200_prefill_pool_scores_ragged", "kb200_prefill_sparse_ragged",
     "kb200_prefill_budgets_ragged", "kb200_zero_padding", "kb200_peer_push", "kb200_stream_wait_events", "kb200_selftest_wait_timeout", "kb200_tensor_map_encodes", "kb200_decode_noalloc_splits",
+    "kb200_kv_write_at", "kb200_kv_read", "kb200_mass_add", "kb200_mass_add_prompt", "kb200_evict_keys", "kb200_evict_plan",
+    "kb200_evict_move",
 ]
 
 
@@ -43,7 +45,16 @@ class KvLayout(C.Structure):
                 ("block_table", C.c_void_p), ("block_table_stride", C.c_int32),
                 ("page_size", C.c_int32), ("dtype", C.c_int32),
                 ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_stride_batch", C.c_int64),
-                ("scale_stride_page", C.c_int64), ("scale_stride_head", C.c_int64)]
+                ("scale_stride_page", C.c_int64), ("scale_stride_head", C.c_int64),
+                ("k_param", C.c_void_p), ("v_param", C.c_void_p), ("param_stride_batch", C.c_int64),
+                ("param_stride_page", C.c_int64), ("param_stride_token", C.c_int64), ("param_stride_head", C.c_int64),
+                ("act_dtype", C.c_int32)]
+
+
+class Positions(C.Structure):
+    """kb200_positions: rotary positions of new tokens that are not their places in the cache."""
+    _fields_ = [("positions", C.c_void_p), ("stride_axis", C.c_int64), ("stride_batch", C.c_int64), ("pair_axis", C.c_void_p),
+                ("axes", C.c_int32), ("token_positions", C.c_void_p), ("token_stride", C.c_int64), ("token_rows", C.c_int32)]
 
 
 class ActLayout(C.Structure):
@@ -149,6 +160,14 @@ def load() -> C.CDLL:
         lib.kb200_zero_padding.argtypes = [vp, RG, i32, i32, i64, vp]
         lib.kb200_kv_write.argtypes = [AL, vp, AL, AL, vp, vp, C.POINTER(KvLayout), vp, vp, f32, vp, f32, i32, i32,
                                        i32, i32, vp]
+        lib.kb200_kv_write_at.argtypes = [AL, vp, AL, AL, vp, vp, C.POINTER(KvLayout), vp, vp, f32, vp, f32,
+                                          C.POINTER(Positions), i32, i32, i32, i32, vp]
+        lib.kb200_kv_read.argtypes = [C.POINTER(KvLayout), vp, vp, vp, i32, i32, i32, vp]
+        lib.kb200_mass_add.argtypes = [vp, i64, vp, vp, vp, i64, i32, i32, i32, vp]
+        lib.kb200_mass_add_prompt.argtypes = [vp, i64, vp, vp, vp, i64, i64, i32, i32, i32, i32, vp]
+        lib.kb200_evict_keys.argtypes = [vp, i64, vp, vp, i64, i32, i32, vp, i64, i32, i32, vp]
+        lib.kb200_evict_plan.argtypes = [vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i32, i32, vp]
+        lib.kb200_evict_move.argtypes = [C.POINTER(KvLayout), i32, vp, i64, vp, i32, i32, i32, vp]
         lib.kb200_selftest_umma.argtypes = [vp, vp, vp, vp, vp]
         lib.kb200_peer_push.argtypes = [C.POINTER(PushPlan), vp, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, vp, vp]
         lib.kb200_stream_wait_events.argtypes = [vp, C.POINTER(C.c_void_p), i32]
@@ -236,6 +255,12 @@ def _want(t: torch.Tensor, dtype, name: str):
         raise KascadeNativeError(f"{name}: expected a CUDA {dtype} tensor, got {t.dtype} on {t.device}")
 
 
+def _same_device(first: torch.Tensor, **others: Optional[torch.Tensor]):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise KascadeNativeError(f"{name} is on {t.device}, expected {first.device}")
+
+
 def _half_code(t: torch.Tensor, name: str) -> int:
     """KB200_FP16 / KB200_BF16 of a CUDA fp16 or bf16 tensor."""
     if t.dtype not in DTYPES or not t.is_cuda:
@@ -308,10 +333,53 @@ def _holding(layout, *tensors):
     return layout
 
 
+def is_int4(cache: torch.Tensor) -> bool:
+    """Whether a cache holds 4-bit codes: uint8 rows of 64 bytes (a raw FP8 row has 128)."""
+    return cache.dtype == torch.uint8 and cache.shape[-1] == HEAD_DIM // 2
+
+
+def _int4_params(k, v, k_param, v_param):
+    """The checks of an INT4 cache: codes [..., 64] uint8 and parameters [..., 8] fp16 of the same leading shape."""
+    if not k.is_cuda:
+        raise KascadeNativeError(f"k_cache: expected a CUDA uint8 tensor, got one on {k.device}")
+    if k.dim() != 4 or k.stride(3) != 1:
+        raise KascadeNativeError("an INT4 cache holds rows of 64 contiguous bytes: [num_pages, page_size, G, 64]")
+    if v is not None and (v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype):
+        raise KascadeNativeError("k_cache and v_cache must have the same type, shape and strides")
+    if k_param is None or (v is not None and v_param is None):
+        raise KascadeNativeError("an INT4 cache needs k_scale (and v_scale): eight fp16 per row, four scales and four zeros")
+    for name, par in (("k_scale", k_param), ("v_scale", v_param if v is not None else None)):
+        if par is None:
+            continue
+        _want(par, torch.float16, name)
+        if par.shape != k.shape[:3] + (8,) or par.stride(3) != 1:
+            raise KascadeNativeError(f"{name} of an INT4 cache: expected {tuple(k.shape[:3]) + (8,)}, the last dimension "
+                                     f"contiguous, got {tuple(par.shape)}")
+    if v is not None and v_param.stride() != k_param.stride():
+        raise KascadeNativeError("k_scale and v_scale must have the same shape and strides")
+    _same_device(k, v_cache=v, k_scale=k_param, v_scale=v_param)
+
+
 def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], block_table: torch.Tensor,
-                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> KvLayout:
+                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                    act_dtype: torch.dtype = torch.float16) -> KvLayout:
     """vLLM-style cache [num_pages, page_size, G, D] and block table [B, max_pages] int32.  An FP8 cache
-    (torch.float8_e4m3fn or raw uint8) comes with k_scale / v_scale [num_pages, G] fp32."""
+    (torch.float8_e4m3fn or raw uint8) comes with k_scale / v_scale [num_pages, G] fp32; an INT4 cache (uint8
+    [num_pages, page_size, G, 64]) with k_scale / v_scale [num_pages, page_size, G, 8] fp16 and `act_dtype`, the type of the
+    queries, outputs and new rows."""
+    if is_int4(k_cache):
+        _int4_params(k_cache, v_cache, k_scale, v_scale)
+        if act_dtype not in DTYPES:
+            raise KascadeNativeError(f"act_dtype of an INT4 cache: expected fp16 or bf16, got {act_dtype}")
+        _want(block_table, torch.int32, "block_table")
+        _same_device(k_cache, block_table=block_table)
+        if block_table.dim() != 2 or block_table.stride(1) != 1:
+            raise KascadeNativeError("block_table: expected [B, max_pages], the last dimension contiguous")
+        st, ps = k_cache.stride(), k_scale.stride()
+        return _holding(KvLayout(k_cache.data_ptr(), _ptr(v_cache), 0, st[0], st[1], st[2], block_table.data_ptr(),
+                                 block_table.stride(0), k_cache.shape[1], INT4, 0, 0, 0, 0, 0, k_scale.data_ptr(),
+                                 _ptr(v_scale) if v_cache is not None else 0, 0, ps[0], ps[1], ps[2], DTYPES[act_dtype]),
+                        k_cache, v_cache, block_table, k_scale, v_scale)
     if k_cache.dtype in FP8_TORCH:
         assert k_cache.is_cuda and k_cache.dim() == 4 and k_cache.stride(3) == 1
         assert block_table.dtype == torch.int32 and block_table.stride(1) == 1
@@ -336,9 +404,18 @@ def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], bloc
 
 
 def kv_layout_contiguous(k: torch.Tensor, v: Optional[torch.Tensor], page_size: int = 16,
-                         k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> KvLayout:
+                         k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                         act_dtype: torch.dtype = torch.float16) -> KvLayout:
     """HF cache view [B, G, L, D] (any batch / head / token strides, D contiguous).  An FP8 cache comes with
-    k_scale / v_scale [B, G, ceil(L / page_size)] fp32."""
+    k_scale / v_scale [B, G, ceil(L / page_size)] fp32, an INT4 cache [B, G, L, 64] with [B, G, L, 8] fp16."""
+    if is_int4(k):
+        _int4_params(k, v, k_scale, v_scale)
+        if act_dtype not in DTYPES:
+            raise KascadeNativeError(f"act_dtype of an INT4 cache: expected fp16 or bf16, got {act_dtype}")
+        st, ps = k.stride(), k_scale.stride()
+        return _holding(KvLayout(k.data_ptr(), _ptr(v), st[0], st[2] * page_size, st[2], st[1], 0, 0, page_size, INT4, 0, 0, 0, 0,
+                                 0, k_scale.data_ptr(), _ptr(v_scale) if v is not None else 0, ps[0], ps[2] * page_size, ps[2],
+                                 ps[1], DTYPES[act_dtype]), k, v, k_scale, v_scale)
     if k.dtype in FP8_TORCH:
         assert k.is_cuda and k.dim() == 4 and k.stride(3) == 1
         if v is not None:
@@ -385,13 +462,19 @@ def sm_count(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
+def _check_q(q, kv: KvLayout):
+    want = FP16 if kv.dtype == FP8_E4M3 else kv.act_dtype if kv.dtype == INT4 else kv.dtype
+    if _half_code(q, "q") != want:
+        raise KascadeNativeError(f"q is {q.dtype} but the KV cache has dtype code {kv.dtype} (an FP8 cache takes fp16 q, an INT4 "
+                                 "cache the type given as act_dtype)")
+
+
 @_on_device_of(0)
 def decode_sparse_paged(q, kv: KvLayout, topk_idx, topk_count, k_max, head_map, scale, out, lse2=None,
                         workspace=None, num_splits=0):
     """q [B,H,D] fp16; topk_idx [B,G,kstride] int32; out [B,H,D] fp16 contiguous."""
     lib = init(q.get_device())
-    if _half_code(q, "q") != (FP16 if kv.dtype == FP8_E4M3 else kv.dtype):
-        raise KascadeNativeError(f"q is {q.dtype} but the KV cache has dtype code {kv.dtype} (an FP8 cache takes fp16 q)")
+    _check_q(q, kv)
     _want(out, q.dtype, "out")
     _want(topk_idx, torch.int32, "topk_idx")
     _want_opt(topk_count, torch.int32, "topk_count")
@@ -418,8 +501,7 @@ def decode_sparse_paged_noalloc(q, kv: KvLayout, topk_idx, topk_count, k_max, he
     partials live in a fixed array inside the library (batch * heads * splits <= NOALLOC_MAX_SLOTS).
     Calls that overlap on the GPU race on that array; the first call on a device belongs in set-up."""
     lib = init(q.get_device())
-    if _half_code(q, "q") != (FP16 if kv.dtype == FP8_E4M3 else kv.dtype):
-        raise KascadeNativeError(f"q is {q.dtype} but the KV cache has dtype code {kv.dtype} (an FP8 cache takes fp16 q)")
+    _check_q(q, kv)
     _want(out, q.dtype, "out")
     _want(topk_idx, torch.int32, "topk_idx")
     _want_opt(topk_count, torch.int32, "topk_count")
@@ -439,8 +521,7 @@ def decode_anchor_paged(q, kv: KvLayout, seq_lens, max_seq_len, scale, logits, p
                         workspace=None, num_splits=0):
     """q [B,H,D]; logits [B,H,stride] fp32; pooled [B,G,stride] fp32; out [B,H,D] fp16 or None."""
     lib = init(q.get_device())
-    if _half_code(q, "q") != (FP16 if kv.dtype == FP8_E4M3 else kv.dtype):
-        raise KascadeNativeError(f"q is {q.dtype} but the KV cache has dtype code {kv.dtype} (an FP8 cache takes fp16 q)")
+    _check_q(q, kv)
     _want_opt(out, q.dtype, "out")
     _want(logits, torch.float32, "logits")
     _want(pooled, torch.float32, "pooled")
@@ -567,10 +648,11 @@ def prefill_sparse(q, k, v, tile_idx, tile_count, head_map, scale, out, lse2=Non
 
 @_on_device_of(2)
 def kv_write(q_in, q_out, k_new, v_new, start_pos, n_new, kv: KvLayout, q_gain=None, k_gain=None, eps=1e-6,
-             inv_freq=None, rope_scale=1.0):
+             inv_freq=None, rope_scale=1.0, positions=None, pair_axis=None, token_positions=None):
     """q_in [B,T,H,D] (or None), k_new / v_new [B,T,G,D] views, all fp16 or all bf16 like the cache and the gains;
     start_pos [B] int32; n_new [B] int32 or None; kv: the cache to append to (kv_layout_paged /
-    kv_layout_contiguous); inv_freq [D/2] fp32 or None."""
+    kv_layout_contiguous); inv_freq [D/2] fp32 or None.  With `positions` [axes, B, T] int32 the tokens have rotary positions of
+    their own (kb200_kv_write_at): pair_axis [D/2] int32 or None, token_positions [B, rows] int32 or None."""
     lib = init(k_new.get_device())
     B, T, G, _ = k_new.shape
     kl, vl = act_layout(k_new), act_layout(v_new)
@@ -586,10 +668,166 @@ def kv_write(q_in, q_out, k_new, v_new, start_pos, n_new, kv: KvLayout, q_gain=N
     if inv_freq is not None:
         _want(inv_freq, torch.float32, "inv_freq")
         assert inv_freq.is_contiguous() and inv_freq.numel() == HEAD_DIM // 2
+    if positions is not None:
+        _want(positions, torch.int32, "positions")
+        _want_opt(pair_axis, torch.int32, "pair_axis")
+        _want_opt(token_positions, torch.int32, "token_positions")
+        _same_device(k_new, positions=positions, pair_axis=pair_axis, token_positions=token_positions)
+        if positions.dim() != 3 or positions.shape[1:] != (B, T) or (T > 1 and positions.stride(2) != 1) or not positions.shape[0]:
+            raise KascadeNativeError(f"positions: expected [axes, {B}, {T}], the last dimension contiguous, got "
+                                     f"{tuple(positions.shape)}")
+        if pair_axis is not None and (pair_axis.shape != (HEAD_DIM // 2,) or not pair_axis.is_contiguous()):
+            raise KascadeNativeError(f"pair_axis: expected [{HEAD_DIM // 2}] contiguous, got {tuple(pair_axis.shape)}")
+        if token_positions is not None and (token_positions.dim() != 2 or token_positions.shape[0] != B
+                                            or token_positions.stride(1) != 1):
+            raise KascadeNativeError(f"token_positions: expected [{B}, rows], the last dimension contiguous, got "
+                                     f"{tuple(token_positions.shape)}")
+        at = Positions(positions.data_ptr(), positions.stride(0), positions.stride(1), _ptr(pair_axis), positions.shape[0],
+                       _ptr(token_positions), 0 if token_positions is None else token_positions.stride(0),
+                       0 if token_positions is None else token_positions.shape[1])
+        _check(lib.kb200_kv_write_at(C.byref(ql), _ptr(q_out), C.byref(kl), C.byref(vl), _ptr(start_pos), _ptr(n_new),
+                                     C.byref(kv), _ptr(q_gain), _ptr(k_gain), float(eps), _ptr(inv_freq), float(rope_scale),
+                                     C.byref(at), B, T, H, G, _stream()), "kb200_kv_write_at")
+        _launched(1)
+        return
     _check(lib.kb200_kv_write(C.byref(ql), _ptr(q_out), C.byref(kl), C.byref(vl), _ptr(start_pos), _ptr(n_new),
                               C.byref(kv), _ptr(q_gain), _ptr(k_gain), float(eps), _ptr(inv_freq), float(rope_scale),
                               B, T, H, G, _stream()), "kb200_kv_write")
     _launched(1)
+
+
+@_on_device_of(2)
+def kv_read(kv: KvLayout, seq_lens, k_out, v_out):
+    """Rows 0 .. seq_lens[b] - 1 of an INT4 cache into k_out / v_out [B, max_len, G, D] (contiguous, of the layout's act_dtype);
+    rows behind a sequence are written as zeros."""
+    lib = init(k_out.get_device())
+    B, T, G, _ = k_out.shape
+    if kv.dtype != INT4:
+        raise KascadeNativeError("kv_read: the cache is not INT4: its rows need no conversion")
+    _want(seq_lens, torch.int32, "seq_lens")
+    if _half_code(k_out, "k_out") != kv.act_dtype or v_out.dtype != k_out.dtype or v_out.shape != k_out.shape:
+        raise KascadeNativeError("kv_read: k_out and v_out must have one shape and the layout's act_dtype")
+    if not (k_out.is_contiguous() and v_out.is_contiguous() and seq_lens.is_contiguous()) or seq_lens.shape != (B,) \
+            or k_out.shape[3] != HEAD_DIM:
+        raise KascadeNativeError(f"kv_read: expected contiguous k_out / v_out [B, T, G, {HEAD_DIM}] and seq_lens [B]")
+    _same_device(k_out, v_out=v_out, seq_lens=seq_lens)
+    _check(lib.kb200_kv_read(C.byref(kv), _ptr(seq_lens), _ptr(k_out), _ptr(v_out), B, T, G, _stream()), "kb200_kv_read")
+    _launched(1 if k_out.numel() else 0)
+
+
+def _want_rows(t: torch.Tensor, dtype, batch: int, name: str):
+    """[batch, rows] with the rows of a sequence contiguous."""
+    _want(t, dtype, name)
+    if t.dim() != 2 or t.shape[0] != batch or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise KascadeNativeError(f"{name}: expected [{batch}, rows], the last dimension contiguous, got {tuple(t.shape)} with strides "
+                                 f"{t.stride()}")
+
+
+@_on_device_of(0)
+def mass_add(pooled, seq_lens, mass, out, max_len: int):
+    """out[b, j] = mass[b, j] + sum over the heads of pooled [B, G, row_stride], for j < seq_lens[b]; `out` may be `mass`."""
+    lib = init(pooled.get_device())
+    _want(pooled, torch.float32, "pooled")
+    _want(seq_lens, torch.int32, "seq_lens")
+    B, G, stride = pooled.shape
+    _want_rows(mass, torch.float32, B, "mass")
+    _want_rows(out, torch.float32, B, "out")
+    if not pooled.is_contiguous() or not seq_lens.is_contiguous() or seq_lens.shape != (B,) or out.stride(0) != mass.stride(0):
+        raise KascadeNativeError("mass_add: pooled and seq_lens must be contiguous, mass and out equally strided")
+    if mass.shape[1] < max_len or out.shape[1] < max_len:
+        raise KascadeNativeError(f"mass_add: mass holds {mass.shape[1]} rows, {max_len} are needed")
+    _same_device(pooled, seq_lens=seq_lens, mass=mass, out=out)
+    _check(lib.kb200_mass_add(_ptr(pooled), stride, _ptr(seq_lens), _ptr(mass), _ptr(out),
+                              mass.stride(0) if B > 1 else mass.shape[1], B, G, max_len, _stream()), "kb200_mass_add")
+    _launched(1 if B and max_len else 0)
+
+
+@_on_device_of(0)
+def mass_add_prompt(pooled, mass, out, seq_len=None):
+    """out[b, j] = mass[b, j] + the scores of row j over the heads and the later tiles of pooled [B, G, T, row_stride];
+    `out` may be `mass`."""
+    lib = init(pooled.get_device())
+    _want(pooled, torch.float32, "pooled")
+    B, G, T, stride = pooled.shape
+    _want_rows(mass, torch.float32, B, "mass")
+    _want_rows(out, torch.float32, B, "out")
+    _want_opt(seq_len, torch.int32, "seq_len")
+    if not pooled.is_contiguous() or (seq_len is not None and (seq_len.shape != (B,) or not seq_len.is_contiguous())) \
+            or out.shape != mass.shape:
+        raise KascadeNativeError("mass_add_prompt: pooled and seq_len [B] must be contiguous, out must have the shape of mass")
+    _same_device(pooled, seq_len=seq_len, mass=mass, out=out)
+    rows = mass.shape[1]
+    _check(lib.kb200_mass_add_prompt(_ptr(pooled), stride, _ptr(seq_len), _ptr(mass), _ptr(out),
+                                     mass.stride(0) if B > 1 else rows, out.stride(0) if B > 1 else rows, B, G, T, rows,
+                                     _stream()), "kb200_mass_add_prompt")
+    _launched(1 if B and rows else 0)
+
+
+@_on_device_of(0)
+def evict_keys(mass, seq_lens, token_positions, sinks: int, recent: int, keys):
+    """keys [B, key_stride >= rows] fp32: what the rows of a cache are ranked by, see kb200_evict_keys."""
+    lib = init(mass.get_device())
+    B, rows = mass.shape
+    _want_rows(mass, torch.float32, B, "mass")
+    _want(keys, torch.float32, "keys")
+    _want(seq_lens, torch.int32, "seq_lens")
+    if token_positions is not None:
+        _want_rows(token_positions, torch.int32, B, "token_positions")
+        if token_positions.shape[1] != rows:
+            raise KascadeNativeError(f"token_positions: expected {(B, rows)}, got {tuple(token_positions.shape)}")
+    if seq_lens.shape != (B,) or not seq_lens.is_contiguous() or not keys.is_contiguous() or keys.shape[0] != B:
+        raise KascadeNativeError("evict_keys: seq_lens [B] and keys [B, key_stride] must be contiguous")
+    _same_device(mass, seq_lens=seq_lens, token_positions=token_positions, keys=keys)
+    _check(lib.kb200_evict_keys(_ptr(mass), mass.stride(0), _ptr(seq_lens), _ptr(token_positions),
+                                0 if token_positions is None else token_positions.stride(0), int(sinks), int(recent), _ptr(keys),
+                                keys.shape[1], B, rows, _stream()), "kb200_evict_keys")
+    _launched(1 if B and rows else 0)
+
+
+@_on_device_of(0)
+def evict_plan(keep, keep_count, mass, token_positions, moves, move_count, new_lens, mass_out, pos_out):
+    """keep [B, budget] int32 ascending and keep_count [B]: the rows that stay; moves [B, budget, 2], move_count, new_lens [B] int32
+    and the rows' weight and token position after the moves, see kb200_evict_plan."""
+    lib = init(keep.get_device())
+    B, rows = mass.shape
+    for name, t in (("keep", keep), ("keep_count", keep_count), ("moves", moves), ("move_count", move_count), ("new_lens", new_lens)):
+        _want(t, torch.int32, name)
+        if not t.is_contiguous() or t.shape[0] != B:
+            raise KascadeNativeError(f"evict_plan: {name} must be contiguous, with a row for each of {B} sequences")
+    _want_rows(mass, torch.float32, B, "mass")
+    _want(mass_out, torch.float32, "mass_out")
+    _want(pos_out, torch.int32, "pos_out")
+    if token_positions is not None:
+        _want_rows(token_positions, torch.int32, B, "token_positions")
+    if moves.shape != keep.shape + (2,) or mass_out.shape != mass.shape or pos_out.shape != mass.shape \
+            or not mass_out.is_contiguous() or not pos_out.is_contiguous() \
+            or (token_positions is not None and token_positions.shape != mass.shape):
+        raise KascadeNativeError("evict_plan: moves must be [B, budget, 2], the weights and positions [B, rows]")
+    _same_device(keep, keep_count=keep_count, mass=mass, token_positions=token_positions, moves=moves, move_count=move_count,
+                 new_lens=new_lens, mass_out=mass_out, pos_out=pos_out)
+    _check(lib.kb200_evict_plan(_ptr(keep), keep.shape[1], _ptr(keep_count), _ptr(mass), mass.stride(0), _ptr(token_positions),
+                                0 if token_positions is None else token_positions.stride(0), _ptr(moves), keep.shape[1],
+                                _ptr(move_count), _ptr(new_lens), _ptr(mass_out), _ptr(pos_out), rows, B, rows, _stream()),
+           "kb200_evict_plan")
+    _launched(1 if B and rows else 0)
+
+
+@_on_device_of(1)
+def evict_move(layers, moves, move_count, max_moves: int, num_kv_heads: int):
+    """Moves rows inside the caches of several layers (KvLayouts that share a block table, a type and strides)."""
+    lib = init(moves.get_device())
+    _want(moves, torch.int32, "moves")
+    _want(move_count, torch.int32, "move_count")
+    B, budget = moves.shape[:2]
+    if not moves.is_contiguous() or moves.shape[2:] != (2,) or move_count.shape != (B,) or not move_count.is_contiguous():
+        raise KascadeNativeError("evict_move: expected contiguous moves [B, budget, 2] and move_count [B]")
+    _same_device(moves, move_count=move_count)
+    for layer in layers:
+        _same_device(moves, **{f"cache {i}": t for i, t in enumerate(layer._keep)})
+    array = (KvLayout * len(layers))(*layers)
+    _check(lib.kb200_evict_move(array, len(layers), _ptr(moves), budget, _ptr(move_count), max_moves, B, num_kv_heads, _stream()),
+           "kb200_evict_move")
+    _launched(-(-len(layers) // 32) if B and max_moves else 0)
 
 
 @_on_device_of(0)

@@ -54,6 +54,19 @@ int check_on_current_device(const void* ptr, const char* what) {
   return 0;
 }
 
+int check_int4(const kb200_kv_layout* kv, bool need_v, const char* what) {
+  KB_REQUIRE(kv->k_param && (!need_v || kv->v_param), "%s: an INT4 cache needs k_param (and v_param): eight fp16 per row", what);
+  KB_REQUIRE(kv->act_dtype == KB200_FP16 || kv->act_dtype == KB200_BF16,
+             "%s: act_dtype of an INT4 cache (%d) must be fp16 or bf16", what, kv->act_dtype);
+  KB_REQUIRE(((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v) | (uintptr_t)kv->stride_batch |
+               (uintptr_t)kv->stride_page | (uintptr_t)kv->stride_token | (uintptr_t)kv->stride_head) & 15) == 0,
+             "%s: the codes of an INT4 cache must be 16-byte aligned, with strides that are multiples of 16 bytes", what);
+  KB_REQUIRE(((reinterpret_cast<uintptr_t>(kv->k_param) | reinterpret_cast<uintptr_t>(kv->v_param)) & 15) == 0 &&
+                 ((kv->param_stride_batch | kv->param_stride_page | kv->param_stride_token | kv->param_stride_head) & 7) == 0,
+             "%s: the parameters of an INT4 cache must be 16-byte aligned, with strides that are multiples of 8 elements", what);
+  return 0;
+}
+
 }  // namespace kb200
 
 extern "C" int kb200_abi_version(void) { return 2; }
@@ -71,7 +84,7 @@ extern "C" int kb200_init(int device) {
   KB_CUDA(cudaGetDevice(&prev));
   KB_CUDA(cudaSetDevice(device));
   int rc = 0;
-  if (kb200::init_decode() != 0 || kb200::init_prefill() != 0 || kb200::init_topk() != 0 || kb200::init_selftest() != 0) rc = -1;
+  if (kb200::init_decode() != 0 || kb200::init_decode4() != 0 || kb200::init_prefill() != 0 || kb200::init_topk() != 0 || kb200::init_selftest() != 0) rc = -1;
   if (prev != device) cudaSetDevice(prev);
   if (rc != 0) return -1;
   kb200::g_sm_count[device] = prop.multiProcessorCount;

@@ -13,6 +13,8 @@ namespace kb200 {
 void set_error(const char* fmt, ...);
 bool initialised(int* device_out);
 int check_on_current_device(const void* ptr, const char* what);
+// the parameters and strides of an INT4 cache (KB200_INT4) that a call is handed
+int check_int4(const kb200_kv_layout* kv, bool need_v, const char* what);
 
 #define KB_ENTRY(first_ptr, what)                                                                 \
   do {                                                                                            \
@@ -111,6 +113,7 @@ int sm_count();
 
 // per-module init hooks (raise dynamic shared memory limits); defined in the kernel files
 int init_decode();
+int init_decode4();
 int init_prefill();
 int init_topk();
 int init_selftest();

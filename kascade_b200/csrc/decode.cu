@@ -12,11 +12,9 @@
 // Replaces kernels/flash_decoding/reuse_kascade_gqa_decode.py:50-200 (gathered split-K decode and
 // its combine) and recompute_kascade_gqa_decode.py:49-315 (dense split-K pass with raw-score dump,
 // combine, per-KV-head pooled score).
-#include <cuda_bf16.h>
-
 #include <mutex>
 
-#include "common.cuh"
+#include "decode.cuh"
 
 namespace kb200 {
 
@@ -26,96 +24,6 @@ constexpr int kDecStages = 3;
 constexpr int kSub = 16;                                  // keys per sub-tile
 constexpr int kDecStageBytes = kSub * kD * 2 * 2;         // K + V rows of one sub-tile
 constexpr int kDecSmem = kDecWarps * kDecStages * kDecStageBytes;
-
-struct DecodeParams {
-  const __half* q;
-  int64_t q_stride_b, q_stride_h;
-  const __half* k;
-  const __half* v;
-  int64_t kv_stride_batch, kv_stride_page, kv_stride_token, kv_stride_head;
-  const int32_t* block_table;
-  int32_t block_table_stride;
-  int32_t page_shift, page_mask;
-  const int32_t* idx;            // sparse: index rows
-  int64_t idx_stride_b, idx_stride_g;
-  const int32_t* count;          // sparse: [B,G] valid entries (or NULL)
-  int32_t k_max;
-  const int32_t* head_map;       // sparse: [G] or NULL
-  const int32_t* seq_lens;       // dense: [B]
-  float scale2;                  // softmax_scale * log2(e)
-  float* logits;                 // dense: [B,H,logit_stride]
-  int64_t logit_stride;
-  __half* out;                   // [B,H,D] (written here only when num_splits == 1)
-  float* lse2;                   // [B,H]
-  float* ws_m;                   // [B,H,S]
-  float* ws_l;                   // [B,H,S]
-  float* ws_o;                   // [B,H,S,D]
-  int32_t H, G, num_splits;
-  int32_t by_length;             // the longest sequences' CTAs come first (see longest_first)
-  int32_t bf16;                  // host side: cache, q and the output are bf16, not fp16
-  // FP8 (e4m3) cache: one fp32 scale per (page, KV head) for K and for V; q and the output are fp16
-  int32_t fp8;
-  const float* k_scale;
-  const float* v_scale;
-  int64_t sc_stride_batch, sc_stride_page, sc_stride_head;
-};
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src));
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N));
-}
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void lds128(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d, uint32_t addr) {
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr));
-}
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  if (BF16) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};\n"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};\n"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  if (BF16) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-// one output element in the storage type
-template <bool BF16>
-__device__ __forceinline__ void store_half(__half* dst, float x) {
-  if (BF16) *reinterpret_cast<__nv_bfloat16*>(dst) = __float2bfloat16_rn(x);
-  else *dst = __float2half_rn(x);
-}
 
 // byte offset of 16-byte chunk `c` of row `r` inside a [16 rows x 256 B] sub-tile buffer
 __device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)(r * 256 + ((c ^ (r & 7)) << 4)); }
@@ -143,11 +51,6 @@ __device__ __forceinline__ uint32_t swz8(int r, int c) { return (uint32_t)(r * 1
 // probability before P.V.  q and the output are fp16 then.
 constexpr int kRawStage = kSub * kD * 2;                  // FP8: K + V rows of a sub-tile as stored (4 KB)
 
-__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
-  return r;
-}
 // the two 16-bit halves of a word of e4m3 bytes -> two fp16 pairs
 __device__ __forceinline__ void fp8x4_to_half2x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}\n"
@@ -460,27 +363,7 @@ __global__ void __launch_bounds__(dec_warps(KV) * 32, 1) decode_attn_kernel(cons
     }
   }
   __syncthreads();
-  for (int t = threadIdx.x; t < kHg * kD; t += WARPS * 32) {
-    const int h = t / kD, d = t % kD;
-    float M = -INFINITY;
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_m[w * kHg + h]);
-    float L = 0.f, O = 0.f;
-    for (int w = 0; w < WARPS; ++w) {
-      float mw = sm_m[w * kHg + h];
-      float f = (mw == -INFINITY) ? 0.f : exp2f(mw - M);
-      L += sm_l[w * kHg + h] * f;
-      if (HAS_V) O += sm_o[(w * kHg + h) * kD + d] * f;
-    }
-    const int64_t bh = (int64_t)b * p.H + g * kHg + h;
-    if (p.num_splits == 1) {
-      if (HAS_V) store_half<BF16>(p.out + bh * kD + d, L > 0.f ? O / L : 0.f);
-      if (d == 0 && p.lse2) p.lse2[bh] = L > 0.f ? M + log2f(L) : -INFINITY;
-    } else {
-      const int64_t slot = bh * p.num_splits + split;
-      if (HAS_V) p.ws_o[slot * kD + d] = O;
-      if (d == 0) { p.ws_m[slot] = M; p.ws_l[slot] = L; }
-    }
-  }
+  merge_warps<HAS_V, BF16>(p, sm_m, sm_l, sm_o, WARPS, b, g, split);
 }
 
 // Merge of the split partials: grid (H, B), 128 threads (one per output element).  A few hundred bytes per output row,
@@ -621,10 +504,21 @@ static int fill_kv(DecodeParams& p, const kb200_kv_layout* kv, bool need_v) {
   KB_REQUIRE(kv->stride_batch % 8 == 0 && kv->stride_page % 8 == 0 && kv->stride_token % 8 == 0 &&
                  kv->stride_head % 8 == 0,
              "decode: KV strides must be multiples of 8 elements (16 bytes)");
-  KB_REQUIRE(kv->dtype == KB200_FP16 || kv->dtype == KB200_BF16 || kv->dtype == KB200_FP8_E4M3,
+  KB_REQUIRE(kv->dtype == KB200_FP16 || kv->dtype == KB200_BF16 || kv->dtype == KB200_FP8_E4M3 || kv->dtype == KB200_INT4,
              "decode: unknown dtype code %d of the KV cache", kv->dtype);
   p.bf16 = kv->dtype == KB200_BF16;
   p.fp8 = kv->dtype == KB200_FP8_E4M3;
+  p.int4 = kv->dtype == KB200_INT4;
+  if (p.int4) {
+    if (check_int4(kv, need_v, "decode") != 0) return -1;
+    p.bf16 = kv->act_dtype == KB200_BF16;
+    p.k_param = static_cast<const __half*>(kv->k_param);
+    p.v_param = static_cast<const __half*>(kv->v_param);
+    p.pa_stride_batch = kv->param_stride_batch;
+    p.pa_stride_page = kv->param_stride_page;
+    p.pa_stride_token = kv->param_stride_token;
+    p.pa_stride_head = kv->param_stride_head;
+  }
   if (p.fp8) {
     KB_REQUIRE(kv->k_scale && (!need_v || kv->v_scale), "decode: an FP8 cache needs k_scale / v_scale");
     KB_REQUIRE(kv->stride_batch % 16 == 0 && kv->stride_page % 16 == 0 && kv->stride_token % 16 == 0 &&
@@ -774,7 +668,8 @@ extern "C" int kb200_decode_sparse_paged(const void* q, int64_t q_stride_b, int6
   cudaStream_t st = (cudaStream_t)stream;
   dim3 grid(splits, num_kv_heads, batch);
   cudaError_t rc;
-  if (p.fp8) rc = launch_attn<false, true, false, 2>(p, grid, k_max, st);
+  if (p.int4) rc = launch_attn4(p, false, true, grid, st);
+  else if (p.fp8) rc = launch_attn<false, true, false, 2>(p, grid, k_max, st);
   else if (p.bf16) rc = launch_attn<false, true, false, 1>(p, grid, k_max, st);
   else rc = launch_attn<false, true, false, 0>(p, grid, k_max, st);
   KB_LAUNCH("decode_attn_kernel<sparse>", rc);
@@ -826,7 +721,8 @@ extern "C" int kb200_decode_anchor_paged(const void* q, int64_t q_stride_b, int6
   cudaStream_t st = (cudaStream_t)stream;
   dim3 grid(splits, num_kv_heads, batch);
   cudaError_t rc;
-  if (has_v && p.fp8) rc = launch_attn<true, true, true, 2>(p, grid, max_seq_len, st);
+  if (p.int4) rc = launch_attn4(p, true, has_v, grid, st);
+  else if (has_v && p.fp8) rc = launch_attn<true, true, true, 2>(p, grid, max_seq_len, st);
   else if (has_v && p.bf16) rc = launch_attn<true, true, true, 1>(p, grid, max_seq_len, st);
   else if (has_v) rc = launch_attn<true, true, true, 0>(p, grid, max_seq_len, st);
   else if (p.fp8) rc = launch_attn<true, false, true, 2>(p, grid, max_seq_len, st);
@@ -896,7 +792,8 @@ extern "C" int kb200_decode_sparse_paged_noalloc(const void* q, int64_t q_stride
   cudaStream_t st = (cudaStream_t)stream;
   dim3 grid(splits, num_kv_heads, batch);
   cudaError_t rc;
-  if (p.fp8) rc = launch_attn<false, true, false, 2>(p, grid, k_max, st);
+  if (p.int4) rc = launch_attn4(p, false, true, grid, st);
+  else if (p.fp8) rc = launch_attn<false, true, false, 2>(p, grid, k_max, st);
   else if (p.bf16) rc = launch_attn<false, true, false, 1>(p, grid, k_max, st);
   else rc = launch_attn<false, true, false, 0>(p, grid, k_max, st);
   KB_LAUNCH("decode_attn_kernel<sparse, noalloc>", rc);

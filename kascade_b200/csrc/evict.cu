@@ -1,0 +1,294 @@
+// Eviction from a KV cache by accumulated attention weight: the weight that rows collect in prompts and decode steps, the
+// choice of the rows that stay, and the moves that bring them together.  The declarations in kascade_b200.h say what each
+// entry point computes; the reference has no counterpart.
+#include "common.cuh"
+
+namespace kb200 {
+
+// ---- weight of a decode step ---------------------------------------------------------------------------------------
+// Four rows per thread, the heads one after the other: bound by the pooled scores' way out of L2, where the pooling kernel has
+// just put them.
+__global__ void __launch_bounds__(128) mass_add_kernel(const float* pooled, int64_t row_stride, const int32_t* seq_lens,
+                                                       const float* mass_in, float* mass_out, int64_t mass_stride, int G,
+                                                       int max_len) {
+  pdl_begin();
+  const int b = blockIdx.y, n = min(seq_lens[b], max_len);
+  const int j = (blockIdx.x * 128 + threadIdx.x) * 4;
+  if (j >= n) return;
+  const float* src = pooled + (int64_t)b * G * row_stride + j;
+  float4 a = *reinterpret_cast<const float4*>(src);
+  for (int g = 1; g < G; ++g) {
+    const float4 x = *reinterpret_cast<const float4*>(src + g * row_stride);   // (row_stride is a multiple of 4: readable)
+    a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+  }
+  const float s[4] = {a.x, a.y, a.z, a.w};
+  for (int e = 0; e < 4 && j + e < n; ++e) mass_out[b * mass_stride + j + e] = mass_in[b * mass_stride + j + e] + s[e];
+}
+
+// ---- weight of a prompt ----------------------------------------------------------------------------------------------
+struct PromptMassParams {
+  const float* pooled; int64_t row_stride;
+  const int32_t* seq_len;
+  const float* mass_in; float* mass_out; int64_t in_stride, out_stride;
+  int G, T, n_rows;
+};
+
+// One column of four rows per thread, over all heads and tiles.
+__global__ void __launch_bounds__(64) mass_prompt_kernel(const PromptMassParams p) {
+  pdl_begin();
+  const int b = blockIdx.y, j = (blockIdx.x * 64 + threadIdx.x) * 4;
+  if (j >= p.n_rows) return;
+  const int tiles = p.seq_len ? min((max(p.seq_len[b], 0) + kTile - 1) / kTile, p.T) : p.T;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int t = j / kTile + 1; t < tiles; ++t) {                   // j is a multiple of 4: its four rows lie in one tile
+    for (int g = 0; g < p.G; ++g) {
+      const float4 x = *reinterpret_cast<const float4*>(p.pooled + (((int64_t)b * p.G + g) * p.T + t) * p.row_stride + j);
+      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    }
+  }
+  const float s[4] = {a.x, a.y, a.z, a.w};
+  for (int e = 0; e < 4 && j + e < p.n_rows; ++e)
+    p.mass_out[b * p.out_stride + j + e] = p.mass_in[b * p.in_stride + j + e] + s[e];
+}
+
+// ---- what stays ------------------------------------------------------------------------------------------------------
+// One CTA per sequence: the newest position, then the keys.
+__global__ void __launch_bounds__(1024) evict_keys_kernel(const float* mass, int64_t mass_stride, const int32_t* seq_lens,
+                                                          const int32_t* positions, int64_t pos_stride, int sinks, int recent,
+                                                          float* keys, int64_t key_stride, int n_rows) {
+  pdl_begin();
+  __shared__ int newest_of[32];
+  const int b = blockIdx.x, n = min(seq_lens[b], n_rows), tid = threadIdx.x;
+  int newest = -1;
+  if (positions) {
+    for (int j = tid; j < n; j += 1024) newest = max(newest, positions[b * pos_stride + j]);
+    newest = __reduce_max_sync(0xFFFFFFFFu, newest);
+    if ((tid & 31) == 0) newest_of[tid >> 5] = newest;
+    __syncthreads();
+    newest = __reduce_max_sync(0xFFFFFFFFu, newest_of[tid & 31]);
+  } else {
+    newest = n - 1;
+  }
+  for (int j = tid; j < n; j += 1024) {
+    const int pos = positions ? positions[b * pos_stride + j] : j;
+    const float m = mass[b * mass_stride + j];
+    keys[b * key_stride + j] = pos < sinks || (int64_t)pos > (int64_t)newest - recent ? INFINITY : m == m ? m : 0.f;
+  }
+}
+
+struct EvictPlanParams {
+  const int32_t* keep; int64_t keep_stride; const int32_t* keep_count;
+  const float* mass_in; int64_t mass_stride;
+  const int32_t* pos_in; int64_t pos_stride;
+  int2* moves; int64_t move_stride; int32_t* move_count; int32_t* new_lens;
+  float* mass_out; int32_t* pos_out; int64_t out_stride;
+  int n_rows;
+};
+
+// the first place of the ascending list a[0..n) whose value is not below x
+__device__ __forceinline__ int lower_bound(const int32_t* a, int n, int x) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] < x) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A thread per row i.  With the kept rows ascending, r = rank of i among them says whether i is kept (keep[r] == i); if it is
+// not, i - r rows below it are let go too, so it takes the (i - r)-th of the kept rows that lie behind the new length.
+__global__ void __launch_bounds__(256) evict_plan_kernel(const EvictPlanParams p) {
+  pdl_begin();
+  const int b = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.n_rows) return;
+  const int left = p.keep_count[b];
+  const int32_t* keep = p.keep + b * p.keep_stride;
+  const int stay = lower_bound(keep, left, left);                  // kept rows below the new length
+  if (i == 0) {
+    p.new_lens[b] = left;
+    p.move_count[b] = left - stay;
+  }
+  float mass = 0.f;
+  int pos = -1;
+  if (i < left) {
+    const int r = lower_bound(keep, stay, i);
+    int from = i;
+    if (r >= stay || keep[r] != i) {
+      from = keep[stay + i - r];
+      p.moves[b * p.move_stride + i - r] = make_int2(from, i);
+    }
+    mass = p.mass_in[b * p.mass_stride + from];
+    pos = p.pos_in ? p.pos_in[b * p.pos_stride + from] : from;
+  }
+  p.mass_out[b * p.out_stride + i] = mass;
+  if (p.pos_out) p.pos_out[b * p.out_stride + i] = pos;
+}
+
+// ---- the moves -------------------------------------------------------------------------------------------------------
+constexpr int kMoveLayers = 32;                                    // layers of one launch (the parameters have to hold their addresses)
+struct EvictMoveParams {
+  uint8_t* k[kMoveLayers]; uint8_t* v[kMoveLayers];               // codes or 16-bit rows
+  uint8_t* kp[kMoveLayers]; uint8_t* vp[kMoveLayers];             // parameters of an INT4 cache
+  int64_t sb, sp, st, sh;                                          // bytes
+  int64_t pb, pp, pt, ph;
+  const int32_t* block_table; int bt_stride, page_shift, page_mask;
+  const int2* moves; int64_t move_stride; const int32_t* move_count;
+  int G, row_chunks;                                               // 16-byte pieces of a row: 16, or 4 of an INT4 cache
+};
+
+// One warp per move and layer, 16 bytes per lane and step.
+__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ EvictMoveParams p) {
+  pdl_begin();
+  const int b = blockIdx.z, layer = blockIdx.y, lane = threadIdx.x & 31;
+  const int j = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (j >= p.move_count[b]) return;
+  const int2 move = p.moves[b * p.move_stride + j];
+  int64_t page[2], slot[2];
+  const int rows[2] = {move.x, move.y};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int lp = rows[e] >> p.page_shift;
+    slot[e] = rows[e] & p.page_mask;
+    page[e] = p.block_table ? p.block_table[(int64_t)b * p.bt_stride + lp] : lp;
+  }
+  for (int what = 0; what < (p.kp[layer] ? 4 : 2); ++what) {
+    const bool par = what >= 2;
+    uint8_t* base = what == 0 ? p.k[layer] : what == 1 ? p.v[layer] : what == 2 ? p.kp[layer] : p.vp[layer];
+    const int64_t from = b * (par ? p.pb : p.sb) + page[0] * (par ? p.pp : p.sp) + slot[0] * (par ? p.pt : p.st);
+    const int64_t to = b * (par ? p.pb : p.sb) + page[1] * (par ? p.pp : p.sp) + slot[1] * (par ? p.pt : p.st);
+    const int chunks = par ? 1 : p.row_chunks;
+    for (int c = lane; c < p.G * chunks; c += 32) {
+      const int64_t at = (c / chunks) * (par ? p.ph : p.sh) + (c % chunks) * 16;
+      *reinterpret_cast<uint4*>(base + to + at) = *reinterpret_cast<const uint4*>(base + from + at);
+    }
+  }
+}
+
+}  // namespace kb200
+
+extern "C" int kb200_mass_add(const float* pooled, int64_t row_stride, const int32_t* seq_lens, const float* mass_in,
+                              float* mass_out, int64_t mass_stride, int batch, int num_kv_heads, int max_len, void* stream) {
+  using namespace kb200;
+  KB_ENTRY(pooled, "mass_add: pooled");
+  KB_REQUIRE(pooled && seq_lens && mass_in && mass_out, "mass_add: null pointer");
+  KB_REQUIRE(batch >= 0 && batch <= 65535 && num_kv_heads > 0 && max_len >= 0, "mass_add: bad sizes");
+  KB_REQUIRE(row_stride % 4 == 0 && row_stride >= max_len && (reinterpret_cast<uintptr_t>(pooled) & 15) == 0,
+             "mass_add: pooled rows must be 16-byte aligned (row_stride %% 4 == 0) and hold max_len (%d) scores", max_len);
+  KB_REQUIRE(mass_stride >= max_len, "mass_add: mass holds %lld rows, %d are needed", (long long)mass_stride, max_len);
+  if (batch == 0 || max_len == 0) return 0;
+  KB_LAUNCH("mass_add_kernel", launch_pdl(mass_add_kernel, dim3(ceil_div(max_len, 512), batch), 128, 0, (cudaStream_t)stream, 1,
+                                          pooled, row_stride, seq_lens, mass_in, mass_out, mass_stride, num_kv_heads, max_len));
+  return 0;
+}
+
+extern "C" int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t* seq_len, const float* mass_in,
+                                     float* mass_out, int64_t mass_in_stride, int64_t mass_out_stride, int batch,
+                                     int num_kv_heads, int num_tiles, int n_rows, void* stream) {
+  using namespace kb200;
+  KB_ENTRY(pooled, "mass_add_prompt: pooled");
+  KB_REQUIRE(pooled && mass_in && mass_out, "mass_add_prompt: null pointer");
+  KB_REQUIRE(batch >= 0 && batch <= 65535 && num_kv_heads > 0 && num_tiles >= 0 && n_rows >= 0, "mass_add_prompt: bad sizes");
+  const int64_t need = num_tiles > 0 ? (int64_t)(num_tiles - 1) * kTile : 0;
+  KB_REQUIRE(row_stride % 4 == 0 && row_stride >= need && (reinterpret_cast<uintptr_t>(pooled) & 15) == 0,
+             "mass_add_prompt: pooled rows must be 16-byte aligned (row_stride %% 4 == 0) and hold %lld scores", (long long)need);
+  KB_REQUIRE(n_rows >= need, "mass_add_prompt: mass holds %d rows, %d tiles need %lld", n_rows, num_tiles, (long long)need);
+  if (batch == 0 || n_rows == 0) return 0;
+  PromptMassParams p{pooled, row_stride, seq_len, mass_in, mass_out, mass_in_stride, mass_out_stride, num_kv_heads, num_tiles, n_rows};
+  KB_LAUNCH("mass_prompt_kernel",
+            launch_pdl(mass_prompt_kernel, dim3(ceil_div(n_rows, 256), batch), 64, 0, (cudaStream_t)stream, 1, p));
+  return 0;
+}
+
+extern "C" int kb200_evict_keys(const float* mass, int64_t mass_stride, const int32_t* seq_lens,
+                                const int32_t* token_positions, int64_t pos_stride, int sinks, int recent, float* keys,
+                                int64_t key_stride, int batch, int n_rows, void* stream) {
+  using namespace kb200;
+  KB_ENTRY(mass, "evict_keys: mass");
+  KB_REQUIRE(mass && seq_lens && keys, "evict_keys: null pointer");
+  KB_REQUIRE(batch >= 0 && n_rows >= 0 && sinks >= 0 && recent >= 0, "evict_keys: negative size");
+  KB_REQUIRE(key_stride >= n_rows, "evict_keys: keys hold %lld rows, %d are needed", (long long)key_stride, n_rows);
+  if (batch == 0 || n_rows == 0) return 0;
+  KB_LAUNCH("evict_keys_kernel", launch_pdl(evict_keys_kernel, dim3(batch), 1024, 0, (cudaStream_t)stream, 1, mass, mass_stride,
+                                            seq_lens, token_positions, pos_stride, sinks, recent, keys, key_stride, n_rows));
+  return 0;
+}
+
+extern "C" int kb200_evict_plan(const int32_t* keep, int64_t keep_stride, const int32_t* keep_count,
+                                const float* mass_in, int64_t mass_stride, const int32_t* pos_in, int64_t pos_stride,
+                                int32_t* moves, int64_t move_stride, int32_t* move_count, int32_t* new_lens, float* mass_out,
+                                int32_t* pos_out, int64_t out_stride, int batch, int n_rows, void* stream) {
+  using namespace kb200;
+  KB_ENTRY(keep, "evict_plan: keep");
+  KB_REQUIRE(keep && keep_count && mass_in && moves && move_count && new_lens && mass_out, "evict_plan: null pointer");
+  KB_REQUIRE(batch >= 0 && batch <= 65535 && n_rows >= 0 && out_stride >= n_rows, "evict_plan: bad sizes");
+  KB_REQUIRE((reinterpret_cast<uintptr_t>(moves) & 7) == 0, "evict_plan: moves must be 8-byte aligned");
+  KB_REQUIRE(move_stride >= keep_stride || move_stride >= n_rows, "evict_plan: %lld moves per sequence may not hold them all",
+             (long long)move_stride);
+  KB_REQUIRE(mass_out != mass_in && (!pos_out || pos_out != pos_in), "evict_plan: an output is its own input");
+  if (batch == 0 || n_rows == 0) return 0;
+  EvictPlanParams p{keep, keep_stride, keep_count, mass_in, mass_stride, pos_in, pos_stride,
+                    reinterpret_cast<int2*>(moves), move_stride, move_count, new_lens, mass_out, pos_out, out_stride, n_rows};
+  KB_LAUNCH("evict_plan_kernel",
+            launch_pdl(evict_plan_kernel, dim3(ceil_div(n_rows, 256), batch), 256, 0, (cudaStream_t)stream, 1, p));
+  return 0;
+}
+
+extern "C" int kb200_evict_move(const kb200_kv_layout* layers, int n_layers, const int32_t* moves, int64_t move_stride,
+                                const int32_t* move_count, int max_moves, int batch, int num_kv_heads, void* stream) {
+  using namespace kb200;
+  KB_REQUIRE(layers && moves && move_count, "evict_move: null pointer");
+  KB_REQUIRE(n_layers >= 0 && max_moves >= 0 && batch >= 0 && batch <= 65535 && num_kv_heads > 0, "evict_move: bad sizes");
+  KB_REQUIRE((reinterpret_cast<uintptr_t>(moves) & 7) == 0, "evict_move: moves must be 8-byte aligned");
+  KB_ENTRY(moves, "evict_move: moves");
+  if (n_layers == 0 || max_moves == 0 || batch == 0) return 0;
+  const kb200_kv_layout& one = layers[0];
+  const bool int4 = one.dtype == KB200_INT4;
+  KB_REQUIRE(one.dtype == KB200_FP16 || one.dtype == KB200_BF16 || int4,
+             "evict_move: fp16, bf16 or INT4 caches (dtype code %d): an FP8 row is stored in the scale of its page and cannot leave it",
+             one.dtype);
+  KB_REQUIRE(one.page_size >= 1 && (one.page_size & (one.page_size - 1)) == 0,
+             "evict_move: page_size must be a power of two (got %d)", one.page_size);
+  for (int i = 0; i < n_layers; ++i) {
+    const kb200_kv_layout& l = layers[i];
+    KB_REQUIRE(l.k && l.v, "evict_move: null cache of layer %d", i);
+    KB_REQUIRE(l.dtype == one.dtype && l.page_size == one.page_size && l.block_table == one.block_table &&
+                   l.block_table_stride == one.block_table_stride && l.stride_batch == one.stride_batch &&
+                   l.stride_page == one.stride_page && l.stride_token == one.stride_token && l.stride_head == one.stride_head &&
+                   (!int4 || (l.param_stride_batch == one.param_stride_batch && l.param_stride_page == one.param_stride_page &&
+                              l.param_stride_token == one.param_stride_token && l.param_stride_head == one.param_stride_head)),
+               "evict_move: layer %d has another type, block table or strides than layer 0", i);
+    KB_REQUIRE(((reinterpret_cast<uintptr_t>(l.k) | reinterpret_cast<uintptr_t>(l.v)) & 15) == 0 &&
+                   ((l.stride_batch | l.stride_page | l.stride_token | l.stride_head) & (int4 ? 15 : 7)) == 0,
+               "evict_move: caches must be 16-byte aligned, with strides that are multiples of 16 bytes");
+    if (int4 && check_int4(&l, true, "evict_move") != 0) return -1;
+  }
+  EvictMoveParams p{};
+  const int64_t unit = int4 ? 1 : 2;
+  p.sb = one.stride_batch * unit; p.sp = one.stride_page * unit; p.st = one.stride_token * unit; p.sh = one.stride_head * unit;
+  p.pb = one.param_stride_batch * 2; p.pp = one.param_stride_page * 2; p.pt = one.param_stride_token * 2; p.ph = one.param_stride_head * 2;
+  p.block_table = one.block_table;
+  p.bt_stride = one.block_table_stride;
+  int shift = 0;
+  while ((1 << shift) < one.page_size) ++shift;
+  p.page_shift = shift;
+  p.page_mask = one.page_size - 1;
+  p.moves = reinterpret_cast<const int2*>(moves);
+  p.move_stride = move_stride;
+  p.move_count = move_count;
+  p.G = num_kv_heads;
+  p.row_chunks = int4 ? kD / 2 / 16 : kD * 2 / 16;
+  for (int first = 0; first < n_layers; first += kMoveLayers) {
+    const int n = n_layers - first < kMoveLayers ? n_layers - first : kMoveLayers;
+    for (int i = 0; i < n; ++i) {
+      const kb200_kv_layout& l = layers[first + i];
+      p.k[i] = static_cast<uint8_t*>(const_cast<void*>(l.k));
+      p.v[i] = static_cast<uint8_t*>(const_cast<void*>(l.v));
+      p.kp[i] = int4 ? static_cast<uint8_t*>(const_cast<void*>(l.k_param)) : nullptr;
+      p.vp[i] = int4 ? static_cast<uint8_t*>(const_cast<void*>(l.v_param)) : nullptr;
+    }
+    KB_LAUNCH("evict_move_kernel",
+              launch_pdl(evict_move_kernel, dim3(ceil_div(max_moves, 8), n, batch), 256, 0, (cudaStream_t)stream, 1, p));
+  }
+  return 0;
+}

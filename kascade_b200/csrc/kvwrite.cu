@@ -12,7 +12,14 @@
 // in fp32 from position * inv_freq[i] (the model's own inverse-frequency table, so every rope-scaling
 // variant is covered), scaled and rounded to that type, and  x * cos + rotate_half(x) * sin  is evaluated
 // in that type with a rounding after each product and after the sum (apply_rotary_pos_emb).
+//
+// Tokens with positions of their own (kb200_kv_write_at) are not the modules' arithmetic repeated: a cache that rows have
+// left, or images and video with several axes, continue at positions far beyond the cache, where an angle formed in fp32 is
+// off by up to pos 2^-24 and each rounding to bf16 costs as much again.  There the angle is formed and reduced in 64 bits
+// (a few instructions of 64 of the threads of a CTA), norm and rotation are computed in fp32 and rounded once.
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -32,6 +39,12 @@ struct KvWriteParams {
   const float* k_scale; const float* v_scale; int64_t s_sb, s_sp, s_sh;
   const float* inv_freq; float rope_scale;                            // [D/2] inverse frequencies or null (no rotary)
   int B, T, H, G;
+  // INT4 cache: codes behind k_cache / v_cache (strides of the cache in bytes), eight fp16 parameters per row
+  __half* k_param; __half* v_param; int64_t pa_sb, pa_sp, pa_st, pa_sh;
+  // positions of their own: [axes, B, T], the axis of every rotary pair [D/2] or null (the first), and where the position on
+  // the first axis is noted per cache row, [B, rows], or null
+  const int32_t* positions; int64_t ps_axis, ps_b; const int32_t* pair_axis; int axes;
+  int32_t* token_positions; int64_t tp_sb; int tp_rows;
 };
 
 // One CTA per (sequence, new token): the token's 64 (cos, sin) pairs are computed once and shared by all
@@ -71,11 +84,53 @@ __device__ __forceinline__ uint2 quantize8(const H2* x, float scale) {
   return make_uint2(w[0], w[1]);
 }
 
+// The 4-bit form of a row.  Called by the eight lanes of the row together, whose values are x[0..7] = 8c .. 8c+7 (group c / 4)
+// and x[8..15] = 64+8c .. 64+8c+7 (group 2 + c / 4), so a group lies in four lanes:
+//   z = fp16(min), s = fp16((max - z) / 15), c = round((x - z) / s) clamped to 0..15 (half to even, decided exactly).
+// What fp16 cannot hold saturates; a group with a value that is not finite gets z = NaN.  par[0..1]: scales of the two groups,
+// par[2..3]: zeros; words: the eight codes of this lane in either group, the lowest nibble first.
+__device__ __forceinline__ void quantize_int4(const float (&x)[16], uint32_t (&words)[2], __half (&par)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float mn = INFINITY, mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = x[i * 8 + e];
+      mn = fminf(mn, v);
+      mx = fabsf(v) < INFINITY ? fmaxf(mx, v) : INFINITY;                    // (also where v is a NaN)
+    }
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      mn = fminf(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, o));
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    }
+    const __half zh = __float2half_rn(mx == INFINITY ? NAN : fminf(fmaxf(mn, -65504.f), 65504.f));
+    const float z = __half2float(zh);
+    const __half sh = mx == INFINITY ? __float2half_rn(0.f) : __float2half_rn(fminf(fmaxf(__fdiv_rn(mx - z, 15.f), 0.f), 65504.f));
+    const float s = __half2float(sh), inv = s > 0.f ? 1.f / s : 0.f;
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = x[i * 8 + e] - z;
+      float c = rintf(a * inv);
+      const float rest = fmaf(-c, s, a);                                    // the product alone may be on the wrong side
+      if (s > 0.f && (fabsf(rest) > 0.5f * s || (fabsf(rest) == 0.5f * s && ((int)c & 1)))) c += copysignf(1.f, rest);
+      w |= (uint32_t)(int)fminf(fmaxf(c, 0.f), 15.f) << (4 * e);             // (a NaN becomes 0)
+    }
+    words[i] = w;
+    par[i] = sh;
+    par[2 + i] = zh;
+  }
+}
+
+// How a row is stored, and whether its token has a position of its own (kb200_kv_write_at)
+constexpr int kSame = 0, kFp8 = 1, kInt4 = 2;
+
 // CTAS: CTAs per SM that the registers have to allow (0: left to the compiler); see launch_kv_write
-template <bool BF16, bool FP8, int CTAS>
+template <bool BF16, int STORE, bool AT, int CTAS>
 __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const KvWriteParams p) {
   using H2 = typename Pair<BF16>::T;
-  using H1 = typename Pair<BF16>::S;
+  using H1 = typename std::conditional<AT, float, typename Pair<BF16>::S>::type;
   __shared__ __align__(16) H1 cos_s[kD / 2];
   __shared__ __align__(16) H1 sin_s[kD / 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -98,11 +153,26 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
   uint4 next_lo = make_uint4(0u, 0u, 0u, 0u), next_hi = next_lo;
   if (warp * 4 < heads) load_rows(warp * 4, next_lo, next_hi);
   const int pos = p.start_pos[b] + t;
-  if (p.inv_freq && tid < kD / 2) {
-    float sn, cs;
-    sincosf((float)pos * p.inv_freq[tid], &sn, &cs);
-    cos_s[tid] = from_f<BF16>(cs * p.rope_scale);
-    sin_s[tid] = from_f<BF16>(sn * p.rope_scale);
+  if constexpr (AT) {
+    const int32_t* own_pos = p.positions + b * p.ps_b + t;
+    if (p.inv_freq && tid < kD / 2) {
+      const int axis = p.pair_axis ? min(max(p.pair_axis[tid], 0), p.axes - 1) : 0;
+      constexpr double kTurn = 6.283185307179586476925;
+      double angle = (double)own_pos[axis * p.ps_axis] * (double)p.inv_freq[tid];
+      angle -= rint(angle * (1.0 / kTurn)) * kTurn;
+      float sn, cs;
+      sincosf((float)angle, &sn, &cs);
+      cos_s[tid] = cs * p.rope_scale;
+      sin_s[tid] = sn * p.rope_scale;
+    }
+    if (tid == 0 && p.token_positions && pos < p.tp_rows) p.token_positions[b * p.tp_sb + pos] = own_pos[0];
+  } else {
+    if (p.inv_freq && tid < kD / 2) {
+      float sn, cs;
+      sincosf((float)pos * p.inv_freq[tid], &sn, &cs);
+      cos_s[tid] = from_f<BF16>(cs * p.rope_scale);
+      sin_s[tid] = from_f<BF16>(sn * p.rope_scale);
+    }
   }
   __syncthreads();
   for (int h0 = warp * 4; h0 < heads; h0 += kStep) {                 // uniform per warp
@@ -124,42 +194,94 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
     }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-    if (gain) {
-      // x.float() * rsqrt(mean(x^2) + eps), rounded to the storage type, times the gain (a product in that type)
-      const float r = rsqrtf(ss / kD + p.eps);
-      const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
-      const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
-      const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
-      const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
+    float x[16];                                                     // AT, INT4: the row in fp32
+    if constexpr (AT) {
+      const float r = gain ? rsqrtf(ss / kD + p.eps) : 1.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
-        lo[e] = __hmul2_rn(g_lo[e], from_f2<BF16>(a.x * r, a.y * r));
-        hi[e] = __hmul2_rn(g_hi[e], from_f2<BF16>(d2.x * r, d2.y * r));
+        x[2 * e] = a.x * r; x[2 * e + 1] = a.y * r;
+        x[8 + 2 * e] = d2.x * r; x[8 + 2 * e + 1] = d2.y * r;
       }
-    }
-    if (kind != 2 && p.inv_freq) {
-      const uint4 cs4 = reinterpret_cast<const uint4*>(cos_s)[c];
-      const uint4 sn4 = reinterpret_cast<const uint4*>(sin_s)[c];
-      const H2* cs = reinterpret_cast<const H2*>(&cs4);
-      const H2* sn = reinterpret_cast<const H2*>(&sn4);
+      if (gain) {
+        const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
+        const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
+        const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
+        const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // first half:  x_lo * cos + (-x_hi) * sin ; second half:  x_hi * cos + x_lo * sin
-        // (the _rn forms are never contracted into a fused multiply-add, which would skip a rounding)
-        const H2 new_lo = __hadd2_rn(__hmul2_rn(lo[e], cs[e]), __hmul2_rn(__hneg2(hi[e]), sn[e]));
-        const H2 new_hi = __hadd2_rn(__hmul2_rn(hi[e], cs[e]), __hmul2_rn(lo[e], sn[e]));
-        lo[e] = new_lo;
-        hi[e] = new_hi;
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = to_f2(g_lo[e]), d2 = to_f2(g_hi[e]);
+          x[2 * e] *= a.x; x[2 * e + 1] *= a.y;
+          x[8 + 2 * e] *= d2.x; x[8 + 2 * e + 1] *= d2.y;
+        }
+      }
+      if (kind != 2 && p.inv_freq) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float cs = cos_s[c * 8 + e], sn = sin_s[c * 8 + e], l = x[e], h2 = x[8 + e];
+          x[e] = l * cs - h2 * sn;
+          x[8 + e] = h2 * cs + l * sn;
+        }
+      }
+      if (STORE != kInt4 || kind == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = from_f2<BF16>(x[2 * e], x[2 * e + 1]);
+          hi[e] = from_f2<BF16>(x[8 + 2 * e], x[8 + 2 * e + 1]);
+        }
+      }
+    } else {
+      if (gain) {
+        // x.float() * rsqrt(mean(x^2) + eps), rounded to the storage type, times the gain (a product in that type)
+        const float r = rsqrtf(ss / kD + p.eps);
+        const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
+        const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
+        const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
+        const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
+          lo[e] = __hmul2_rn(g_lo[e], from_f2<BF16>(a.x * r, a.y * r));
+          hi[e] = __hmul2_rn(g_hi[e], from_f2<BF16>(d2.x * r, d2.y * r));
+        }
+      }
+      if (kind != 2 && p.inv_freq) {
+        const uint4 cs4 = reinterpret_cast<const uint4*>(cos_s)[c];
+        const uint4 sn4 = reinterpret_cast<const uint4*>(sin_s)[c];
+        const H2* cs = reinterpret_cast<const H2*>(&cs4);
+        const H2* sn = reinterpret_cast<const H2*>(&sn4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // first half:  x_lo * cos + (-x_hi) * sin ; second half:  x_hi * cos + x_lo * sin
+          // (the _rn forms are never contracted into a fused multiply-add, which would skip a rounding)
+          const H2 new_lo = __hadd2_rn(__hmul2_rn(lo[e], cs[e]), __hmul2_rn(__hneg2(hi[e]), sn[e]));
+          const H2 new_hi = __hadd2_rn(__hmul2_rn(hi[e], cs[e]), __hmul2_rn(lo[e], sn[e]));
+          lo[e] = new_lo;
+          hi[e] = new_hi;
+        }
       }
     }
-    __half* dst;
+    __half* dst = nullptr;
+    bool code_rows = false;                                          // this lane's row goes to an INT4 cache
+    int64_t row4 = 0, par4 = 0;
     if (kind == 0) {
       dst = p.q_out + (((int64_t)b * p.T + t) * p.H + hh) * kD;
     } else {
       const int page = pos >> p.page_shift, slot = pos & p.page_mask;
       const int64_t phys = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + page] : page;
-      if (FP8) {
+      if constexpr (STORE == kInt4) {
+        if constexpr (!AT) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
+            x[2 * e] = a.x; x[2 * e + 1] = a.y;
+            x[8 + 2 * e] = d2.x; x[8 + 2 * e + 1] = d2.y;
+          }
+        }
+        code_rows = true;
+        row4 = phys * p.c_sp + slot * p.c_st + hh * p.c_sh + b * p.c_sb;
+        par4 = phys * p.pa_sp + slot * p.pa_st + hh * p.pa_sh + b * p.pa_sb;
+      } else if constexpr (STORE == kFp8) {
         if (active) {
           const float sc = (kind == 1 ? p.k_scale : p.v_scale)[b * p.s_sb + phys * p.s_sp + hh * p.s_sh];
           uint8_t* d8 = reinterpret_cast<uint8_t*>(kind == 1 ? p.k_cache : p.v_cache) + b * p.c_sb + phys * p.c_sp +
@@ -169,9 +291,35 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
         }
         continue;
       }
-      dst = (kind == 1 ? p.k_cache : p.v_cache) + b * p.c_sb + phys * p.c_sp + slot * p.c_st + hh * p.c_sh;
+      if constexpr (STORE != kInt4) dst = (kind == 1 ? p.k_cache : p.v_cache) + b * p.c_sb + phys * p.c_sp + slot * p.c_st + hh * p.c_sh;
     }
-    if (active) {
+    if constexpr (STORE == kInt4) {
+      // all lanes of the warp take part in the shuffles; rows of Q among them come to nothing
+      uint32_t words[2];
+      __half par[4];
+      quantize_int4(x, words, par);
+      if (code_rows && active) {
+        const int g = c >> 2, q = c & 3;                             // groups g and g + 2, values 8q .. 8q+7 of either
+        if (kind == 1) {
+          uint8_t* row = reinterpret_cast<uint8_t*>(p.k_cache) + row4;
+          *reinterpret_cast<uint32_t*>(row + q * 16 + g * 4) = words[0];
+          *reinterpret_cast<uint32_t*>(row + q * 16 + (g + 2) * 4) = words[1];
+        } else {
+          uint8_t* row = reinterpret_cast<uint8_t*>(p.v_cache) + row4;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            *reinterpret_cast<uint16_t*>(row + (2 * q) * 8 + (g + 2 * i) * 2) = (uint16_t)words[i];
+            *reinterpret_cast<uint16_t*>(row + (2 * q + 1) * 8 + (g + 2 * i) * 2) = (uint16_t)(words[i] >> 16);
+          }
+        }
+        if (q == 0) {
+          __half* pr = (kind == 1 ? p.k_param : p.v_param) + par4;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) { pr[g + 2 * i] = par[i]; pr[4 + g + 2 * i] = par[2 + i]; }
+        }
+      }
+    }
+    if (active && !code_rows) {
       reinterpret_cast<uint4*>(dst)[c] = lo4;
       reinterpret_cast<uint4*>(dst + kD / 2)[c] = hi4;
     }
@@ -183,31 +331,94 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
 // hold the missing CTA costs time: those are compiled for seven per SM.  Measured before the loads ahead / with them /
 // as it is now, us without Q, with and without rotary table: 32768 tokens 61.0 / 66.5 / 58.3, 56.0 / 63.2 / 54.3; 16 x 600
 // 20.7 / 22.0 / 19.2, 19.2 / 21.2 / 18.2; 64 tokens 2.45 / 2.51 / 2.51, 2.26 / 2.26 / 2.26.
-template <bool BF16, bool FP8>
+template <bool BF16, int STORE>
 static void launch_kv_write(const KvWriteParams& p, int64_t blocks, cudaStream_t st) {
-  if (p.H + 2 * p.G <= kKvWriteThreads / 32 * 4 && blocks > 6ll * sm_count())
-    kv_write_kernel<BF16, FP8, 7><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
+  if (p.positions)
+    kv_write_kernel<BF16, STORE, true, 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
+  else if (STORE != kInt4 && p.H + 2 * p.G <= kKvWriteThreads / 32 * 4 && blocks > 6ll * sm_count())
+    kv_write_kernel<BF16, STORE, false, STORE != kInt4 ? 7 : 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
   else
-    kv_write_kernel<BF16, FP8, 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
+    kv_write_kernel<BF16, STORE, false, 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
+}
+
+// Rows of a 4-bit cache in 16 bits: eight lanes per row, lane c the values 8c .. 8c+7 and 64+8c .. 64+8c+7 of K and of V.
+struct KvReadParams {
+  const uint8_t* k; const uint8_t* v; int64_t c_sb, c_sp, c_st, c_sh;
+  const __half* k_param; const __half* v_param; int64_t pa_sb, pa_sp, pa_st, pa_sh;
+  const int32_t* block_table; int bt_stride; int page_shift, page_mask;
+  const int32_t* seq_lens;
+  __half* k_out; __half* v_out;                                       // [B, T, G, D]
+  int T, G; int64_t rows;
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint4 from_codes(uint32_t w, float s, float z) {
+  using H2 = typename Pair<BF16>::T;
+  H2 out[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    out[e] = from_f2<BF16>(fmaf((float)((w >> (8 * e)) & 15u), s, z), fmaf((float)((w >> (8 * e + 4)) & 15u), s, z));
+  return *reinterpret_cast<uint4*>(out);
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
+  const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int c = threadIdx.x & 7, g4 = c >> 2, q = c & 3;
+  if (row >= p.rows) return;
+  const int head = (int)(row % p.G);
+  const int64_t token = row / p.G;
+  const int b = (int)(token / p.T), t = (int)(token - (int64_t)b * p.T);
+  uint4 kl = make_uint4(0u, 0u, 0u, 0u), kh = kl, vl = kl, vh = kl;     // rows behind a sequence read as zeros
+  if (t < p.seq_lens[b]) {
+    const int lp = t >> p.page_shift, slot = t & p.page_mask;
+    const int64_t page = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + lp] : lp;
+    const int64_t at = b * p.c_sb + page * p.c_sp + slot * p.c_st + head * p.c_sh;
+    const int64_t pa = b * p.pa_sb + page * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
+    const __half* kp = p.k_param + pa;
+    const __half* vp = p.v_param + pa;
+    const uint32_t* kw = reinterpret_cast<const uint32_t*>(p.k + at);
+    const uint16_t* vw = reinterpret_cast<const uint16_t*>(p.v + at);
+    auto v_word = [&](int g) { return (uint32_t)vw[2 * q * 4 + g] | ((uint32_t)vw[(2 * q + 1) * 4 + g] << 16); };
+    kl = from_codes<BF16>(kw[q * 4 + g4], __half2float(kp[g4]), __half2float(kp[4 + g4]));
+    kh = from_codes<BF16>(kw[q * 4 + g4 + 2], __half2float(kp[g4 + 2]), __half2float(kp[6 + g4]));
+    vl = from_codes<BF16>(v_word(g4), __half2float(vp[g4]), __half2float(vp[4 + g4]));
+    vh = from_codes<BF16>(v_word(g4 + 2), __half2float(vp[g4 + 2]), __half2float(vp[6 + g4]));
+  }
+  uint4* ko = reinterpret_cast<uint4*>(p.k_out + row * kD);
+  uint4* vo = reinterpret_cast<uint4*>(p.v_out + row * kD);
+  ko[c] = kl;
+  ko[c + 8] = kh;
+  vo[c] = vl;
+  vo[c + 8] = vh;
 }
 
 }  // namespace kb200
 
-extern "C" int kb200_kv_write(const kb200_act_layout* q_in, void* q_out, const kb200_act_layout* k_new,
-                              const kb200_act_layout* v_new, const int32_t* start_pos, const int32_t* n_new,
-                              const kb200_kv_layout* kv, const void* q_norm_gain, const void* k_norm_gain,
-                              float norm_eps, const float* inv_freq, float rope_scale, int batch, int max_new,
-                              int num_q_heads, int num_kv_heads, void* stream) {
+static int kv_write_call(const kb200_act_layout* q_in, void* q_out, const kb200_act_layout* k_new,
+                         const kb200_act_layout* v_new, const int32_t* start_pos, const int32_t* n_new,
+                         const kb200_kv_layout* kv, const void* q_norm_gain, const void* k_norm_gain,
+                         float norm_eps, const float* inv_freq, float rope_scale, const kb200_positions* at, int batch,
+                         int max_new, int num_q_heads, int num_kv_heads, void* stream) {
   using namespace kb200;
   KB_ENTRY(k_new ? k_new->ptr : nullptr, "kv_write: k_new");
   KB_REQUIRE(k_new && k_new->ptr && v_new && v_new->ptr && start_pos && kv && kv->k && kv->v,
              "kv_write: null pointer");
   KB_REQUIRE(batch >= 0 && max_new >= 0 && num_kv_heads > 0 && num_q_heads >= 0, "kv_write: bad sizes");
-  const bool fp8 = kv->dtype == KB200_FP8_E4M3;
+  const bool fp8 = kv->dtype == KB200_FP8_E4M3, int4 = kv->dtype == KB200_INT4;
   KB_REQUIRE((k_new->dtype == KB200_FP16 || k_new->dtype == KB200_BF16) && v_new->dtype == k_new->dtype &&
-                 (fp8 || kv->dtype == k_new->dtype) && (!q_in || !q_in->ptr || q_in->dtype == k_new->dtype),
+                 (fp8 || int4 || kv->dtype == k_new->dtype) && (!q_in || !q_in->ptr || q_in->dtype == k_new->dtype),
              "kv_write: q / k / v and the cache must all be fp16 or all bf16 (its arithmetic follows the Hugging Face "
-             "modules step by step in that type; gains are in the same type), or the cache FP8 (e4m3) with scales");
+             "modules step by step in that type; gains are in the same type), or the cache FP8 (e4m3) with scales, or INT4");
+  if (int4) {
+    if (check_int4(kv, true, "kv_write") != 0) return -1;
+    KB_REQUIRE(kv->act_dtype == k_new->dtype, "kv_write: act_dtype of the INT4 cache (%d) is not the rows' type (%d)",
+               kv->act_dtype, k_new->dtype);
+  }
+  if (at) {
+    KB_REQUIRE(at->positions && at->axes >= 1, "kv_write_at: positions [axes, B, T] with at least one axis are required");
+    KB_REQUIRE(!at->token_positions || at->token_rows >= 0, "kv_write_at: negative number of rows of token_positions");
+  }
   KB_REQUIRE(!fp8 || (kv->k_scale && kv->v_scale), "kv_write: an FP8 cache needs k_scale / v_scale");
   const bool bf16 = k_new->dtype == KB200_BF16;
   KB_REQUIRE(kv->page_size >= 1 && (kv->page_size & (kv->page_size - 1)) == 0,
@@ -257,14 +468,88 @@ extern "C" int kb200_kv_write(const kb200_act_layout* q_in, void* q_out, const k
   p.eps = norm_eps;
   p.inv_freq = inv_freq;
   p.rope_scale = rope_scale;
+  if (int4) {
+    p.k_param = static_cast<__half*>(const_cast<void*>(kv->k_param));
+    p.v_param = static_cast<__half*>(const_cast<void*>(kv->v_param));
+    p.pa_sb = kv->param_stride_batch; p.pa_sp = kv->param_stride_page; p.pa_st = kv->param_stride_token; p.pa_sh = kv->param_stride_head;
+  }
+  if (at) {
+    p.positions = at->positions;
+    p.ps_axis = at->stride_axis; p.ps_b = at->stride_batch;
+    p.pair_axis = at->pair_axis;
+    p.axes = at->axes;
+    p.token_positions = at->token_positions;
+    p.tp_sb = at->token_stride; p.tp_rows = at->token_rows;
+  }
   p.B = batch; p.T = max_new; p.H = with_q ? num_q_heads : 0; p.G = num_kv_heads;
   const int64_t blocks = (int64_t)batch * max_new;                   // one CTA per (sequence, new token)
   KB_REQUIRE(blocks < (1ll << 31), "kv_write: too many tokens for one launch");
   cudaStream_t st = (cudaStream_t)stream;
-  if (bf16 && fp8) launch_kv_write<true, true>(p, blocks, st);
-  else if (bf16) launch_kv_write<true, false>(p, blocks, st);
-  else if (fp8) launch_kv_write<false, true>(p, blocks, st);
-  else launch_kv_write<false, false>(p, blocks, st);
+  if (bf16 && int4) launch_kv_write<true, kInt4>(p, blocks, st);
+  else if (int4) launch_kv_write<false, kInt4>(p, blocks, st);
+  else if (bf16 && fp8) launch_kv_write<true, kFp8>(p, blocks, st);
+  else if (bf16) launch_kv_write<true, kSame>(p, blocks, st);
+  else if (fp8) launch_kv_write<false, kFp8>(p, blocks, st);
+  else launch_kv_write<false, kSame>(p, blocks, st);
   KB_CHECK_LAUNCH("kv_write_kernel");
+  return 0;
+}
+
+extern "C" int kb200_kv_write(const kb200_act_layout* q_in, void* q_out, const kb200_act_layout* k_new,
+                              const kb200_act_layout* v_new, const int32_t* start_pos, const int32_t* n_new,
+                              const kb200_kv_layout* kv, const void* q_norm_gain, const void* k_norm_gain,
+                              float norm_eps, const float* inv_freq, float rope_scale, int batch, int max_new,
+                              int num_q_heads, int num_kv_heads, void* stream) {
+  return kv_write_call(q_in, q_out, k_new, v_new, start_pos, n_new, kv, q_norm_gain, k_norm_gain, norm_eps, inv_freq, rope_scale,
+                       nullptr, batch, max_new, num_q_heads, num_kv_heads, stream);
+}
+
+extern "C" int kb200_kv_write_at(const kb200_act_layout* q_in, void* q_out, const kb200_act_layout* k_new,
+                                 const kb200_act_layout* v_new, const int32_t* start_pos, const int32_t* n_new,
+                                 const kb200_kv_layout* kv, const void* q_norm_gain, const void* k_norm_gain,
+                                 float norm_eps, const float* inv_freq, float rope_scale, const kb200_positions* at, int batch,
+                                 int max_new, int num_q_heads, int num_kv_heads, void* stream) {
+  KB_REQUIRE(at, "kv_write_at: null pointer");
+  return kv_write_call(q_in, q_out, k_new, v_new, start_pos, n_new, kv, q_norm_gain, k_norm_gain, norm_eps, inv_freq, rope_scale,
+                       at, batch, max_new, num_q_heads, num_kv_heads, stream);
+}
+
+extern "C" int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens, void* k_out, void* v_out, int batch,
+                             int max_len, int num_kv_heads, void* stream) {
+  using namespace kb200;
+  KB_ENTRY(k_out, "kv_read: k_out");
+  KB_REQUIRE(kv && kv->k && kv->v && seq_lens && k_out && v_out, "kv_read: null pointer");
+  KB_REQUIRE(kv->dtype == KB200_INT4, "kv_read: the cache is not INT4 (dtype code %d): its rows need no conversion", kv->dtype);
+  if (check_int4(kv, true, "kv_read") != 0) return -1;
+  KB_REQUIRE(batch >= 0 && max_len >= 0 && num_kv_heads > 0, "kv_read: bad sizes");
+  KB_REQUIRE(kv->page_size >= 1 && (kv->page_size & (kv->page_size - 1)) == 0,
+             "kv_read: page_size must be a power of two (got %d)", kv->page_size);
+  KB_REQUIRE(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0,
+             "kv_read: k_out and v_out must be 16-byte aligned");
+  KvReadParams p{};
+  p.rows = (int64_t)batch * max_len * num_kv_heads;
+  if (p.rows == 0) return 0;
+  KB_REQUIRE((p.rows + 31) / 32 < (1ll << 31), "kv_read: too many rows for one launch");
+  p.k = static_cast<const uint8_t*>(kv->k);
+  p.v = static_cast<const uint8_t*>(kv->v);
+  p.c_sb = kv->stride_batch; p.c_sp = kv->stride_page; p.c_st = kv->stride_token; p.c_sh = kv->stride_head;
+  p.k_param = static_cast<const __half*>(kv->k_param);
+  p.v_param = static_cast<const __half*>(kv->v_param);
+  p.pa_sb = kv->param_stride_batch; p.pa_sp = kv->param_stride_page; p.pa_st = kv->param_stride_token; p.pa_sh = kv->param_stride_head;
+  p.block_table = kv->block_table;
+  p.bt_stride = kv->block_table_stride;
+  int shift = 0;
+  while ((1 << shift) < kv->page_size) ++shift;
+  p.page_shift = shift;
+  p.page_mask = kv->page_size - 1;
+  p.seq_lens = seq_lens;
+  p.k_out = static_cast<__half*>(k_out);
+  p.v_out = static_cast<__half*>(v_out);
+  p.T = max_len;
+  p.G = num_kv_heads;
+  const unsigned blocks = (unsigned)((p.rows + 31) / 32);
+  if (kv->act_dtype == KB200_BF16) kv_read_kernel<true><<<blocks, 256, 0, (cudaStream_t)stream>>>(p);
+  else kv_read_kernel<false><<<blocks, 256, 0, (cudaStream_t)stream>>>(p);
+  KB_CHECK_LAUNCH("kv_read_kernel");
   return 0;
 }

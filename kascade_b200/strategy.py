@@ -27,7 +27,7 @@ import torch
 from . import _native as nat
 
 __all__ = ["Strategy", "EfficientKascadeStrategy", "topk_budget", "shard_kv_heads", "shard_head_map",
-           "gather_index_rows"]
+           "gather_index_rows", "int4_kv_cache", "rope_axis_map"]
 
 
 def shard_kv_heads(num_kv_heads: int, rank: int, world: int) -> List[int]:
@@ -69,6 +69,32 @@ def topk_budget(pct: float, lk: int, tile_size: int) -> int:
     if tile_size > 1:
         k -= tile_size
     return k
+
+
+def int4_kv_cache(num_pages: int, num_kv_heads: int, page_size: int = 16, device="cuda"):
+    """An empty 4-bit KV cache: key_cache, value_cache uint8 [num_pages, page_size, G, 64] and k_scale, v_scale fp16
+    [num_pages, page_size, G, 8] (four scales and four zeros per row), for ``append_kv``, ``paged_decode_forward``, ``read_kv`` and
+    ``evict_kv``.  The parameters of a row's K and V lie beside each other, so that one 32-byte access fetches both."""
+    shape = (int(num_pages), int(page_size), int(num_kv_heads))
+    k, v = (torch.zeros(*shape, nat.HEAD_DIM // 2, dtype=torch.uint8, device=device) for _ in range(2))
+    params = torch.zeros(*shape, 16, dtype=torch.float16, device=device)
+    return k, v, params[..., :8], params[..., 8:]
+
+
+def rope_axis_map(sections: Sequence[int], interleaved: bool = False, device="cuda") -> torch.Tensor:
+    """The position axis of each rotary pair, [64] int32, for ``append_kv(rope_axes=)``: `sections[a]` pairs turn with axis a, one
+    section after the other, or interleaved: pair i with axis i % axes while that axis has pairs left, with axis 0 otherwise."""
+    sections = [int(n) for n in sections]
+    pairs, axes = nat.HEAD_DIM // 2, len(sections)
+    if not axes or min(sections) < 0 or sum(sections) != pairs:
+        raise ValueError(f"sections must add up to {pairs} pairs, got {sections}")
+    if interleaved:
+        row = [i % axes if i // axes < sections[i % axes] else 0 for i in range(pairs)]
+        if [row.count(a) for a in range(axes)] != sections:
+            raise ValueError(f"sections {sections} cannot be interleaved over {pairs} pairs")
+    else:
+        row = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(row, dtype=torch.int32, device=device)
 
 
 class Strategy:
@@ -250,7 +276,14 @@ class EfficientKascadeStrategy(Strategy):
         The reference (strategies/EfficientKascadeStrategy.py:126-161) never reads the mask: prompts are
         causal and unpadded, a decode step attends to the whole cache.  Here the mask is read for one
         thing only, padding of a batch (leading / trailing key positions that no query may see): the kernels
-        then get every sequence's first row and length and treat it as if it had been run alone."""
+        then get every sequence's first row and length and treat it as if it had been run alone.
+
+        With the keyword `attention_mass` [B, rows] fp32 the anchor layers add to it, in place, the attention that each row of a
+        sequence draws, summed over the heads (and, in a prompt, over the query tiles behind the row's own): what
+        ``evict_kv`` chooses by.  Rows are counted from the sequence's first token."""
+        mass = kwargs.get("attention_mass")
+        if mass is not None and self._shard is not None:
+            raise NotImplementedError("attention_mass is summed over all heads; a sharded strategy holds some of them")
         if query.dtype not in nat.DTYPES or key.dtype != query.dtype or value.dtype != query.dtype:
             raise nat.KascadeNativeError(f"efficient_kascade takes fp16 or bf16 q / k / v of one type; got {query.dtype}, "
                                          f"{key.dtype}, {value.dtype}")
@@ -260,18 +293,18 @@ class EfficientKascadeStrategy(Strategy):
         pad = self._padding(attention_mask, B, Lk) if self._shard is None else None
         if pad is not None:
             if Lq == 1:
-                return self._decode_padded(pad, module, query, key, value, scaling), None
+                return self._decode_padded(pad, module, query, key, value, scaling, mass), None
             if Lq != Lk:
                 raise NotImplementedError("prefill expects the whole prompt (Lq == Lk); chunked prefill is not supported")
             q, k, v = self._token_major(query), self._token_major(key), self._token_major(value)
-            return self._prefill(layer, q, k, v, scaling, ragged=self._pad_bounds(pad, query.device)), None
+            return self._prefill(layer, q, k, v, scaling, ragged=self._pad_bounds(pad, query.device), mass=mass), None
         if Lq == 1:
             kv = nat.kv_layout_contiguous(*self._cache_views(key, value))
             dense = Lk <= 128                      # strategies/EfficientKascadeStrategy.py:137-140
             seq_lens = self._scratch("seq_lens_full", (B,), torch.int32, query.device)
             if dense or self.is_anchor(layer):     # a reuse layer's kernels read the counts of the index rows instead
                 seq_lens.fill_(Lk)
-            out = self._decode(layer, query[:, :, 0], kv, seq_lens, Lk, scaling, G, dense_only=dense)
+            out = self._decode(layer, query[:, :, 0], kv, seq_lens, Lk, scaling, G, dense_only=dense, mass=mass)
             return out.unsqueeze(1), None
         if Lq != Lk:
             raise NotImplementedError("prefill expects the whole prompt (Lq == Lk); chunked prefill is not supported")
@@ -282,9 +315,16 @@ class EfficientKascadeStrategy(Strategy):
         q, k, v = self._token_major(query), self._token_major(key), self._token_major(value)
         if Lk <= 128:
             out = torch.empty(B, Lq, H, D, dtype=query.dtype, device=query.device)
-            nat.prefill_dense(q, k, v, scaling, out, None)
+            lse2 = None
+            if mass is not None and self.is_anchor(layer):
+                lse2 = torch.empty(B, Lq, H, dtype=torch.float32, device=query.device)
+            nat.prefill_dense(q, k, v, scaling, out, lse2)
+            if lse2 is not None:
+                pooled = torch.empty(B, G, -(-Lq // self.tile_size), 128, dtype=torch.float32, device=query.device)
+                nat.prefill_pool_scores(q, k, lse2, scaling, pooled)
+                nat.mass_add_prompt(pooled, mass, mass)
             return out, None
-        return self._prefill(layer, q, k, v, scaling), None
+        return self._prefill(layer, q, k, v, scaling, mass=mass), None
 
     # -- padded batches ---------------------------------------------------------------------------
     def _padding(self, attention_mask, B: int, Lk: int):
@@ -322,7 +362,7 @@ class EfficientKascadeStrategy(Strategy):
             cached = self._pad_dev = (pad, both[0], both[1], pad[1])
         return cached[1:]
 
-    def _decode_padded(self, pad, module, query, key, value, scaling) -> torch.Tensor:
+    def _decode_padded(self, pad, module, query, key, value, scaling, mass=None) -> torch.Tensor:
         """One decode step of a padded batch, every kernel launched once: the cache rows of sequence b are
         starts[b] .. starts[b] + lens[b] - 1, described to the decode kernels as a block table with one-token pages
         (logical position -> cache row), so index rows, budgets and lengths are those of the unpadded sequences."""
@@ -342,7 +382,7 @@ class EfficientKascadeStrategy(Strategy):
         kv = nat.kv_layout_rows(key, value, cached[1])
         out = self._decode(int(module.layer_idx), query[:, :, 0], kv, cached[2], max_len, scaling, G,
                            dense_only=max_len <= 128,              # strategies/EfficientKascadeStrategy.py:137-140
-                           mean_len=max(sum(lens) / len(lens), 1.0))
+                           mean_len=max(sum(lens) / len(lens), 1.0), mass=mass)
         return out.unsqueeze(1)
 
     @staticmethod
@@ -353,7 +393,7 @@ class EfficientKascadeStrategy(Strategy):
         return key, value
 
     # -- prefill -----------------------------------------------------------------------------------
-    def _prefill(self, layer: int, q, k, v, scaling, ragged=None) -> torch.Tensor:
+    def _prefill(self, layer: int, q, k, v, scaling, ragged=None, mass=None) -> torch.Tensor:
         """q [B,L,H,D], k / v [B,L,G,D] token-major views.  `ragged` = (first rows [B] int32, lengths [B] int32 on
         the device, lengths on the host): a padded batch, every kernel still launched once; rows outside a sequence
         come back as zeros."""
@@ -385,6 +425,8 @@ class EfficientKascadeStrategy(Strategy):
             stride = -(-L // 128) * 128
             pooled = self._scratch("pooled", (B, G, T, stride), torch.float32, dev)
             nat.prefill_pool_scores(q, k, lse2, scaling, pooled, ragged=rg)
+            if mass is not None:
+                nat.mass_add_prompt(pooled, mass, mass, seq_len=None if ragged is None else ragged[1])
             n_valid = self._scratch("n_valid", (B, G, T), torch.int32, dev)
             k_row = self._scratch("k_row", (B, G, T), torch.int32, dev)
             if ragged is None:
@@ -515,7 +557,7 @@ class EfficientKascadeStrategy(Strategy):
         return s
 
     def _decode(self, layer: int, q, kv, seq_lens, max_len: int, scaling, G: int, dense_only=False,
-                mean_len: Optional[float] = None) -> torch.Tensor:
+                mean_len: Optional[float] = None, mass=None, index_rows=None) -> torch.Tensor:
         B, H, D = q.shape
         dev = q.device
         if q.stride(2) != 1 or q.stride(0) % 2 or q.stride(1) % 2:
@@ -532,6 +574,8 @@ class EfficientKascadeStrategy(Strategy):
             want_out = dense_only or layer == 0
             nat.decode_anchor_paged(q, kv, seq_lens, max_len, scaling, logits, pooled, out if want_out else None,
                                     lse2, ws, splits_a)
+            if mass is not None and self.is_anchor(layer):
+                nat.mass_add(pooled, seq_lens, mass, mass, max_len)
             if dense_only:
                 return out
             self._dec_kmax = kmax = self._decode_row_length(max_len)
@@ -543,39 +587,128 @@ class EfficientKascadeStrategy(Strategy):
                 return out
             head_map = None
         else:
-            if self._dec_idx is None:
+            if self._dec_idx is None and index_rows is None:
                 raise RuntimeError("reuse layer called before any anchor layer")
             head_map = self._mapping(layer, dev)
-        kmax = self._dec_kmax
+        rows, counts = (self._dec_idx, self._dec_count) if index_rows is None else index_rows
+        kmax = rows.shape[2]
         splits = self._splits(B, G, kmax, ragged, dev)
         ws = self._scratch("dec_ws_s", (nat.load().kb200_decode_workspace_bytes(B, H, splits),), torch.uint8, dev)
-        nat.decode_sparse_paged(q, kv, self._dec_idx, self._dec_count, kmax, head_map, scaling, out, None, ws, splits)
+        nat.decode_sparse_paged(q, kv, rows, counts, kmax, head_map, scaling, out, None, ws, splits)
         return out
 
     @staticmethod
     def append_kv(key_new, value_new, key_cache, value_cache, block_table, start_pos, n_new=None, *, query=None,
                   q_norm_weight=None, k_norm_weight=None, norm_eps: float = 1e-6, inv_freq=None,
-                  rope_scale: float = 1.0, k_scale=None, v_scale=None):
+                  rope_scale: float = 1.0, k_scale=None, v_scale=None, positions=None, rope_axes=None, token_positions=None):
         """Prefill -> decode hand-off: write the new tokens' K / V rows (key_new / value_new [B,T,G,D] views,
         positions start_pos[b] + t) into the paged cache the decode kernels read, in one kernel; with
         `inv_freq` (the model's rotary table) and / or the norm weights the rows (and `query` [B,T,H,D], returned
         transformed) are normalised and rotated on the way, as the Hugging Face module would have done; into an FP8
-        (e4m3) cache, with `k_scale` / `v_scale` [num_pages, G] fp32, the rows are stored as value / scale.
+        (e4m3) cache, with `k_scale` / `v_scale` [num_pages, G] fp32, the rows are stored as value / scale; into a 4-bit cache
+        (``int4_kv_cache``), with its `k_scale` / `v_scale`, as codes with a scale and a zero per 32 values.
+
+        `positions` [B,T] or [axes,B,T] (integers) are rotary positions that are not the rows' places in the cache: of a cache that
+        ``evict_kv`` has shortened, or of images and video with several axes, where `rope_axes` [64] int32
+        (``rope_axis_map``) gives the axis of each pair.  Angles are then formed in 64 bits, and the rows rounded once.
+        `token_positions` [B, rows] int32 receives the new tokens' positions (on the first axis) at their rows of the cache.
         The reference has no counterpart (it receives rotated tensors and copies them per call,
         strategies/EfficientKascadeStrategy.py:144-150)."""
-        kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale)
+        if positions is not None:
+            if positions.dtype.is_floating_point or positions.dim() not in (2, 3):
+                raise ValueError(f"positions must be integers [B, T] or [axes, B, T], got {positions.dtype} {tuple(positions.shape)}")
+            positions = positions.to(torch.int32)
+            positions = positions[None] if positions.dim() == 2 else positions
+            if positions.shape[2] > 1 and positions.stride(2) != 1:
+                positions = positions.contiguous()
+            if positions.shape[0] > 1 and rope_axes is None and inv_freq is not None:
+                raise ValueError("positions with several axes need rope_axes, the axis of each rotary pair")
+        elif rope_axes is not None or token_positions is not None:
+            raise ValueError("rope_axes and token_positions belong to positions")
+        kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, key_new.dtype)
         q_out = torch.empty_like(query, memory_format=torch.contiguous_format) if query is not None else None
         nat.kv_write(query, q_out, key_new, value_new, start_pos, n_new, kv, q_norm_weight, k_norm_weight, norm_eps,
-                     inv_freq, rope_scale)
+                     inv_freq, rope_scale, positions, rope_axes, token_positions)
         return q_out
+
+    @staticmethod
+    def read_kv(key_cache, value_cache, block_table, seq_lens, max_seq_len: int, *, k_scale, v_scale,
+                dtype: torch.dtype = torch.float16):
+        """Rows 0 .. seq_lens[b] - 1 of a 4-bit cache as key, value [B, max_seq_len, G, D] in `dtype` (fp16 or bf16), zeros behind
+        a sequence: for a prompt that arrives in pieces, whose attention runs over 16-bit rows."""
+        if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
+            seq_lens = seq_lens.to(torch.int32).contiguous()
+        B, G = seq_lens.shape[0], key_cache.shape[2]
+        if not 0 <= max_seq_len <= block_table.shape[1] * key_cache.shape[1]:
+            raise ValueError(f"max_seq_len {max_seq_len} is beyond the block table's {block_table.shape[1]} pages")
+        if block_table.shape[0] != B:
+            raise ValueError(f"block_table has rows for {block_table.shape[0]} sequences, seq_lens for {B}")
+        kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, dtype)
+        out = torch.empty(2, B, max_seq_len, G, nat.HEAD_DIM, dtype=dtype, device=key_cache.device)
+        nat.kv_read(kv, seq_lens, out[0], out[1])
+        return out[0], out[1]
+
+    @staticmethod
+    def prompt_mass(pooled, attention_mass, seq_lens=None) -> torch.Tensor:
+        """attention_mass [B, rows] fp32 plus the attention that the rows of a prompt drew from the query tiles behind their own:
+        pooled [B, G, tiles, row_stride] as ``kb200_prefill_pool_scores`` leaves it, summed over heads and tiles.  A new tensor
+        (``attention_forward(attention_mass=)`` adds in place)."""
+        out = torch.empty_like(attention_mass, memory_format=torch.contiguous_format)
+        nat.mass_add_prompt(pooled, attention_mass, out, seq_lens)
+        return out
+
+    @staticmethod
+    def evict_kv(caches, block_table, seq_lens, attention_mass, budget: int, *, recent: int = 0, sinks: int = 0,
+                 token_positions=None):
+        """Shortens every sequence of a paged cache to at most `budget` rows: those with the largest `attention_mass` [B, rows]
+        fp32 stay (ties: the lowest row), the first `sinks` token positions and the last `recent` ones in any case.  The rows
+        that go are the same in all layers and heads, because anchor layers hand index rows to other layers and heads.
+
+        caches: the layers' (key_cache, value_cache) or (key_cache, value_cache, k_scale, v_scale); fp16, bf16 or 4-bit, changed in
+        place.  Kept rows behind the new length move into the places before it that became free, no other row moves; so
+        rows lose their order, which attention does not see, and `token_positions` [B, rows] int32 (None: rows in order, of a
+        cache that nothing has left yet) says what each holds.  Pages below the new length must belong to one sequence alone.
+
+        Returns seq_lens [B] int32, attention_mass [B, rows] and token_positions [B, rows] of the shortened cache, as new tensors
+        (0 and -1 behind a sequence).  Append the next tokens with ``start_pos=`` these lengths and ``positions=`` their own."""
+        if not caches:
+            raise ValueError("evict_kv needs the cache of one layer at least")
+        if attention_mass.dim() != 2:
+            raise ValueError(f"attention_mass must be [B, rows], got {tuple(attention_mass.shape)}")
+        B, rows = attention_mass.shape
+        if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+            raise ValueError(f"budget {budget} must be positive and hold the {sinks} first and {recent} last rows")
+        if block_table.shape[0] != B or seq_lens.shape != (B,):
+            raise ValueError(f"block_table and seq_lens must have a row for each of {B} sequences")
+        if rows > block_table.shape[1] * caches[0][0].shape[1]:
+            raise ValueError(f"attention_mass has {rows} rows, the block table {block_table.shape[1]} pages")
+        if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
+            seq_lens = seq_lens.to(torch.int32).contiguous()
+        budget = min(int(budget), rows)
+        layouts = [nat.kv_layout_paged(c[0], c[1], block_table, *c[2:]) for c in caches]
+        dev = attention_mass.device
+        keys = torch.empty(B, -(-rows // 4) * 4, dtype=torch.float32, device=dev)
+        nat.evict_keys(attention_mass, seq_lens, token_positions, sinks, recent, keys)
+        keep = torch.empty(B, budget, dtype=torch.int32, device=dev)
+        counts = torch.empty(3, B, dtype=torch.int32, device=dev)
+        nat.topk_select(keys, seq_lens, None, budget, keep, counts[0], n_cols=rows)
+        moves = torch.empty(B, budget, 2, dtype=torch.int32, device=dev)
+        mass, positions = torch.empty(B, rows, dtype=torch.float32, device=dev), torch.empty(B, rows, dtype=torch.int32, device=dev)
+        nat.evict_plan(keep, counts[0], attention_mass, token_positions, moves, counts[1], counts[2], mass, positions)
+        nat.evict_move(layouts, moves, counts[1], min(budget, rows - budget), caches[0][0].shape[2])
+        return counts[2], mass, positions
 
     def paged_decode_forward(self, layer_idx: int, query, key_cache, value_cache, block_table, seq_lens, scaling,
                              max_seq_len: Optional[int] = None, k_scale=None, v_scale=None,
-                             mean_seq_len: Optional[float] = None) -> torch.Tensor:
+                             mean_seq_len: Optional[float] = None, attention_mass=None, index_rows=None) -> torch.Tensor:
         """Paged-attention backend entry: query [B,H,D] fp16 / bf16, key/value cache
         [num_pages, page_size, G, D] of the same type, block_table [B, max_pages] int32, seq_lens [B] int32
         (other integer types are converted) -> out [B,H,D].  An FP8 (e4m3) cache comes with k_scale / v_scale
-        [num_pages, G] fp32 and takes fp16 queries.  `mean_seq_len` is a hint of the host for batches of very different
+        [num_pages, G] fp32 and takes fp16 queries; a 4-bit cache (``int4_kv_cache``) with its k_scale / v_scale takes
+        either type.  `attention_mass` [B, rows >= max_seq_len] fp32: anchor layers add to it, in place, the attention that each
+        row draws, summed over the heads (reuse layers do not see all rows and leave it as it is); ``evict_kv`` chooses by it.
+        `index_rows` = (rows [B,G,k] int32, counts [B,G] int32): a reuse layer attends to these rows (of the KV head its mapping
+        names) instead of the last anchor layer's, for a layer whose anchor runs elsewhere.  `mean_seq_len` is a hint of the host for batches of very different
         lengths (the work is then cut into more, smaller pieces); results do not depend on it beyond summation order.
         The reference has no paged kernel (README.md:135); the nearest signature is
         kernels/flash_decoding/reuse_kascade_gqa_decode_with_kvcache.py:160-171."""
@@ -583,6 +716,14 @@ class EfficientKascadeStrategy(Strategy):
             max_seq_len = int(seq_lens.max().item())
         if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():     # the kernels read contiguous int32
             seq_lens = seq_lens.to(torch.int32).contiguous()
-        kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale)
+        if index_rows is not None:
+            if self.is_anchor(int(layer_idx)):
+                raise ValueError(f"layer {layer_idx} is an anchor layer: it selects its own rows")
+            rows, counts = index_rows
+            want = (query.shape[0], key_cache.shape[2])
+            if rows.dim() != 3 or tuple(rows.shape[:2]) != want or tuple(counts.shape) != want or not counts.is_contiguous():
+                raise ValueError(f"index_rows must be [{want[0]}, {want[1]}, k] and contiguous counts {want}, got "
+                                 f"{tuple(rows.shape)} and {tuple(counts.shape)}")
+        kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, query.dtype)
         return self._decode(int(layer_idx), query, kv, seq_lens, int(max_seq_len), scaling, key_cache.shape[2],
-                            mean_len=mean_seq_len)
+                            mean_len=mean_seq_len, mass=attention_mass, index_rows=index_rows)
