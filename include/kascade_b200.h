@@ -387,7 +387,7 @@ int kb200_prefill_budgets(int32_t* n_valid, int32_t* k_row, int batch, int num_k
  *               layer): a row is stored as value / scale of its page and KV head (fp32 division, saturating at
  *               +-448, round to nearest even) - the bytes the decode entry points read back as byte x scale;
  *               or an INT4 cache: per group of 32 values  z = fp16(min), s = fp16((max - z) / 15 in fp32) and the codes
- *               round((x - z) / s), half to even, clamped to 0..15.  What fp16 cannot hold saturates; a group with a value
+ *               round((x - z) / s), half to even, clamped to 0..15.  Values saturate at +-65504; a group with a value
  *               that is not finite gets z = NaN
  *   q_norm_gain / k_norm_gain  [D] in the same type, or NULL (no norm);  norm_eps
  *   inv_freq    [D/2] fp32 inverse frequencies of the model's rotary embedding (device memory), or NULL

@@ -2,22 +2,68 @@
 //
 // A row of 128 values is four groups of 32 codes c in 0..15 that stand for s c + z, with s and z in fp16 per group; the
 // order of the codes in a row is written beside kb200_kv_layout.  Same division of the work as in decode.cu: a CTA owns one
-// (sequence, KV head, split), and its partial results meet in merge_warps and decode_combine_kernel.
+// (sequence, KV head, split), every warp streams steps of 32 keys through a private cp.async ring, and partial results meet in
+// merge_warps and decode_combine_kernel.
 //
-// One warp per key: a lane holds four values of the row (16 bits of codes).
+// At 160 bytes a key the copies leave a warp scheduler some 230 issue slots per eight keys, so the rows are never turned into
+// fp16 values.  A code in the low bits of an fp16 word IS a number: the subnormal c 2^-24, or 16 c 2^-24 four bits further
+// up, and the tensor core takes subnormals as they are.  One AND therefore makes a pair of matrix operands from a word of
+// codes (two, after a shift by eight), and scales and zeros are applied where they are few:
+//   * S = K Q^T, keys as rows:  S = sum_g s_g (sum_{d in g} c_d q_d) + sum_g z_g (sum_{d in g} q_d).  Two products of 16 d for each
+//     group, whose sums are scaled by the key's s_g in fp32; the zeros are one more product, of the keys' parameters with the
+//     queries' sums over the groups (as two fp16 terms, exact to 2^-22).
+//   * O^T = V^T P^T, values as rows:  sum_k (p_k s_gk) c_dk  with the scale on the probabilities, which are one row per head,
+//     not on the 128 values, and sum_k p_k z_gk as one product with the transposed parameters.
+// The orders of the codes in K and V rows are those in which a lane needs them: 16 bytes of a K row, 8 of a V row.
+// Queries are brought to a largest element of 64..128 per head by a power of two, so that bf16 ones fit fp16 exactly.
 #include "decode.cuh"
 
 namespace kb200 {
 
-constexpr int kWarps4 = 8;
+constexpr int kWarps4 = 16;                                // warps of a full-size CTA (one per SM); half-size CTAs run two per SM
+constexpr int kKeys4 = 32;                                 // keys of a step, one per lane while they are copied
+constexpr int kCodes4 = kKeys4 * kD / 2;                   // bytes of the codes of a step's K or V rows
+constexpr int kHalf4 = kCodes4 + kKeys4 * 16;              // ... with their parameters
+constexpr int kCodeOne = 1 << 24;                          // 1 / (the value of code 1 as an fp16 subnormal)
+constexpr float kShift4 = 2.f;                             // probabilities are at most 2^2: their products with a scale stay in fp16's
+                                                           // range (s <= 8734) and further away from its subnormals
+__host__ __device__ constexpr int stages4(bool has_v) { return has_v ? 2 : 4; }
+__host__ __device__ constexpr int stage_bytes4(bool has_v) { return has_v ? 2 * kHalf4 : kHalf4; }
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void ldmatrix_x2(uint32_t& a, uint32_t& b, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];\n" : "=r"(a), "=r"(b) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x2_trans(uint32_t& a, uint32_t& b, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];\n" : "=r"(a), "=r"(b) : "r"(addr));
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(r.x), "=r"(r.y) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 template <bool DENSE, bool HAS_V, bool BF16>
-__global__ void __launch_bounds__(kWarps4 * 32) decode_attn4_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const DecodeParams p) {
   pdl_wait();
   constexpr uint32_t FULL = 0xFFFFFFFFu;
-  __shared__ float sm_m[kWarps4 * kHg], sm_l[kWarps4 * kHg], sm_o[HAS_V ? kWarps4 * kHg * kD : 1];
+  constexpr int kStages = stages4(HAS_V), kStage = stage_bytes4(HAS_V);
+  const int WARPS = blockDim.x >> 5;
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int grp = lane >> 2, quad = lane & 3;
+
+  // ---- this CTA's slice of the key list, in steps of 32 keys --------------------------------------
   int n;
   const int32_t* idx_row = nullptr;
   if (DENSE) {
@@ -28,91 +74,303 @@ __global__ void __launch_bounds__(kWarps4 * 32) decode_attn4_kernel(const Decode
     idx_row = p.idx + b * p.idx_stride_b + src_g * p.idx_stride_g;
   }
   n = max(n, 0);
-  const int nst = (n + 15) / 16, per = (nst + p.num_splits - 1) / p.num_splits;
-  const int begin = min(split * per * 16, n), end = min(begin + per * 16, n);
+  const int nst = (n + kKeys4 - 1) / kKeys4, per = (nst + p.num_splits - 1) / p.num_splits;
+  const int st_begin = min(split * per, nst), st_end = min(st_begin + per, nst);
+  const int my_count = (st_end - st_begin - warp + WARPS - 1) / WARPS;                 // may be <= 0
 
-  // the values of this lane: nibbles 4 lane .. 4 lane + 3 of a row
-  const int k_group = (lane & 7) >> 1, k_d = 32 * k_group + 8 * (lane >> 3) + 4 * (lane & 1);
-  const int v_group = lane & 3, v_d = 32 * v_group + 4 * (lane >> 2);
-  float q[kHg][4];
+  // ---- queries: B operand Q^T[d][head], column = head grp (zero for grp >= 4) -----------------------
+  // k-step (group e, half f): k = 2 quad, 2 quad + 1 are d = 32 e + 8 quad + {2f, 2f + 4}, k + 8 the d one further, whose codes
+  // lie four bits further up: times 4 here, a quarter there
+  uint32_t qb[4][2][2], zb0, zb1;
+  float c_head[2];                                         // scale * log2 e * 2^(exponent of the head's queries), heads 2 quad, + 1
+  {
+    const __half* qp = p.q + b * p.q_stride_b + (int64_t)(g * kHg + (grp & 3)) * p.q_stride_h;
+    float q[4][8], top = 0.f;
 #pragma unroll
-  for (int h = 0; h < kHg; ++h) {
-    const __half* qp = p.q + b * p.q_stride_b + (int64_t)(g * kHg + h) * p.q_stride_h + k_d;
+    for (int e = 0; e < 4; ++e) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[h][e] = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(qp)[e]) : __half2float(qp[e]);
-  }
-  const uint8_t* k8 = reinterpret_cast<const uint8_t*>(p.k) + (int64_t)b * p.kv_stride_batch + (int64_t)g * p.kv_stride_head;
-  const uint8_t* v8 = reinterpret_cast<const uint8_t*>(p.v) + (int64_t)b * p.kv_stride_batch + (int64_t)g * p.kv_stride_head;
-  const int64_t pa_base = (int64_t)b * p.pa_stride_batch + (int64_t)g * p.pa_stride_head;
-  float m[kHg], l[kHg], o[kHg][4];
-#pragma unroll
-  for (int h = 0; h < kHg; ++h) {
-    m[h] = -INFINITY;
-    l[h] = o[h][0] = o[h][1] = o[h][2] = o[h][3] = 0.f;
-  }
-  for (int j = begin + warp; j < end; j += kWarps4) {
-    const int pos = DENSE ? j : idx_row[j];
-    const int lp = pos >> p.page_shift, slot = pos & p.page_mask;
-    const int64_t page = p.block_table ? p.block_table[(int64_t)b * p.block_table_stride + lp] : lp;
-    const int64_t at = page * p.kv_stride_page + slot * p.kv_stride_token;
-    const int64_t pa = pa_base + page * p.pa_stride_page + slot * p.pa_stride_token;
-    const uint32_t kc = reinterpret_cast<const uint16_t*>(k8 + at)[lane];
-    const float ks = __half2float(p.k_param[pa + k_group]), kz = __half2float(p.k_param[pa + 4 + k_group]);
-    float x[kHg];
-#pragma unroll
-    for (int h = 0; h < kHg; ++h) {
-      x[h] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[h] += q[h][e] * (ks * (float)((kc >> (4 * e)) & 15) + kz);
-#pragma unroll
-      for (int sh = 16; sh > 0; sh >>= 1) x[h] += __shfl_xor_sync(FULL, x[h], sh);
-      x[h] *= p.scale2;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(qp + 32 * e + 8 * quad + 2 * i);
+        const float2 f = BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)) : half2_floats(w);
+        q[e][2 * i] = f.x;
+        q[e][2 * i + 1] = f.y;
+        top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
     }
-    if (DENSE && lane < kHg) {
-      float mine = x[0];
+    top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+    const int up = 6 - max((int)(__float_as_uint(top) >> 23) - 127, -90);   // exponent of the factor: -121 .. 96
+    const float factor = grp < kHg ? __uint_as_float((uint32_t)(up + 127) << 23) : 0.f;
+    const float unit = p.scale2 * __uint_as_float((uint32_t)(127 - up) << 23);
+    c_head[0] = __shfl_sync(FULL, unit, (quad & 1) * 8);                    // heads 2 quad and 2 quad + 1 (the lanes of quads 2, 3
+    c_head[1] = __shfl_sync(FULL, unit, (quad & 1) * 8 + 4);                // hold the unused columns)
+    float sum[4];
 #pragma unroll
-      for (int h = 1; h < kHg; ++h) mine = lane == h ? x[h] : mine;
-      p.logits[((int64_t)b * p.H + g * kHg + lane) * p.logit_stride + j] = mine;
+    for (int e = 0; e < 4; ++e) {
+      sum[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[e][i] = __half2float(__float2half_rn(q[e][i] * factor));
+        sum[e] += q[e][i];
+      }
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        qb[e][f][0] = pack_half2<false>(q[e][2 * f] * 4.f, q[e][2 * f + 4] * 4.f);
+        qb[e][f][1] = pack_half2<false>(q[e][2 * f + 1] * 0.25f, q[e][2 * f + 5] * 0.25f);
+      }
+      sum[e] += __shfl_xor_sync(FULL, sum[e], 1);
+      sum[e] += __shfl_xor_sync(FULL, sum[e], 2);
     }
-    float v[4];
+    // zeros: k = 4 + e of the parameters is z_e; the high parts of the sums below, the rests in k + 8
+    const float s0 = quad == 2 ? sum[0] : sum[2], s1 = quad == 2 ? sum[1] : sum[3];
+    zb0 = quad < 2 ? 0u : pack_half2<false>(s0, s1);
+    const float2 high = half2_floats(zb0);
+    zb1 = quad < 2 ? 0u : pack_half2<false>(s0 - high.x, s1 - high.y);
+  }
+
+  const uint8_t* k_base = reinterpret_cast<const uint8_t*>(p.k) + (int64_t)b * p.kv_stride_batch + (int64_t)g * p.kv_stride_head;
+  const uint8_t* v_base = reinterpret_cast<const uint8_t*>(p.v) + (int64_t)b * p.kv_stride_batch + (int64_t)g * p.kv_stride_head;
+  const __half* kp_base = p.k_param + (int64_t)b * p.pa_stride_batch + (int64_t)g * p.pa_stride_head;
+  const __half* vp_base = p.v_param + (int64_t)b * p.pa_stride_batch + (int64_t)g * p.pa_stride_head;
+  const int32_t* table = p.block_table ? p.block_table + (int64_t)b * p.block_table_stride : nullptr;
+  const uint32_t ring = smem_u32(smem) + warp * (kStages * kStage);
+
+  // Codes in shared memory: two rows to a line of 128 bytes, the 16-byte pieces of line i exchanged by XOR with 2 i, so that
+  // the copies, the reads of K (eight pieces of a line at once) and of V (two pieces of four lines) use all banks.
+  // A lane copies piece quad of row grp (+ 8 i) and later reads the same piece of K.
+  const uint32_t k_at = (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) * 2)) << 4);
+  const uint32_t v_at = quad * 128 + (((grp >> 1) ^ (quad * 2)) << 4) + (grp & 1) * 8;   // row 2 quad, bytes 8 grp ..; the next row: ^ 64
+
+  auto load_pos = [&](int j) -> int {                      // position of key `lane` of step j of this warp
+    if (j >= my_count) return 0;
+    const int s = min((st_begin + warp + j * WARPS) * kKeys4 + lane, n - 1);
+    return DENSE ? s : idx_row[s];
+  };
+  auto load_page = [&](int pos) -> int {
+    const int lp = pos >> p.page_shift;
+    return table ? table[lp] : lp;
+  };
+  auto issue = [&](int j, int pos, int page) {
+    if (j < my_count) {
+      const int slot = pos & p.page_mask;
+      const int64_t off = (int64_t)page * p.kv_stride_page + (int64_t)slot * p.kv_stride_token;
+      const int64_t par = (int64_t)page * p.pa_stride_page + (int64_t)slot * p.pa_stride_token;
+      const uint32_t dst = ring + (j % kStages) * kStage;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t row = __shfl_sync(FULL, off, i * 8 + grp) + quad * 16;
+        cp_async16(dst + i * 512 + k_at, k_base + row);
+        if (HAS_V) cp_async16(dst + kHalf4 + i * 512 + k_at, v_base + row);
+      }
+      cp_async16(dst + kCodes4 + lane * 16, kp_base + par);
+      if (HAS_V) cp_async16(dst + kHalf4 + kCodes4 + lane * 16, vp_base + par);
+    }
+    cp_async_commit();
+  };
+
+  int pos_a, page_a, pos_b;
+  {
+    int pos[kStages], page[kStages];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) pos[i] = load_pos(i);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) page[i] = load_page(pos[i]);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i, pos[i], page[i]);
+    pos_a = pos[kStages - 1];
+    page_a = page[kStages - 1];
+    pos_b = load_pos(kStages);
+  }
+
+  // o_acc[e][f]: values d = 32 e + 4 grp + 2 f (rows 0-7) and + 1, times 16 (rows 8-15), of heads 2 quad, 2 quad + 1; o_zero: row
+  // 4 + e is the zeros' share of group e
+  float o_acc[4][2][4], o_zero[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    o_zero[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o_acc[e][0][i] = o_acc[e][1][i] = 0.f;
+  }
+  float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
+
+  for (int j = 0; j < my_count; ++j) {
+    __syncwarp();                      // every lane is done with the buffer about to be refilled
+    issue(j + kStages - 1, pos_a, page_a);
+    pos_a = pos_b;
+    page_a = load_page(pos_a);
+    pos_b = load_pos(j + kStages + 1);
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t buf = ring + (j % kStages) * kStage;
+    const int key0 = (st_begin + warp + j * WARPS) * kKeys4;
+
+    // ---- logits: x[i] of keys 16 i + grp and + 8, heads 2 quad, 2 quad + 1 -------------------------------
+    float x[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t wa[4], wb[4];                                 // group e's eight codes of keys grp and grp + 8
+      lds128(wa[0], wa[1], wa[2], wa[3], buf + i * 1024 + k_at);
+      lds128(wb[0], wb[1], wb[2], wb[3], buf + i * 1024 + 512 + k_at);
+      const uint32_t par = buf + kCodes4 + i * 256;
+      uint32_t za, zc;
+      ldmatrix_x2(za, zc, par + (lane & 15) * 16);
+      float zero[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
+      mma16816<false>(zero, za, zc, za, zc, zb0, zb1);
+      const uint2 sa = lds64(par + grp * 16), sb = lds64(par + grp * 16 + 128);
+      const float2 sa01 = half2_floats(sa.x), sa23 = half2_floats(sa.y), sb01 = half2_floats(sb.x), sb23 = half2_floats(sb.y);
+      const float fa[4] = {sa01.x, sa01.y, sa23.x, sa23.y}, fb[4] = {sb01.x, sb01.y, sb23.x, sb23.y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816<false>(s, wa[e] & 0x000F000Fu, wb[e] & 0x000F000Fu, wa[e] & 0x00F000F0u, wb[e] & 0x00F000F0u, qb[e][0][0], qb[e][0][1]);
+        const uint32_t ha = wa[e] >> 8, hb = wb[e] >> 8;
+        mma16816<false>(s, ha & 0x000F000Fu, hb & 0x000F000Fu, ha & 0x00F000F0u, hb & 0x00F000F0u, qb[e][1][0], qb[e][1][1]);
+        t[0] += fa[e] * s[0];
+        t[1] += fa[e] * s[1];
+        t[2] += fb[e] * s[2];
+        t[3] += fb[e] * s[3];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[i][r] = fmaf(t[r], (float)(kCodeOne / 4), zero[r]) * c_head[r & 1];
+    }
+    if (key0 + kKeys4 > n) {                                 // the list ends inside this step
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (key0 + 16 * i + grp >= n) x[i][0] = x[i][1] = -INFINITY;
+        if (key0 + 16 * i + grp + 8 >= n) x[i][2] = x[i][3] = -INFINITY;
+      }
+    }
+    if (DENSE && quad < 2) {
+      float* lp = p.logits + ((int64_t)b * p.H + g * kHg + quad * 2) * p.logit_stride + key0 + grp;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (key0 + 16 * i + grp < n) { lp[16 * i] = x[i][0]; lp[p.logit_stride + 16 * i] = x[i][1]; }
+        if (key0 + 16 * i + grp + 8 < n) { lp[16 * i + 8] = x[i][2]; lp[p.logit_stride + 16 * i + 8] = x[i][3]; }
+      }
+    }
+    // ---- running maximum and sum, per lane for its two heads ---------------------------------------------
+    float t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])), t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
+#pragma unroll
+    for (int sh = 4; sh <= 16; sh <<= 1) {
+      t0 = fmaxf(t0, __shfl_xor_sync(FULL, t0, sh));
+      t1 = fmaxf(t1, __shfl_xor_sync(FULL, t1, sh));
+    }
+    const float m0 = fmaxf(m_run[0], t0 - kShift4), m1 = fmaxf(m_run[1], t1 - kShift4);   // every step has a valid key
+    const float alpha0 = ex2(m_run[0] - m0), alpha1 = ex2(m_run[1] - m1);
+    m_run[0] = m0;
+    m_run[1] = m1;
+    float w[2][4], sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i][0] = ex2(x[i][0] - m0);
+      w[i][1] = ex2(x[i][1] - m1);
+      w[i][2] = ex2(x[i][2] - m0);
+      w[i][3] = ex2(x[i][3] - m1);
+      sum0 += w[i][0] + w[i][2];
+      sum1 += w[i][1] + w[i][3];
+    }
+    l_part[0] = l_part[0] * alpha0 + sum0;
+    l_part[1] = l_part[1] * alpha1 + sum1;
     if (HAS_V) {
-      const uint32_t vc = reinterpret_cast<const uint16_t*>(v8 + at)[lane];
-      const float vs = __half2float(p.v_param[pa + v_group]), vz = __half2float(p.v_param[pa + 4 + v_group]);
+      if (!__all_sync(FULL, alpha0 == 1.f && alpha1 == 1.f)) {           // a factor of exactly 1 changes nothing
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = vs * (float)((vc >> (4 * e)) & 15) + vz;
-    }
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-    for (int h = 0; h < kHg; ++h) {
-      const float m_new = fmaxf(m[h], x[h]);
-      const float alpha = exp2f(m[h] - m_new), w = exp2f(x[h] - m_new);
-      m[h] = m_new;
-      l[h] = l[h] * alpha + w;
-      if (HAS_V) {
+          for (int f = 0; f < 2; ++f) {
+            o_acc[e][f][0] *= alpha0; o_acc[e][f][1] *= alpha1; o_acc[e][f][2] *= alpha0; o_acc[e][f][3] *= alpha1;
+          }
+        }
+        o_zero[0] *= alpha0; o_zero[1] *= alpha1; o_zero[2] *= alpha0; o_zero[3] *= alpha1;
+      }
+      // ---- O^T += V^T P^T -------------------------------------------------------------------------------
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[h][e] = o[h][e] * alpha + w * v[e];
+      for (int i = 0; i < 2; ++i) {
+        // B operand P^T[key][head]: column = head grp, rows = keys 2 quad, 2 quad + 1 (pb0) and + 8 (pb1)
+        const uint32_t pb0 = movmatrix_trans(pack_half2<false>(w[i][0], w[i][1]));
+        const uint32_t pb1 = movmatrix_trans(pack_half2<false>(w[i][2], w[i][3]));
+        uint32_t z0, z1;                                       // lane (r, quad): parameter r of keys 2 quad, 2 quad + 1 / + 8
+        ldmatrix_x2_trans(z0, z1, buf + kHalf4 + kCodes4 + i * 256 + (lane & 15) * 16);
+        mma16816<false>(o_zero, z0, 0u, z1, 0u, pb0, pb1);
+        const uint32_t v = buf + kHalf4 + i * 1024 + v_at;
+        const uint2 ka = lds64(v), kb = lds64(v ^ 64u), kc = lds64(v + 512), kd = lds64((v + 512) ^ 64u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t sel = (e & 1) ? 0x7632 : 0x5410;
+          const uint32_t lo = __byte_perm(e < 2 ? ka.x : ka.y, e < 2 ? kb.x : kb.y, sel);      // keys 2 quad, 2 quad + 1
+          const uint32_t hi = __byte_perm(e < 2 ? kc.x : kc.y, e < 2 ? kd.x : kd.y, sel);      // ... + 8
+          const uint32_t sb0 = mul_half2(pb0, __shfl_sync(FULL, z0, e * 4 + quad));
+          const uint32_t sb1 = mul_half2(pb1, __shfl_sync(FULL, z1, e * 4 + quad));
+          mma16816<false>(o_acc[e][0], lo & 0x000F000Fu, lo & 0x00F000F0u, hi & 0x000F000Fu, hi & 0x00F000F0u, sb0, sb1);
+          const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+          mma16816<false>(o_acc[e][1], lo8 & 0x000F000Fu, lo8 & 0x00F000F0u, hi8 & 0x000F000Fu, hi8 & 0x00F000F0u, sb0, sb1);
+        }
       }
     }
   }
-  pdl_trigger();
+  cp_async_wait<0>();
+  __syncthreads();
+  pdl_trigger();                       // only the merge is left: most SMs have room by now
+
 #pragma unroll
-  for (int h = 0; h < kHg; ++h) {
-    if (lane == 0) { sm_m[warp * kHg + h] = m[h]; sm_l[warp * kHg + h] = l[h]; }
-    if (HAS_V) {
+  for (int sh = 4; sh <= 16; sh <<= 1) {
+    l_part[0] += __shfl_xor_sync(FULL, l_part[0], sh);
+    l_part[1] += __shfl_xor_sync(FULL, l_part[1], sh);
+  }
+  float* sm_m = reinterpret_cast<float*>(smem);                  // [warps][4]
+  float* sm_l = sm_m + WARPS * kHg;                              // [warps][4]
+  float* sm_o = sm_l + WARPS * kHg;                              // [warps][4][128]
+  float zero[4][2];
+  if (HAS_V) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sm_o[(warp * kHg + h) * kD + v_d + e] = o[h][e];
+    for (int e = 0; e < 4; ++e) {
+      zero[e][0] = __shfl_sync(FULL, o_zero[0], (4 + e) * 4 + quad);
+      zero[e][1] = __shfl_sync(FULL, o_zero[1], (4 + e) * 4 + quad);
+    }
+  }
+  if (quad < 2) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int h = quad * 2 + r;
+      if (grp == 0) { sm_m[warp * kHg + h] = m_run[r]; sm_l[warp * kHg + h] = l_part[r]; }
+      if (HAS_V) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float4 o;
+          o.x = fmaf(o_acc[e][0][r], (float)kCodeOne, zero[e][r]);
+          o.y = fmaf(o_acc[e][0][2 + r], (float)(kCodeOne / 16), zero[e][r]);
+          o.z = fmaf(o_acc[e][1][r], (float)kCodeOne, zero[e][r]);
+          o.w = fmaf(o_acc[e][1][2 + r], (float)(kCodeOne / 16), zero[e][r]);
+          *reinterpret_cast<float4*>(sm_o + (warp * kHg + h) * kD + 32 * e + 4 * grp) = o;
+        }
+      }
     }
   }
   __syncthreads();
-  merge_warps<HAS_V, BF16>(p, sm_m, sm_l, sm_o, kWarps4, b, g, split);
+  merge_warps<HAS_V, BF16>(p, sm_m, sm_l, sm_o, WARPS, b, g, split);
 }
 
-int init_decode4() { return 0; }
+template <bool DENSE, bool HAS_V>
+static int init_one() {
+  const int bytes = kWarps4 * stages4(HAS_V) * stage_bytes4(HAS_V);
+  KB_CUDA(cudaFuncSetAttribute(decode_attn4_kernel<DENSE, HAS_V, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  KB_CUDA(cudaFuncSetAttribute(decode_attn4_kernel<DENSE, HAS_V, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return 0;
+}
+
+int init_decode4() { return init_one<false, true>() || init_one<true, true>() || init_one<true, false>() ? -1 : 0; }
+
+// CTAs of 16 warps, one per SM, while the grid is small; of 8, two per SM, from 1.5 CTAs per SM on, as in decode.cu.
+template <bool DENSE, bool HAS_V>
+static cudaError_t launch(const DecodeParams& p, dim3 grid, cudaStream_t st) {
+  const long long total = (long long)grid.x * grid.y * grid.z;
+  const int warps = total * 2 >= 3ll * sm_count() ? kWarps4 / 2 : kWarps4;
+  const size_t smem = (size_t)warps * stages4(HAS_V) * stage_bytes4(HAS_V);
+  return launch_pdl(p.bf16 ? decode_attn4_kernel<DENSE, HAS_V, true> : decode_attn4_kernel<DENSE, HAS_V, false>, grid, warps * 32, smem,
+                    st, 1, p);
+}
 
 cudaError_t launch_attn4(const DecodeParams& p, bool dense, bool has_v, dim3 grid, cudaStream_t st) {
-  auto* kernel = !dense ? (p.bf16 ? decode_attn4_kernel<false, true, true> : decode_attn4_kernel<false, true, false>)
-                 : !has_v ? (p.bf16 ? decode_attn4_kernel<true, false, true> : decode_attn4_kernel<true, false, false>)
-                 : p.bf16 ? decode_attn4_kernel<true, true, true> : decode_attn4_kernel<true, true, false>;
-  return launch_pdl(kernel, grid, kWarps4 * 32, 0, st, 1, p);
+  return !dense ? launch<false, true>(p, grid, st) : has_v ? launch<true, true>(p, grid, st) : launch<true, false>(p, grid, st);
 }
 
 }  // namespace kb200

@@ -87,7 +87,7 @@ __device__ __forceinline__ uint2 quantize8(const H2* x, float scale) {
 // The 4-bit form of a row.  Called by the eight lanes of the row together, whose values are x[0..7] = 8c .. 8c+7 (group c / 4)
 // and x[8..15] = 64+8c .. 64+8c+7 (group 2 + c / 4), so a group lies in four lanes:
 //   z = fp16(min), s = fp16((max - z) / 15), c = round((x - z) / s) clamped to 0..15 (half to even, decided exactly).
-// What fp16 cannot hold saturates; a group with a value that is not finite gets z = NaN.  par[0..1]: scales of the two groups,
+// Values saturate at +-65504, what fp16 can hold; a group with a value that is not finite gets z = NaN.  par[0..1]: scales of the two groups,
 // par[2..3]: zeros; words: the eight codes of this lane in either group, the lowest nibble first.
 __device__ __forceinline__ void quantize_int4(const float (&x)[16], uint32_t (&words)[2], __half (&par)[4]) {
 #pragma unroll
@@ -106,7 +106,7 @@ __device__ __forceinline__ void quantize_int4(const float (&x)[16], uint32_t (&w
     }
     const __half zh = __float2half_rn(mx == INFINITY ? NAN : fminf(fmaxf(mn, -65504.f), 65504.f));
     const float z = __half2float(zh);
-    const __half sh = mx == INFINITY ? __float2half_rn(0.f) : __float2half_rn(fminf(fmaxf(__fdiv_rn(mx - z, 15.f), 0.f), 65504.f));
+    const __half sh = __float2half_rn(mx == INFINITY ? 0.f : fmaxf(__fdiv_rn(fminf(mx, 65504.f) - z, 15.f), 0.f));
     const float s = __half2float(sh), inv = s > 0.f ? 1.f / s : 0.f;
     uint32_t w = 0;
 #pragma unroll

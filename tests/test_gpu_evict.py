@@ -268,9 +268,10 @@ def test_a_conversation_in_a_4bit_cache_that_is_kept_short():
                 for b in range(B):
                     n = int(lens[b]) + 1
                     rows = table[b, torch.arange(n) // 16].long(), torch.arange(n) % 16
-                    kf, vf = (unpack(c.cpu()[rows], s.cpu()[rows], p) for c, s, p in ((k, kp, K_PIECES), (v, vp, V_PIECES)))
+                    kf, vf, vc = (unpack(c.cpu()[rows], s.cpu()[rows], p, z) for c, s, p, z in ((k, kp, K_PIECES, True), (v, vp, V_PIECES, True),
+                                                                                            (v, vp, V_PIECES, False)))
                     for h in range(G):
-                        want, _, p, bound, _ = attention(q[b, 0].cpu().double().view(G, 4, 128)[h], kf[:, h], vf[:, h], scale)
+                        want, _, p, bound, _ = attention(q[b, 0].cpu().double().view(G, 4, 128)[h], kf[:, h], vf[:, h], vc[:, h], scale)
                         off = (out[b].view(G, 4, 128)[h].cpu().double() - want).abs()
                         assert bool((off <= bound + 2.0 ** -11 * want.abs() + 2.0 ** -24).all())
                         before[b, :n] += p.sum(0)

@@ -122,7 +122,7 @@ def test_append_normalises_and_rotates_before_it_quantises(dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lens,G,page", [([1], 8, 16), ([33, 0, 17], 2, 16), ([5, 64], 3, 4)])
 def test_rows_are_read_back(dtype, lens, G, page):
-    k, v, kp, vp, table, kf, vf = make_cache(lens, G, page, seed=3)
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, page, seed=3)
     longest = max(lens)
     ko, vo = _strategy(G).read_kv(k, v, table, torch.tensor(lens, device="cuda"), longest, k_scale=kp, v_scale=vp, dtype=dtype)
     assert ko.shape == (len(lens), longest, G, 128) and ko.dtype == dtype
@@ -134,14 +134,14 @@ def test_rows_are_read_back(dtype, lens, G, page):
         assert bool(((got - want).abs() <= (HALF_STEP[dtype] + 2.0 ** -23) * want.abs()).all())
 
 
-def _check_attention(out, lse, q, kf, vf, rows_of, scale, dtype, what):
+def _check_attention(out, lse, q, kf, vf, vc, rows_of, scale, dtype, what):
     B, H, D = q.shape
     G = kf.shape[1]
     q = q.cpu().double().view(B, G, 4, D)
     for b in range(B):
         for g in range(G):
             rows = rows_of(b, g)
-            want, want_lse, _, bound, logit = attention(q[b, g], kf[b, g, rows], vf[b, g, rows], scale)
+            want, want_lse, _, bound, logit = attention(q[b, g], kf[b, g, rows], vf[b, g, rows], vc[b, g, rows], scale)
             got = out[b].view(G, 4, D)[g].cpu().double()
             off = (got - want).abs() - bound - HALF_STEP[dtype] * want.abs() - 2.0 ** -24
             assert bool((off <= 0).all()), f"{what} b{b} g{g} ({len(rows)} rows): {float(off.max()):.3g} too much"
@@ -165,7 +165,7 @@ def test_sparse_decode(dtype, splits, G, page):
     """Rows in any order, empty rows, counts at and around a tile's edge, a head map, strided index tensors."""
     from kascade_b200 import _native as nat
     lens = [700, 33, 1, 260]
-    k, v, kp, vp, table, kf, vf = make_cache(lens, G, page, seed=11, interleaved=page != 1)
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, page, seed=11, interleaved=page != 1)
     B, H, kmax = len(lens), 4 * G, 300
     g = torch.Generator().manual_seed(12)
     rows = torch.zeros(B, G, kmax + 5, dtype=torch.int32)
@@ -183,7 +183,7 @@ def test_sparse_decode(dtype, splits, G, page):
     ws = nat.decode_workspace(B, H, splits, q.device)
     rd = rows.cuda()[:, :, :kmax]
     nat.decode_sparse_paged(q, kv, rd, counts.cuda(), kmax, head_map.cuda(), 128 ** -0.5, out, lse, ws, splits)
-    _check_attention(out, lse, q, kf, vf, lambda b, h: rows[b, head_map[h], :counts[b, head_map[h]]].tolist(), 128 ** -0.5, dtype,
+    _check_attention(out, lse, q, kf, vf, vc, lambda b, h: rows[b, head_map[h], :counts[b, head_map[h]]].tolist(), 128 ** -0.5, dtype,
                      f"sparse, {splits} splits")
     if splits <= 3:
         again = torch.empty_like(out)
@@ -194,7 +194,7 @@ def test_sparse_decode(dtype, splits, G, page):
     out = torch.empty(2, H, 128, dtype=dtype, device="cuda")
     kv = nat.kv_layout_paged(k, v, table[:2], kp, vp, dtype)
     nat.decode_sparse_paged(q[:2], kv, full.cuda(), None, 33, None, 0.3, out, None, ws, splits)
-    _check_attention(out, None, q[:2], kf[:2], vf[:2], lambda b, h: full[b, h].tolist(), 0.3, dtype, "sparse, no counts")
+    _check_attention(out, None, q[:2], kf[:2], vf[:2], vc[:2], lambda b, h: full[b, h].tolist(), 0.3, dtype, "sparse, no counts")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -204,7 +204,7 @@ def test_sparse_decode(dtype, splits, G, page):
 def test_dense_decode(dtype, splits, has_v, lens):
     from kascade_b200 import _native as nat
     G = 2
-    k, v, kp, vp, table, kf, vf = make_cache(lens, G, 16, seed=21)
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, 16, seed=21)
     B, H, longest = len(lens), 4 * G, max(lens)
     q = _queries(B, H, dtype, 22)
     stride = -(-longest // 4) * 4
@@ -217,14 +217,14 @@ def test_dense_decode(dtype, splits, has_v, lens):
     seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
     nat.decode_anchor_paged(q, kv, seq, longest, 128 ** -0.5, logits, pooled, out, lse, ws, splits)
     if has_v:
-        _check_attention(out, lse, q, kf, vf, lambda b, h: list(range(lens[b])), 128 ** -0.5, dtype, f"dense, {splits} splits")
+        _check_attention(out, lse, q, kf, vf, vc, lambda b, h: list(range(lens[b])), 128 ** -0.5, dtype, f"dense, {splits} splits")
     mass = torch.rand(B, stride + 3, device="cuda")
     added = mass.clone()
     nat.mass_add(pooled, seq, mass, added, longest)
     for b, n in enumerate(lens):
         total = torch.zeros(n, dtype=torch.float64)
         for h in range(G):
-            _, want_lse, p, _, logit = attention(q[b].cpu().double().view(G, 4, 128)[h], kf[b, h, :n], vf[b, h, :n], 128 ** -0.5)
+            _, want_lse, p, _, logit = attention(q[b].cpu().double().view(G, 4, 128)[h], kf[b, h, :n], vf[b, h, :n], vc[b, h, :n], 128 ** -0.5)
             got = lse[b].view(G, 4)[h].cpu().double()
             if n:
                 assert float((got - want_lse).abs().max()) <= logit + 2.0 ** -22 * (1 + float(want_lse.abs().max()))
@@ -245,7 +245,7 @@ def test_decode_of_queries_of_any_size(dtype, size):
     """Very small queries (every row weighs the same) and very large ones (one row takes all)."""
     from kascade_b200 import _native as nat
     lens, G = [200], 2
-    k, v, kp, vp, table, kf, vf = make_cache(lens, G, 16, seed=31)
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, 16, seed=31)
     q = _queries(1, 8, dtype, 32, size)
     q[0, 3] = 0
     q[0, 5, 3] = 3e4                                                 # one element far above the others
@@ -253,7 +253,7 @@ def test_decode_of_queries_of_any_size(dtype, size):
     rows = torch.arange(200, dtype=torch.int32).expand(1, G, 200).contiguous()
     kv = nat.kv_layout_paged(k, v, table, kp, vp, dtype)
     nat.decode_sparse_paged(q, kv, rows.cuda(), None, 200, None, 128 ** -0.5, out, None, None, 1)
-    _check_attention(out, None, q, kf, vf, lambda b, h: list(range(200)), 128 ** -0.5, dtype, f"queries of {size}")
+    _check_attention(out, None, q, kf, vf, vc, lambda b, h: list(range(200)), 128 ** -0.5, dtype, f"queries of {size}")
 
 
 @pytest.mark.parametrize("size", [1e-3, 100.0], ids=["small", "large"])
@@ -266,20 +266,21 @@ def test_decode_of_values_of_any_size(size):
     vc, vp = quantize(x[1])
     k, v = pack(kc, K_PIECES), pack(vc, V_PIECES)
     table = torch.arange(21, dtype=torch.int32)[None]
-    kf, vf = (unpack(p, s, n).flatten(0, 1)[:, 0] for p, s, n in ((k, kp, K_PIECES), (v, vp, V_PIECES)))
+    kf, vf, vc = (unpack(p, s, n, z).flatten(0, 1)[None, None, :, 0] for p, s, n, z in ((k, kp, K_PIECES, True), (v, vp, V_PIECES, True),
+                                                                                     (v, vp, V_PIECES, False)))
     q = _queries(1, 4, torch.bfloat16, 42, 1.0 / size)
     out = torch.empty(1, 4, 128, dtype=torch.bfloat16, device="cuda")
     rows = torch.randperm(n, generator=g).to(torch.int32).view(1, 1, n)
     kv = nat.kv_layout_paged(k.cuda(), v.cuda(), table.cuda(), kp.cuda(), vp.cuda(), torch.bfloat16)
     nat.decode_sparse_paged(q, kv, rows.cuda(), None, n, None, 0.05, out, None, None, 1)
-    _check_attention(out, None, q, kf[None, None], vf[None, None], lambda b, h: list(range(n)), 0.05, torch.bfloat16, f"values of {size}")
+    _check_attention(out, None, q, kf, vf, vc, lambda b, h: list(range(n)), 0.05, torch.bfloat16, f"values of {size}")
 
 
 def test_layouts_and_strides_of_a_4bit_cache():
     """A contiguous [B, G, L, 64] cache, one that is a slice of a larger tensor, queries that are a slice: equal results."""
     from kascade_b200 import _native as nat
     lens, G = [150, 150], 2
-    k, v, kp, vp, table, kf, vf = make_cache(lens, G, 16, seed=51)
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, 16, seed=51)
     q_all = _queries(2, 16, torch.float16, 52)
     q = q_all[:, ::2]
     rows = torch.arange(150, dtype=torch.int32, device="cuda").expand(2, G, 150)
@@ -290,7 +291,7 @@ def test_layouts_and_strides_of_a_4bit_cache():
         return out
 
     want = run(nat.kv_layout_paged(k, v, table, kp, vp))
-    _check_attention(want, None, q, kf, vf, lambda b, h: list(range(150)), 0.1, torch.float16, "paged")
+    _check_attention(want, None, q, kf, vf, vc, lambda b, h: list(range(150)), 0.1, torch.float16, "paged")
     wide = [torch.zeros(k.shape[0], 16, G + 1, d, dtype=t, device="cuda") for d, t in ((128, torch.uint8), (32, torch.float16))]
     wide[0][:, :, 1:, :64], wide[0][:, :, 1:, 64:] = k, v
     wide[1][:, :, 1:, 8:16], wide[1][:, :, 1:, 16:24] = kp, vp
@@ -304,14 +305,14 @@ def test_steps_over_a_4bit_cache_through_the_strategy():
     """Anchor and reuse layers select and attend as over the values that the cache stands for."""
     from oracle.kascade_oracle import band_check, pooled_scores_decode, topk_budget
     lens, G, pct = [900, 1500], 2, 20
-    k, v, kp, vp, table, kf, vf = make_cache(lens, G, 16, seed=61)
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, 16, seed=61)
     strat = _strategy(G, pct, mapping=[1, 1])
     seq = torch.tensor(lens, device="cuda")
     q = [_queries(2, 8, torch.bfloat16, 62 + i) for i in range(2)]
     scale = 128 ** -0.5
     mass = torch.zeros(2, 1600, device="cuda")
     out = strat.paged_decode_forward(0, q[0], k, v, table, seq, scale, 1500, kp, vp, mean_seq_len=1200.0, attention_mass=mass)
-    _check_attention(out, None, q[0], kf, vf, lambda b, h: list(range(lens[b])), scale, torch.bfloat16, "layer 0")
+    _check_attention(out, None, q[0], kf, vf, vc, lambda b, h: list(range(lens[b])), scale, torch.bfloat16, "layer 0")
     idx, cnt = strat._dec_idx.cpu().clone(), strat._dec_count.cpu().clone()
     for b, n in enumerate(lens):
         pooled, _ = pooled_scores_decode(q[0][b:b + 1].float().cpu()[:, :, None], kf[b:b + 1, :, :n].float(), scale)
@@ -322,7 +323,7 @@ def test_steps_over_a_4bit_cache_through_the_strategy():
             ok, msg = band_check(pooled[0, h], idx[b, h, :cnt[b, h]].tolist(), int(cnt[b, h]), n)
             assert ok, msg
     out = strat.paged_decode_forward(1, q[1], k, v, table, seq, scale, 1500, kp, vp, attention_mass=mass)
-    _check_attention(out, None, q[1], kf, vf, lambda b, h: idx[b, 1, :cnt[b, 1]].tolist(), scale, torch.bfloat16, "layer 1")
+    _check_attention(out, None, q[1], kf, vf, vc, lambda b, h: idx[b, 1, :cnt[b, 1]].tolist(), scale, torch.bfloat16, "layer 1")
     # the same rows handed over by the caller; the strategy's own rows stay
     again = _strategy(G, pct, mapping=[1, 1]).paged_decode_forward(1, q[1], k, v, table, seq, scale, 1500, kp, vp,
                                                                    index_rows=(idx.cuda(), cnt.cuda()))
@@ -331,13 +332,13 @@ def test_steps_over_a_4bit_cache_through_the_strategy():
     short = torch.tensor([100, 128], device="cuda")
     strat.paged_decode_forward(0, q[0], k, v, table, short, scale, 128, kp, vp)
     out = strat.paged_decode_forward(1, q[1], k, v, table, short, scale, 128, kp, vp)
-    _check_attention(out, None, q[1], kf, vf, lambda b, h: list(range([100, 128][b])), scale, torch.bfloat16, "short")
+    _check_attention(out, None, q[1], kf, vf, vc, lambda b, h: list(range([100, 128][b])), scale, torch.bfloat16, "short")
 
 
 def test_a_step_over_a_4bit_cache_replays_from_a_cuda_graph():
     from kascade_b200 import rope_axis_map
     lens, G = [700, 41], 2
-    k, v, kp, vp, table, _, _ = make_cache([n + 1 for n in lens], G, 16, seed=71)
+    k, v, kp, vp, table, _, _, _ = make_cache([n + 1 for n in lens], G, 16, seed=71)
     strat = _strategy(G, 20, mapping=[1, 0])
     g = torch.Generator().manual_seed(72)
     q = torch.randn(2, 1, 8, 128, generator=g).half().cuda()
