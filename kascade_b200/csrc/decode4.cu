@@ -25,8 +25,10 @@ constexpr int kKeys4 = 32;                                 // keys of a step, on
 constexpr int kCodes4 = kKeys4 * kD / 2;                   // bytes of the codes of a step's K or V rows
 constexpr int kHalf4 = kCodes4 + kKeys4 * 16;              // ... with their parameters
 constexpr int kCodeOne = 1 << 24;                          // 1 / (the value of code 1 as an fp16 subnormal)
-constexpr float kShift4 = 2.f;                             // probabilities are at most 2^2: their products with a scale stay in fp16's
-                                                           // range (s <= 8734) and further away from its subnormals
+// A row's reference point for its exponentials moves only when a logit exceeds it by more than 2^kSlack4: probabilities are at
+// most 4, so that their products with a scale (s <= 8734) stay in fp16's range, and the maximum over the lanes, the
+// factors and the rescaling of O are needed in a few steps per list only.
+constexpr float kSlack4 = 2.f;
 __host__ __device__ constexpr int stages4(bool has_v) { return has_v ? 2 : 4; }
 __host__ __device__ constexpr int stage_bytes4(bool has_v) { return has_v ? 2 * kHalf4 : kHalf4; }
 
@@ -49,6 +51,10 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
 __device__ __forceinline__ float2 half2_floats(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
@@ -78,11 +84,11 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
   const int st_begin = min(split * per, nst), st_end = min(st_begin + per, nst);
   const int my_count = (st_end - st_begin - warp + WARPS - 1) / WARPS;                 // may be <= 0
 
-  // ---- queries: B operand Q^T[d][head], column = head grp (zero for grp >= 4) -----------------------
+  // ---- queries: B operand Q^T[d][head], columns 0-3 = heads 0-3, 4-7 = the same again ---------------
   // k-step (group e, half f): k = 2 quad, 2 quad + 1 are d = 32 e + 8 quad + {2f, 2f + 4}, k + 8 the d one further, whose codes
   // lie four bits further up: times 4 here, a quarter there
   uint32_t qb[4][2][2], zb0, zb1;
-  float c_head[2];                                         // scale * log2 e * 2^(exponent of the head's queries), heads 2 quad, + 1
+  float c_head[2];                                         // scale * log2 e * 2^(exponent of the head's queries), columns 2 quad, + 1
   {
     const __half* qp = p.q + b * p.q_stride_b + (int64_t)(g * kHg + (grp & 3)) * p.q_stride_h;
     float q[4][8], top = 0.f;
@@ -100,10 +106,10 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
     top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
     top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
     const int up = 6 - max((int)(__float_as_uint(top) >> 23) - 127, -90);   // exponent of the factor: -121 .. 96
-    const float factor = grp < kHg ? __uint_as_float((uint32_t)(up + 127) << 23) : 0.f;
+    const float factor = __uint_as_float((uint32_t)(up + 127) << 23);
     const float unit = p.scale2 * __uint_as_float((uint32_t)(127 - up) << 23);
-    c_head[0] = __shfl_sync(FULL, unit, (quad & 1) * 8);                    // heads 2 quad and 2 quad + 1 (the lanes of quads 2, 3
-    c_head[1] = __shfl_sync(FULL, unit, (quad & 1) * 8 + 4);                // hold the unused columns)
+    c_head[0] = __shfl_sync(FULL, unit, (quad & 1) * 8);
+    c_head[1] = __shfl_sync(FULL, unit, (quad & 1) * 8 + 4);
     float sum[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -193,6 +199,15 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
   }
   float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
 
+  // p s in fp16 for columns 0-3, and for columns 4-7 (the same heads) what its rounding left, exactly: the products with the
+  // codes, whose mean is far from zero, would carry the rounding of p s twice as far as that of p.  bf16 outputs are rounded
+  // ten times as coarsely and do without.
+  const uint32_t rest = grp < kHg ? 0u : 0xFFFFFFFFu;
+  auto scaled = [&](uint32_t pb, uint32_t s) -> uint32_t {
+    const uint32_t ps = mul_half2(pb, s);
+    return BF16 ? ps : fma_half2(pb, s, (ps ^ 0x80008000u) & rest);
+  };
+
   for (int j = 0; j < my_count; ++j) {
     __syncwarp();                      // every lane is done with the buffer about to be refilled
     issue(j + kStages - 1, pos_a, page_a);
@@ -248,31 +263,21 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
         if (key0 + 16 * i + grp + 8 < n) { lp[16 * i + 8] = x[i][2]; lp[p.logit_stride + 16 * i + 8] = x[i][3]; }
       }
     }
-    // ---- running maximum and sum, per lane for its two heads ---------------------------------------------
+    // ---- exponentials against the reference of either head ---------------------------------------------
     float t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])), t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
+    if (__any_sync(FULL, t0 > m_run[0] + kSlack4 || t1 > m_run[1] + kSlack4)) {     // (the first step: it has a valid key)
 #pragma unroll
-    for (int sh = 4; sh <= 16; sh <<= 1) {
-      t0 = fmaxf(t0, __shfl_xor_sync(FULL, t0, sh));
-      t1 = fmaxf(t1, __shfl_xor_sync(FULL, t1, sh));
-    }
-    const float m0 = fmaxf(m_run[0], t0 - kShift4), m1 = fmaxf(m_run[1], t1 - kShift4);   // every step has a valid key
-    const float alpha0 = ex2(m_run[0] - m0), alpha1 = ex2(m_run[1] - m1);
-    m_run[0] = m0;
-    m_run[1] = m1;
-    float w[2][4], sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      w[i][0] = ex2(x[i][0] - m0);
-      w[i][1] = ex2(x[i][1] - m1);
-      w[i][2] = ex2(x[i][2] - m0);
-      w[i][3] = ex2(x[i][3] - m1);
-      sum0 += w[i][0] + w[i][2];
-      sum1 += w[i][1] + w[i][3];
-    }
-    l_part[0] = l_part[0] * alpha0 + sum0;
-    l_part[1] = l_part[1] * alpha1 + sum1;
-    if (HAS_V) {
-      if (!__all_sync(FULL, alpha0 == 1.f && alpha1 == 1.f)) {           // a factor of exactly 1 changes nothing
+      for (int sh = 4; sh <= 16; sh <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(FULL, t0, sh));
+        t1 = fmaxf(t1, __shfl_xor_sync(FULL, t1, sh));
+      }
+      const float m0 = t0 > m_run[0] + kSlack4 ? t0 : m_run[0], m1 = t1 > m_run[1] + kSlack4 ? t1 : m_run[1];
+      const float alpha0 = ex2(m_run[0] - m0), alpha1 = ex2(m_run[1] - m1);
+      m_run[0] = m0;
+      m_run[1] = m1;
+      l_part[0] *= alpha0;
+      l_part[1] *= alpha1;
+      if (HAS_V) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -282,6 +287,16 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
         }
         o_zero[0] *= alpha0; o_zero[1] *= alpha1; o_zero[2] *= alpha0; o_zero[3] *= alpha1;
       }
+    }
+    float w[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) w[i][r] = ex2(x[i][r] - m_run[r & 1]);
+    }
+    l_part[0] += (w[0][0] + w[0][2]) + (w[1][0] + w[1][2]);
+    l_part[1] += (w[0][1] + w[0][3]) + (w[1][1] + w[1][3]);
+    if (HAS_V) {
       // ---- O^T += V^T P^T -------------------------------------------------------------------------------
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -298,8 +313,8 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
           const uint32_t sel = (e & 1) ? 0x7632 : 0x5410;
           const uint32_t lo = __byte_perm(e < 2 ? ka.x : ka.y, e < 2 ? kb.x : kb.y, sel);      // keys 2 quad, 2 quad + 1
           const uint32_t hi = __byte_perm(e < 2 ? kc.x : kc.y, e < 2 ? kd.x : kd.y, sel);      // ... + 8
-          const uint32_t sb0 = mul_half2(pb0, __shfl_sync(FULL, z0, e * 4 + quad));
-          const uint32_t sb1 = mul_half2(pb1, __shfl_sync(FULL, z1, e * 4 + quad));
+          const uint32_t sb0 = scaled(pb0, __shfl_sync(FULL, z0, e * 4 + quad));
+          const uint32_t sb1 = scaled(pb1, __shfl_sync(FULL, z1, e * 4 + quad));
           mma16816<false>(o_acc[e][0], lo & 0x000F000Fu, lo & 0x00F000F0u, hi & 0x000F000Fu, hi & 0x00F000F0u, sb0, sb1);
           const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
           mma16816<false>(o_acc[e][1], lo8 & 0x000F000Fu, lo8 & 0x00F000F0u, hi8 & 0x000F000Fu, hi8 & 0x00F000F0u, sb0, sb1);
@@ -320,6 +335,16 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
   float* sm_l = sm_m + WARPS * kHg;                              // [warps][4]
   float* sm_o = sm_l + WARPS * kHg;                              // [warps][4][128]
   float zero[4][2];
+  if (HAS_V && !BF16) {                                          // the rests, columns 4-7, to their heads
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o_acc[e][0][i] += __shfl_down_sync(FULL, o_acc[e][0][i], 2);
+        o_acc[e][1][i] += __shfl_down_sync(FULL, o_acc[e][1][i], 2);
+      }
+    }
+  }
   if (HAS_V) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
