@@ -1,6 +1,8 @@
 // Eviction from a KV cache by accumulated attention weight: the weight that rows collect in prompts and decode steps, the
 // choice of the rows that stay, and the moves that bring them together.  The declarations in kascade_b200.h say what each
 // entry point computes; the reference has no counterpart.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace kb200 {
@@ -33,22 +35,71 @@ struct PromptMassParams {
   int G, T, n_rows;
 };
 
-// One column of four rows per thread, over all heads and tiles.
-__global__ void __launch_bounds__(64) mass_prompt_kernel(const PromptMassParams p) {
+// 128 rows of the cache, four per lane, are a block; the pooled scores of a block are one piece of 512 bytes per head and later
+// tile, which a cluster of CTAs deals to its warps, eight loads in flight each.  The first rows have the most later tiles and the
+// last none, so a cluster takes the i-th block from the front and the i-th from the back: equal work everywhere.  A lane
+// adds its pieces up one after the other, the warps' and the CTAs' sums meet in the order of their numbers, so a call
+// gives the same bits every time.
+constexpr int kMassWarps = 16;
+constexpr int kMassUnroll = 8;
+__global__ void __launch_bounds__(kMassWarps * 32) mass_prompt_kernel(const PromptMassParams p) {
+  namespace cg = cooperative_groups;
   pdl_begin();
-  const int b = blockIdx.y, j = (blockIdx.x * 64 + threadIdx.x) * 4;
-  if (j >= p.n_rows) return;
+  __shared__ float4 sums[kMassWarps][32];
+  __shared__ float total[2][128];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tiles = p.seq_len ? min((max(p.seq_len[b], 0) + kTile - 1) / kTile, p.T) : p.T;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int t = j / kTile + 1; t < tiles; ++t) {                   // j is a multiple of 4: its four rows lie in one tile
-    for (int g = 0; g < p.G; ++g) {
-      const float4 x = *reinterpret_cast<const float4*>(p.pooled + (((int64_t)b * p.G + g) * p.T + t) * p.row_stride + j);
-      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+  const int blocks = (p.n_rows + 127) / 128, front = blockIdx.x / ctas, back = blocks - 1 - front;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    const int block = half ? back : front;
+    const int j = block * 128 + lane * 4, own = j / kTile;         // (the same tile for a lane's four rows)
+    const int first = block * 4 + 1;                                // the first tile behind the first of these rows
+    const int later = half && back == front ? 0 : max(tiles - first, 0), pieces = later * p.G, step = ctas * kMassWarps;
+    const float* rows = p.pooled + (int64_t)b * p.G * p.T * p.row_stride + j;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = rank * kMassWarps + warp; i0 < pieces; i0 += step * kMassUnroll) {
+      float4 x[kMassUnroll];
+#pragma unroll
+      for (int u = 0; u < kMassUnroll; ++u) {
+        const int i = i0 + u * step, g = i / later, t = first + i - g * later;
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < pieces && t > own) x[u] = *reinterpret_cast<const float4*>(rows + ((int64_t)g * p.T + t) * p.row_stride);
+      }
+#pragma unroll
+      for (int u = 0; u < kMassUnroll; ++u) { a.x += x[u].x; a.y += x[u].y; a.z += x[u].z; a.w += x[u].w; }
     }
+    sums[warp][lane] = a;
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kMassWarps; ++w) s += reinterpret_cast<const float*>(sums[w])[threadIdx.x];
+      total[half][threadIdx.x] = s;
+    }
+    __syncthreads();
   }
-  const float s[4] = {a.x, a.y, a.z, a.w};
-  for (int e = 0; e < 4 && j + e < p.n_rows; ++e)
-    p.mass_out[b * p.out_stride + j + e] = p.mass_in[b * p.in_stride + j + e] + s[e];
+  cluster.sync();
+  const int half = threadIdx.x >> 7, at = threadIdx.x & 127;
+  if (rank == 0 && half < (back == front ? 1 : 2)) {
+    float s = total[half][at];
+    for (int r = 1; r < ctas; ++r) s += cluster.map_shared_rank(&total[0][0], r)[half * 128 + at];
+    const int i = (half ? back : front) * 128 + at;
+    if (i < p.n_rows) p.mass_out[b * p.out_stride + i] = p.mass_in[b * p.in_stride + i] + s;
+  }
+  cluster.sync();                                                  // the sums have been read
+}
+
+// CTAs that share two blocks: doubled while all of them together are at most two per SM.  512 threads with eight loads each
+// keep enough in flight then, and a second round of CTAs would leave SMs idle at its end.  us with at most two / four CTAs per
+// SM: one prompt of 32768 rows 95 / 102 (5.7 TB/s, 0.88 of the copy), 16384 30.5 / 38.4, 8192 13.8 / 13.6, 8 x 4096 18.8 / 24.6,
+// 4 x 3001 11.9 / 17.3.  (A thread per four rows, over all heads and tiles: 1995 us for 32768 rows.)
+static int mass_ctas(int64_t clusters) {
+  int c = 1;
+  while (c < 8 && clusters * c <= sm_count()) c *= 2;
+  return c;
 }
 
 // ---- what stays ------------------------------------------------------------------------------------------------------
@@ -195,8 +246,9 @@ extern "C" int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, co
   KB_REQUIRE(n_rows >= need, "mass_add_prompt: mass holds %d rows, %d tiles need %lld", n_rows, num_tiles, (long long)need);
   if (batch == 0 || n_rows == 0) return 0;
   PromptMassParams p{pooled, row_stride, seq_len, mass_in, mass_out, mass_in_stride, mass_out_stride, num_kv_heads, num_tiles, n_rows};
-  KB_LAUNCH("mass_prompt_kernel",
-            launch_pdl(mass_prompt_kernel, dim3(ceil_div(n_rows, 256), batch), 64, 0, (cudaStream_t)stream, 1, p));
+  const int clusters = ceil_div(n_rows, 256), ctas = mass_ctas((int64_t)clusters * batch);
+  KB_LAUNCH("mass_prompt_kernel", launch_pdl(mass_prompt_kernel, dim3(clusters * ctas, batch), kMassWarps * 32, 0, (cudaStream_t)stream,
+                                             ctas, p));
   return 0;
 }
 
