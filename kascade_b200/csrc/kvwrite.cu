@@ -45,6 +45,7 @@ struct KvWriteParams {
   // the first axis is noted per cache row, [B, rows], or null
   const int32_t* positions; int64_t ps_axis, ps_b; const int32_t* pair_axis; int axes;
   int32_t* token_positions; int64_t tp_sb; int tp_rows;
+  int tokens;                                                         // kv_append_kernel: tokens of a CTA
 };
 
 // One CTA per (sequence, new token): the token's 64 (cos, sin) pairs are computed once and shared by all
@@ -84,53 +85,46 @@ __device__ __forceinline__ uint2 quantize8(const H2* x, float scale) {
   return make_uint2(w[0], w[1]);
 }
 
-// The 4-bit form of a row.  Called by the eight lanes of the row together, whose values are x[0..7] = 8c .. 8c+7 (group c / 4)
-// and x[8..15] = 64+8c .. 64+8c+7 (group 2 + c / 4), so a group lies in four lanes:
-//   z = fp16(min), s = fp16((max - z) / 15), c = round((x - z) / s) clamped to 0..15 (half to even, decided exactly).
-// Values saturate at +-65504, what fp16 can hold; a group with a value that is not finite gets z = NaN.  par[0..1]: scales of the two groups,
-// par[2..3]: zeros; words: the eight codes of this lane in either group, the lowest nibble first.
-__device__ __forceinline__ void quantize_int4(const float (&x)[16], uint32_t (&words)[2], __half (&par)[4]) {
+// the norm's second half and the rotation as the Hugging Face modules round them; eight lanes per row, r = 1 / rms of the row
+template <bool BF16>
+__device__ __forceinline__ void module_norm(typename Pair<BF16>::T* lo, typename Pair<BF16>::T* hi, const __half* gain, float r, int c) {
+  using H2 = typename Pair<BF16>::T;
+  // x.float() * rsqrt(mean(x^2) + eps), rounded to the storage type, times the gain (a product in that type)
+  const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
+  const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
+  const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
+  const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float mn = INFINITY, mx = -INFINITY;
+  for (int e = 0; e < 4; ++e) {
+    const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
+    lo[e] = __hmul2_rn(g_lo[e], from_f2<BF16>(a.x * r, a.y * r));
+    hi[e] = __hmul2_rn(g_hi[e], from_f2<BF16>(d2.x * r, d2.y * r));
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void module_rotate(typename Pair<BF16>::T* lo, typename Pair<BF16>::T* hi, const typename Pair<BF16>::S* cos_s,
+                                              const typename Pair<BF16>::S* sin_s, int c) {
+  using H2 = typename Pair<BF16>::T;
+  const uint4 cs4 = reinterpret_cast<const uint4*>(cos_s)[c];
+  const uint4 sn4 = reinterpret_cast<const uint4*>(sin_s)[c];
+  const H2* cs = reinterpret_cast<const H2*>(&cs4);
+  const H2* sn = reinterpret_cast<const H2*>(&sn4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = x[i * 8 + e];
-      mn = fminf(mn, v);
-      mx = fabsf(v) < INFINITY ? fmaxf(mx, v) : INFINITY;                    // (also where v is a NaN)
-    }
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-      mn = fminf(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, o));
-      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-    }
-    const __half zh = __float2half_rn(mx == INFINITY ? NAN : fminf(fmaxf(mn, -65504.f), 65504.f));
-    const float z = __half2float(zh);
-    const __half sh = __float2half_rn(mx == INFINITY ? 0.f : fmaxf(__fdiv_rn(fminf(mx, 65504.f) - z, 15.f), 0.f));
-    const float s = __half2float(sh), inv = s > 0.f ? 1.f / s : 0.f;
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = x[i * 8 + e] - z;
-      float c = rintf(a * inv);
-      const float rest = fmaf(-c, s, a);                                    // the product alone may be on the wrong side
-      if (s > 0.f && (fabsf(rest) > 0.5f * s || (fabsf(rest) == 0.5f * s && ((int)c & 1)))) c += copysignf(1.f, rest);
-      w |= (uint32_t)(int)fminf(fmaxf(c, 0.f), 15.f) << (4 * e);             // (a NaN becomes 0)
-    }
-    words[i] = w;
-    par[i] = sh;
-    par[2 + i] = zh;
+  for (int e = 0; e < 4; ++e) {
+    // first half:  x_lo * cos + (-x_hi) * sin ; second half:  x_hi * cos + x_lo * sin
+    // (the _rn forms are never contracted into a fused multiply-add, which would skip a rounding)
+    const H2 new_lo = __hadd2_rn(__hmul2_rn(lo[e], cs[e]), __hmul2_rn(__hneg2(hi[e]), sn[e]));
+    const H2 new_hi = __hadd2_rn(__hmul2_rn(hi[e], cs[e]), __hmul2_rn(lo[e], sn[e]));
+    lo[e] = new_lo;
+    hi[e] = new_hi;
   }
 }
 
-// How a row is stored, and whether its token has a position of its own (kb200_kv_write_at)
-constexpr int kSame = 0, kFp8 = 1, kInt4 = 2;
-
 // CTAS: CTAs per SM that the registers have to allow (0: left to the compiler); see launch_kv_write
-template <bool BF16, int STORE, bool AT, int CTAS>
+template <bool BF16, bool FP8, int CTAS>
 __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const KvWriteParams p) {
   using H2 = typename Pair<BF16>::T;
-  using H1 = typename std::conditional<AT, float, typename Pair<BF16>::S>::type;
+  using H1 = typename Pair<BF16>::S;
   __shared__ __align__(16) H1 cos_s[kD / 2];
   __shared__ __align__(16) H1 sin_s[kD / 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -153,26 +147,11 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
   uint4 next_lo = make_uint4(0u, 0u, 0u, 0u), next_hi = next_lo;
   if (warp * 4 < heads) load_rows(warp * 4, next_lo, next_hi);
   const int pos = p.start_pos[b] + t;
-  if constexpr (AT) {
-    const int32_t* own_pos = p.positions + b * p.ps_b + t;
-    if (p.inv_freq && tid < kD / 2) {
-      const int axis = p.pair_axis ? min(max(p.pair_axis[tid], 0), p.axes - 1) : 0;
-      constexpr double kTurn = 6.283185307179586476925;
-      double angle = (double)own_pos[axis * p.ps_axis] * (double)p.inv_freq[tid];
-      angle -= rint(angle * (1.0 / kTurn)) * kTurn;
-      float sn, cs;
-      sincosf((float)angle, &sn, &cs);
-      cos_s[tid] = cs * p.rope_scale;
-      sin_s[tid] = sn * p.rope_scale;
-    }
-    if (tid == 0 && p.token_positions && pos < p.tp_rows) p.token_positions[b * p.tp_sb + pos] = own_pos[0];
-  } else {
-    if (p.inv_freq && tid < kD / 2) {
-      float sn, cs;
-      sincosf((float)pos * p.inv_freq[tid], &sn, &cs);
-      cos_s[tid] = from_f<BF16>(cs * p.rope_scale);
-      sin_s[tid] = from_f<BF16>(sn * p.rope_scale);
-    }
+  if (p.inv_freq && tid < kD / 2) {
+    float sn, cs;
+    sincosf((float)pos * p.inv_freq[tid], &sn, &cs);
+    cos_s[tid] = from_f<BF16>(cs * p.rope_scale);
+    sin_s[tid] = from_f<BF16>(sn * p.rope_scale);
   }
   __syncthreads();
   for (int h0 = warp * 4; h0 < heads; h0 += kStep) {                 // uniform per warp
@@ -194,94 +173,19 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
     }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-    float x[16];                                                     // AT, INT4: the row in fp32
-    if constexpr (AT) {
-      const float r = gain ? rsqrtf(ss / kD + p.eps) : 1.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
-        x[2 * e] = a.x * r; x[2 * e + 1] = a.y * r;
-        x[8 + 2 * e] = d2.x * r; x[8 + 2 * e + 1] = d2.y * r;
-      }
-      if (gain) {
-        const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
-        const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
-        const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
-        const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 a = to_f2(g_lo[e]), d2 = to_f2(g_hi[e]);
-          x[2 * e] *= a.x; x[2 * e + 1] *= a.y;
-          x[8 + 2 * e] *= d2.x; x[8 + 2 * e + 1] *= d2.y;
-        }
-      }
-      if (kind != 2 && p.inv_freq) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float cs = cos_s[c * 8 + e], sn = sin_s[c * 8 + e], l = x[e], h2 = x[8 + e];
-          x[e] = l * cs - h2 * sn;
-          x[8 + e] = h2 * cs + l * sn;
-        }
-      }
-      if (STORE != kInt4 || kind == 0) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          lo[e] = from_f2<BF16>(x[2 * e], x[2 * e + 1]);
-          hi[e] = from_f2<BF16>(x[8 + 2 * e], x[8 + 2 * e + 1]);
-        }
-      }
-    } else {
-      if (gain) {
-        // x.float() * rsqrt(mean(x^2) + eps), rounded to the storage type, times the gain (a product in that type)
-        const float r = rsqrtf(ss / kD + p.eps);
-        const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
-        const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
-        const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
-        const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
-          lo[e] = __hmul2_rn(g_lo[e], from_f2<BF16>(a.x * r, a.y * r));
-          hi[e] = __hmul2_rn(g_hi[e], from_f2<BF16>(d2.x * r, d2.y * r));
-        }
-      }
-      if (kind != 2 && p.inv_freq) {
-        const uint4 cs4 = reinterpret_cast<const uint4*>(cos_s)[c];
-        const uint4 sn4 = reinterpret_cast<const uint4*>(sin_s)[c];
-        const H2* cs = reinterpret_cast<const H2*>(&cs4);
-        const H2* sn = reinterpret_cast<const H2*>(&sn4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          // first half:  x_lo * cos + (-x_hi) * sin ; second half:  x_hi * cos + x_lo * sin
-          // (the _rn forms are never contracted into a fused multiply-add, which would skip a rounding)
-          const H2 new_lo = __hadd2_rn(__hmul2_rn(lo[e], cs[e]), __hmul2_rn(__hneg2(hi[e]), sn[e]));
-          const H2 new_hi = __hadd2_rn(__hmul2_rn(hi[e], cs[e]), __hmul2_rn(lo[e], sn[e]));
-          lo[e] = new_lo;
-          hi[e] = new_hi;
-        }
-      }
+    if (gain) {
+      module_norm<BF16>(lo, hi, gain, rsqrtf(ss / kD + p.eps), c);
     }
-    __half* dst = nullptr;
-    bool code_rows = false;                                          // this lane's row goes to an INT4 cache
-    int64_t row4 = 0, par4 = 0;
+    if (kind != 2 && p.inv_freq) {
+      module_rotate<BF16>(lo, hi, cos_s, sin_s, c);
+    }
+    __half* dst;
     if (kind == 0) {
       dst = p.q_out + (((int64_t)b * p.T + t) * p.H + hh) * kD;
     } else {
       const int page = pos >> p.page_shift, slot = pos & p.page_mask;
       const int64_t phys = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + page] : page;
-      if constexpr (STORE == kInt4) {
-        if constexpr (!AT) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
-            x[2 * e] = a.x; x[2 * e + 1] = a.y;
-            x[8 + 2 * e] = d2.x; x[8 + 2 * e + 1] = d2.y;
-          }
-        }
-        code_rows = true;
-        row4 = phys * p.c_sp + slot * p.c_st + hh * p.c_sh + b * p.c_sb;
-        par4 = phys * p.pa_sp + slot * p.pa_st + hh * p.pa_sh + b * p.pa_sb;
-      } else if constexpr (STORE == kFp8) {
+      if (FP8) {
         if (active) {
           const float sc = (kind == 1 ? p.k_scale : p.v_scale)[b * p.s_sb + phys * p.s_sp + hh * p.s_sh];
           uint8_t* d8 = reinterpret_cast<uint8_t*>(kind == 1 ? p.k_cache : p.v_cache) + b * p.c_sb + phys * p.c_sp +
@@ -291,35 +195,9 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
         }
         continue;
       }
-      if constexpr (STORE != kInt4) dst = (kind == 1 ? p.k_cache : p.v_cache) + b * p.c_sb + phys * p.c_sp + slot * p.c_st + hh * p.c_sh;
+      dst = (kind == 1 ? p.k_cache : p.v_cache) + b * p.c_sb + phys * p.c_sp + slot * p.c_st + hh * p.c_sh;
     }
-    if constexpr (STORE == kInt4) {
-      // all lanes of the warp take part in the shuffles; rows of Q among them come to nothing
-      uint32_t words[2];
-      __half par[4];
-      quantize_int4(x, words, par);
-      if (code_rows && active) {
-        const int g = c >> 2, q = c & 3;                             // groups g and g + 2, values 8q .. 8q+7 of either
-        if (kind == 1) {
-          uint8_t* row = reinterpret_cast<uint8_t*>(p.k_cache) + row4;
-          *reinterpret_cast<uint32_t*>(row + q * 16 + g * 4) = words[0];
-          *reinterpret_cast<uint32_t*>(row + q * 16 + (g + 2) * 4) = words[1];
-        } else {
-          uint8_t* row = reinterpret_cast<uint8_t*>(p.v_cache) + row4;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            *reinterpret_cast<uint16_t*>(row + (2 * q) * 8 + (g + 2 * i) * 2) = (uint16_t)words[i];
-            *reinterpret_cast<uint16_t*>(row + (2 * q + 1) * 8 + (g + 2 * i) * 2) = (uint16_t)(words[i] >> 16);
-          }
-        }
-        if (q == 0) {
-          __half* pr = (kind == 1 ? p.k_param : p.v_param) + par4;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) { pr[g + 2 * i] = par[i]; pr[4 + g + 2 * i] = par[2 + i]; }
-        }
-      }
-    }
-    if (active && !code_rows) {
+    if (active) {
       reinterpret_cast<uint4*>(dst)[c] = lo4;
       reinterpret_cast<uint4*>(dst + kD / 2)[c] = hi4;
     }
@@ -331,14 +209,328 @@ __global__ void __launch_bounds__(kKvWriteThreads, CTAS) kv_write_kernel(const K
 // hold the missing CTA costs time: those are compiled for seven per SM.  Measured before the loads ahead / with them /
 // as it is now, us without Q, with and without rotary table: 32768 tokens 61.0 / 66.5 / 58.3, 56.0 / 63.2 / 54.3; 16 x 600
 // 20.7 / 22.0 / 19.2, 19.2 / 21.2 / 18.2; 64 tokens 2.45 / 2.51 / 2.51, 2.26 / 2.26 / 2.26.
-template <bool BF16, int STORE>
+template <bool BF16, bool FP8>
 static void launch_kv_write(const KvWriteParams& p, int64_t blocks, cudaStream_t st) {
-  if (p.positions)
-    kv_write_kernel<BF16, STORE, true, 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
-  else if (STORE != kInt4 && p.H + 2 * p.G <= kKvWriteThreads / 32 * 4 && blocks > 6ll * sm_count())
-    kv_write_kernel<BF16, STORE, false, STORE != kInt4 ? 7 : 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
+  if (p.H + 2 * p.G <= kKvWriteThreads / 32 * 4 && blocks > 6ll * sm_count())
+    kv_write_kernel<BF16, FP8, 7><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
   else
-    kv_write_kernel<BF16, STORE, false, 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
+    kv_write_kernel<BF16, FP8, 0><<<(unsigned)blocks, kKvWriteThreads, 0, st>>>(p);
+}
+
+// ---- appends that quantise to 4 bits, or whose tokens have positions of their own ---------------------
+// Eight lanes share a row; lane c has its values 8c .. 8c+7 (four pairs x[0..3], group c / 4) and 64+8c .. 64+8c+7 (x[4..7],
+// group 2 + c / 4), so a group of 32 lies in four lanes.
+
+// pairs of fp32 numbers, for the two-element instructions: these kernels are bound by issue slots
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("sub.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// the ends of the two groups over a lane's eight values of either, as the row's own type or in fp32; a value that is not finite
+// makes the upper end infinite or a NaN
+template <bool BF16>
+__device__ __forceinline__ void group_ends(const uint4& v, float& mn, float& mx) {
+  using H2 = typename Pair<BF16>::T;
+  const H2* h = reinterpret_cast<const H2*>(&v);
+  const float2 lo = to_f2(__hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3])));
+  const float2 hi = to_f2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+  mn = fminf(lo.x, lo.y);
+  mx = hi.x == hi.x && hi.y == hi.y && mn > -INFINITY ? fmaxf(hi.x, hi.y) : INFINITY;
+}
+__device__ __forceinline__ void group_ends(const uint64_t* x, float& mn, float& mx) {
+  uint64_t bad = 0;
+  mn = INFINITY;
+  mx = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 v = unpack2(x[e]);
+    mn = fminf(mn, fminf(v.x, v.y));
+    mx = fmaxf(mx, fmaxf(v.x, v.y));
+    bad = fma2(x[e], 0, bad);                                                  // a NaN if one is not finite
+  }
+  const float2 b = unpack2(bad);
+  if (!(b.x + b.y == 0.f)) mx = INFINITY;
+}
+
+// The 4-bit form of a lane's eight values x of a group whose ends over the lane are mn, mx:
+//   z = fp16(min), s = fp16((max - z) / 15), c = round((x - z) / s) clamped to 0..15, half to even.
+// Values saturate at +-65504, what fp16 can hold; a group with a value that is not finite gets z = NaN.  Returns the eight
+// codes, the lowest nibble first.
+// A quotient is a product with 1 / s (good to 2^-22) and one step of correction by the remainder, which is exact: so quotients that
+// are a number of 24 bits come out as that number, halves among them, and are rounded by adding 1.5 2^23.  (Halves are not rare,
+// 0.07 % of bf16 values, because x, z and s have few bits; testing for them took as long as the division.)  The eight sums add up
+// to the packed codes and a constant.  Clamping is needed only where fp16 rounds an end by a good part of a step.
+__device__ __forceinline__ uint32_t quantize_int4(const uint64_t* x, float mn, float mx, __half& sh, __half& zh) {
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, o));
+    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+  }
+  const bool fine = mx < INFINITY;
+  zh = __float2half_rn(fine ? fminf(fmaxf(mn, -65504.f), 65504.f) : NAN);
+  const float z = __half2float(zh);
+  // (max - z) / 15, rounded once, in the same way (checked for every significand)
+  const float span = fmaxf(fminf(mx, 65504.f) - z, 0.f), q0 = span * (1.f / 15.f);
+  sh = __float2half_rn(fine ? fmaf(fmaf(-15.f, q0, span), 1.f / 15.f, q0) : 0.f);
+  const float s = __half2float(sh);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(s));
+  constexpr float kMagic = 12582912.f;                                          // 1.5 2^23: sums are rounded to whole numbers
+  const uint64_t z2 = pack2(z, z), inv2 = pack2(inv, inv), magic2 = pack2(kMagic, kMagic), minus_s2 = pack2(-s, -s);
+  const bool clamp = !(mn - z > -0.4f * s && mx - z < 15.4f * s);               // (also where s is 0, or z a NaN)
+  uint32_t w = 0u - 0x4B400000u * 0x11111111u;                                  // 0x4B400000: the bits of kMagic
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint64_t a = sub2(x[e], z2), q = mul2(a, inv2);
+    uint64_t u = add2(fma2(fma2(q, minus_s2, a), inv2, q), magic2);
+    if (clamp) {                                                                // (a NaN becomes 0, and so does all of it where s is 0)
+      const float2 v = unpack2(u);
+      u = pack2(fminf(fmaxf(s > 0.f ? v.x : 0.f, kMagic), kMagic + 15.f), fminf(fmaxf(s > 0.f ? v.y : 0.f, kMagic), kMagic + 15.f));
+    }
+    const float2 v = unpack2(u);
+    w += (__float_as_uint(v.x) << (8 * e)) + (__float_as_uint(v.y) << (8 * e + 4));
+  }
+  return w;
+}
+
+// How a row is stored
+constexpr int kSame = 0, kFp8 = 1, kInt4 = 2;
+constexpr int kAppendThreads = 64;
+constexpr int kAppendTokens = 4;                                               // tokens of a CTA at most
+
+// Eight lanes take an item: the K and the V row of a (token, KV head), whose places in the cache are the same, or two Q rows of a
+// token.  A CTA takes p.tokens tokens and has, as a rule, eight lanes for each of their items: all rows are loaded at once,
+// before the angles are computed.  AT: positions of their own.
+template <bool BF16, int STORE, bool AT>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWriteParams p) {
+  using H2 = typename Pair<BF16>::T;
+  using Angle = typename std::conditional<AT, float, typename Pair<BF16>::S>::type;
+  __shared__ __align__(16) Angle cos_s[kAppendTokens][kD / 2];
+  __shared__ __align__(16) Angle sin_s[kAppendTokens][kD / 2];
+  __shared__ int64_t page_s[kAppendTokens];
+  __shared__ int slot_s[kAppendTokens];
+  const int tid = threadIdx.x, c = tid & 7;
+  const int per = p.G + (p.H + 1) / 2, items = p.tokens * per;       // items of a token: KV heads first, then pairs of Q heads
+  const uint32_t first = blockIdx.x * (uint32_t)p.tokens, all = (uint32_t)p.B * p.T;
+  for (int item0 = 0; item0 < items; item0 += blockDim.x >> 3) {     // uniform for the CTA
+    const int item = item0 + (tid >> 3);
+    const int i = (item >= per) + (item >= 2 * per) + (item >= 3 * per), h = item - i * per;
+    static_assert(kAppendTokens == 4, "three comparisons");
+    const uint32_t token = first + i;
+    const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * p.T);
+    const bool active = item < items && token < all && (!p.n_new || t < p.n_new[b]);
+    const bool kv = h < p.G;
+    const int head = kv ? h : 2 * (h - p.G);
+    const bool two = kv || head + 1 < p.H;
+    uint4 row[2][2];                                                    // (all lanes take part in the shuffles)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      row[r][0] = row[r][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (!active || (r && !two)) continue;
+      const __half* src = !kv ? p.q_in + b * p.q_sb + t * p.q_st + (head + r) * p.q_sh
+                              : r == 0 ? p.k_new + b * p.k_sb + t * p.k_st + head * p.k_sh
+                                       : p.v_new + b * p.v_sb + t * p.v_st + head * p.v_sh;
+      row[r][0] = reinterpret_cast<const uint4*>(src)[c];
+      row[r][1] = reinterpret_cast<const uint4*>(src + kD / 2)[c];
+    }
+    if (item0 == 0) {
+      // the tokens' places in the cache, and their angles
+      for (int at = tid; at < p.tokens * (p.inv_freq ? kD / 2 : 1); at += blockDim.x) {
+        const int j = p.inv_freq ? at / (kD / 2) : at, pair = p.inv_freq ? at % (kD / 2) : 0;
+        const uint32_t tk = first + j;
+        const int tb = (int)(tk / (uint32_t)p.T), tt = (int)(tk - (uint32_t)tb * p.T);
+        if (tk >= all || (p.n_new && tt >= p.n_new[tb])) continue;
+        const int pos = p.start_pos[tb] + tt;
+        const int32_t* own = AT ? p.positions + tb * p.ps_b + tt : nullptr;
+        if (pair == 0) {
+          const int page = pos >> p.page_shift;
+          page_s[j] = p.block_table ? (int64_t)p.block_table[(int64_t)tb * p.bt_stride + page] : page;
+          slot_s[j] = pos & p.page_mask;
+          if (AT && p.token_positions && pos < p.tp_rows) p.token_positions[tb * p.tp_sb + pos] = own[0];
+        }
+        if (!p.inv_freq) continue;
+        float sn, cs;
+        if constexpr (AT) {
+          const int axis = p.pair_axis ? min(max(p.pair_axis[pair], 0), p.axes - 1) : 0;
+          constexpr double kTurns = 0.1591549430918953357689;          // 1 / (2 pi)
+          const double turns = (double)own[axis * p.ps_axis] * (double)p.inv_freq[pair] * kTurns;
+          sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+          cos_s[j][pair] = cs * p.rope_scale;
+          sin_s[j][pair] = sn * p.rope_scale;
+        } else {
+          sincosf((float)pos * p.inv_freq[pair], &sn, &cs);
+          cos_s[j][pair] = from_f<BF16>(cs * p.rope_scale);
+          sin_s[j][pair] = from_f<BF16>(sn * p.rope_scale);
+        }
+      }
+      __syncthreads();
+    }
+    const int64_t phys = active ? page_s[i] : 0, slot = active ? slot_s[i] : 0;
+    const int64_t place = b * p.c_sb + phys * p.c_sp + slot * p.c_st + head * p.c_sh;
+    const int64_t params = b * p.pa_sb + phys * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const bool turn = p.inv_freq && (!kv || r == 0);
+      const __half* gain = !kv ? p.q_gain : r == 0 ? p.k_gain : nullptr;
+      H2* lo = reinterpret_cast<H2*>(&row[r][0]);
+      H2* hi = reinterpret_cast<H2*>(&row[r][1]);
+      uint64_t x[8];                                                    // the row in fp32: pairs 0-3 from lo, 4-7 from hi
+      float ends[4];                                                    // the ends of its groups over the lane
+      auto widen = [&] {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
+          x[e] = pack2(a.x, a.y);
+          x[4 + e] = pack2(d2.x, d2.y);
+        }
+      };
+      const bool plain = AT && STORE != kInt4 && kv && r == 1;            // a V row that is stored as it is
+      float inv_rms = 1.f;
+      if (AT && !plain) widen();
+      if (r == 0 ? p.q_gain || p.k_gain : p.q_gain != nullptr) {         // (uniform: the warp's rows are of either kind)
+        uint64_t sq = 0;
+        if constexpr (!AT) widen();
+        if (!plain) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sq = fma2(x[e], x[e], sq);
+        }
+        float ss = unpack2(sq).x + unpack2(sq).y;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+        inv_rms = rsqrtf(ss / kD + p.eps);
+      }
+      if constexpr (AT) {
+        if (!plain) {
+          if (gain) {
+            const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
+            const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
+            const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
+            const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
+            const uint64_t rms2 = pack2(inv_rms, inv_rms);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 a = to_f2(g_lo[e]), d2 = to_f2(g_hi[e]);
+              x[e] = mul2(x[e], mul2(pack2(a.x, a.y), rms2));
+              x[4 + e] = mul2(x[4 + e], mul2(pack2(d2.x, d2.y), rms2));
+            }
+          }
+          if (turn) {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(&cos_s[i][c * 8 + 2 * e]);
+              const ulonglong2 sn = *reinterpret_cast<const ulonglong2*>(&sin_s[i][c * 8 + 2 * e]);
+#pragma unroll
+              for (int f = 0; f < 2; ++f) {
+                const uint64_t l = x[e + f], h2 = x[4 + e + f], cv = f ? cs.y : cs.x, sv = f ? sn.y : sn.x;
+                x[e + f] = sub2(mul2(l, cv), mul2(h2, sv));
+                x[4 + e + f] = fma2(l, sv, mul2(h2, cv));
+              }
+            }
+          }
+          if (STORE != kInt4 || !kv) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 a = unpack2(x[e]), d2 = unpack2(x[4 + e]);
+              lo[e] = from_f2<BF16>(a.x, a.y);
+              hi[e] = from_f2<BF16>(d2.x, d2.y);
+            }
+          }
+        }
+        if constexpr (STORE == kInt4) {
+          group_ends(x, ends[0], ends[1]);
+          group_ends(x + 4, ends[2], ends[3]);
+        }
+      } else {
+        if (gain) module_norm<BF16>(lo, hi, gain, inv_rms, c);
+        if (turn) module_rotate<BF16>(lo, hi, cos_s[i], sin_s[i], c);
+        widen();
+        group_ends<BF16>(row[r][0], ends[0], ends[1]);
+        group_ends<BF16>(row[r][1], ends[2], ends[3]);
+      }
+      uint32_t words[2];
+      __half scale[2], zero[2];
+      if constexpr (STORE == kInt4) {
+        words[0] = quantize_int4(x, ends[0], ends[1], scale[0], zero[0]);
+        words[1] = quantize_int4(x + 4, ends[2], ends[3], scale[1], zero[1]);
+      }
+      if (!active || (r && !two)) continue;
+      if (!kv) {
+        __half* dst = p.q_out + (((int64_t)b * p.T + t) * p.H + head + r) * kD;
+        reinterpret_cast<uint4*>(dst)[c] = row[r][0];
+        reinterpret_cast<uint4*>(dst + kD / 2)[c] = row[r][1];
+        continue;
+      }
+      __half* cache = r == 0 ? p.k_cache : p.v_cache;
+      if constexpr (STORE == kInt4) {
+        const int g = c >> 2, q = c & 3;                                 // groups g and g + 2, values 8q .. 8q+7 of either
+        uint8_t* dst = reinterpret_cast<uint8_t*>(cache) + place;
+        __half* pr = (r == 0 ? p.k_param : p.v_param) + params;
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          if (r == 0) {
+            *reinterpret_cast<uint32_t*>(dst + q * 16 + (g + 2 * f) * 4) = words[f];
+          } else {
+            *reinterpret_cast<uint16_t*>(dst + (2 * q) * 8 + (g + 2 * f) * 2) = (uint16_t)words[f];
+            *reinterpret_cast<uint16_t*>(dst + (2 * q + 1) * 8 + (g + 2 * f) * 2) = (uint16_t)(words[f] >> 16);
+          }
+          if (q == 0) { pr[g + 2 * f] = scale[f]; pr[4 + g + 2 * f] = zero[f]; }
+        }
+      } else if constexpr (STORE == kFp8) {
+        const float sc = (r == 0 ? p.k_scale : p.v_scale)[b * p.s_sb + phys * p.s_sp + head * p.s_sh];
+        uint8_t* d8 = reinterpret_cast<uint8_t*>(cache) + place;
+        reinterpret_cast<uint2*>(d8)[c] = quantize8(lo, sc);              // bytes 8c .. 8c+7
+        reinterpret_cast<uint2*>(d8 + kD / 2)[c] = quantize8(hi, sc);     // bytes 64+8c .. 64+8c+7
+      } else {
+        reinterpret_cast<uint4*>(cache + place)[c] = row[r][0];
+        reinterpret_cast<uint4*>(cache + place + kD / 2)[c] = row[r][1];
+      }
+    }
+  }
+}
+
+// Tokens of a CTA: as many as fill about 16 items, where there are CTAs enough; eight threads per item, up to 256.
+template <bool BF16, int STORE, bool AT>
+static void launch_kv_append(KvWriteParams p, int64_t tokens, cudaStream_t st) {
+  const int per = p.G + (p.H + 1) / 2;
+  p.tokens = 1;
+  while (p.tokens < kAppendTokens && p.tokens * 2 * per <= 16 && tokens >= (int64_t)p.tokens * 2 * 8 * sm_count()) p.tokens *= 2;
+  const int threads = (p.tokens * per * 8 + 31) / 32 * 32;
+  kv_append_kernel<BF16, STORE, AT><<<(unsigned)((tokens + p.tokens - 1) / p.tokens), threads < kAppendThreads ? threads : kAppendThreads,
+                                      0, st>>>(p);
+}
+template <bool BF16>
+static void launch_kv_append(const KvWriteParams& p, int store, int64_t tokens, cudaStream_t st) {
+  if (store == kInt4 && p.positions) launch_kv_append<BF16, kInt4, true>(p, tokens, st);
+  else if (store == kInt4) launch_kv_append<BF16, kInt4, false>(p, tokens, st);
+  else if (store == kFp8) launch_kv_append<BF16, kFp8, true>(p, tokens, st);
+  else launch_kv_append<BF16, kSame, true>(p, tokens, st);
 }
 
 // Rows of a 4-bit cache in 16 bits: eight lanes per row, lane c the values 8c .. 8c+7 and 64+8c .. 64+8c+7 of K and of V.
@@ -485,12 +677,17 @@ static int kv_write_call(const kb200_act_layout* q_in, void* q_out, const kb200_
   const int64_t blocks = (int64_t)batch * max_new;                   // one CTA per (sequence, new token)
   KB_REQUIRE(blocks < (1ll << 31), "kv_write: too many tokens for one launch");
   cudaStream_t st = (cudaStream_t)stream;
-  if (bf16 && int4) launch_kv_write<true, kInt4>(p, blocks, st);
-  else if (int4) launch_kv_write<false, kInt4>(p, blocks, st);
-  else if (bf16 && fp8) launch_kv_write<true, kFp8>(p, blocks, st);
-  else if (bf16) launch_kv_write<true, kSame>(p, blocks, st);
-  else if (fp8) launch_kv_write<false, kFp8>(p, blocks, st);
-  else launch_kv_write<false, kSame>(p, blocks, st);
+  if (at || int4) {
+    const int store = int4 ? kInt4 : fp8 ? kFp8 : kSame;
+    if (bf16) launch_kv_append<true>(p, store, blocks, st);
+    else launch_kv_append<false>(p, store, blocks, st);
+    KB_CHECK_LAUNCH("kv_append_kernel");
+    return 0;
+  }
+  if (bf16 && fp8) launch_kv_write<true, true>(p, blocks, st);
+  else if (bf16) launch_kv_write<true, false>(p, blocks, st);
+  else if (fp8) launch_kv_write<false, true>(p, blocks, st);
+  else launch_kv_write<false, false>(p, blocks, st);
   KB_CHECK_LAUNCH("kv_write_kernel");
   return 0;
 }
