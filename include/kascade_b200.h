@@ -134,7 +134,7 @@ typedef struct kb200_kv_layout {
    * fp16, s of groups 0..3 and z of groups 0..3, at
    *   k_param[b * param_stride_batch + page * param_stride_page + slot * param_stride_token + g * param_stride_head]
    * (strides in elements, multiples of 8, the same for v_param; lay the two rows' parameters beside each other, so that
-   * one 32-byte sector holds both).  A row is complete in itself, so rows can move between pages (kb200_evict_move).
+   * one 32-byte sector holds both).  A row is complete in itself, so rows can move between pages (kb200_evict).
    * act_dtype: KB200_FP16 or KB200_BF16, the type of q and of the output of a decode call, and of the rows that
    * kb200_kv_write takes and kb200_kv_read gives.  The reference has no quantised cache. */
   const void* k_param;
@@ -400,7 +400,7 @@ int kb200_kv_write(const kb200_act_layout* q_in, void* q_out, const kb200_act_la
                    int num_q_heads, int num_kv_heads, void* stream);
 
 /* kb200_kv_write for tokens whose rotary positions are not their places in the cache: a cache that rows have left
- * (kb200_evict_plan), images and video with positions on several axes (time, height, width).
+ * (kb200_evict), images and video with positions on several axes (time, height, width).
  * Pair i of a head (elements i and i + 64) turns by positions[pair_axis[i]] * inv_freq[i].  The angle is formed in 64 bits,
  * norm and rotation are computed in fp32 and rounded once (kb200_kv_write repeats the modules' roundings instead).
  *   positions  [axes, B, T] int32: element (axis, b, t) at axis * stride_axis + b * stride_batch + t
@@ -450,34 +450,25 @@ int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t
                           float* mass_out, int64_t mass_in_stride, int64_t mass_out_stride, int batch, int num_kv_heads,
                           int num_tiles, int n_rows, void* stream);
 
-/* What eviction ranks the rows of a cache by, for kb200_topk_select with k_max = budget:
- *   keys[b, j] = +inf for protected rows, else mass[b, j] (a NaN counts as 0)        for j < seq_lens[b]
- * Protected are the rows whose token position is below `sinks` or within the last `recent` of the sequence's positions.
- *   token_positions  [B, rows] int32 (pos_stride apart), or NULL: the row's number (a cache that no row has left yet) */
-int kb200_evict_keys(const float* mass, int64_t mass_stride, const int32_t* seq_lens, const int32_t* token_positions,
-                     int64_t pos_stride, int sinks, int recent, float* keys, int64_t key_stride, int batch, int n_rows,
-                     void* stream);
-
-/* Turns the kept rows of every sequence (kb200_topk_select's output over the keys: ascending, keep_count[b] of them) into the
- * moves that bring them together in rows 0 .. keep_count[b] - 1.  Kept rows below keep_count[b] stay where they are; those behind
- * fill the rows that were let go, the lowest into the lowest.  That is the smallest number of moves, and no row is both
- * source and target, so the moves have no order.  (The order of rows in a cache has no meaning to attention: positions
- * are in the keys' rotation.)
- *   moves      [B, move_stride] pairs (source row, target row) int32, move_stride >= budget (in pairs); move_count [B]
- *   new_lens   [B] receives keep_count
+/* Shortens every sequence of a cache to at most `budget` rows, in all layers alike: those with the largest mass[b, j] stay
+ * (j < seq_lens[b]; a NaN counts as 0; ties go to the lowest row), and in any case the rows whose token position is below
+ * `sinks` or within the last `recent` of the sequence's positions.  Kept rows below the new length stay where they are, those
+ * behind it fill the rows that were let go, the lowest into the lowest: the smallest number of moves, and no row is both source
+ * and target.  (The order of rows in a cache has no meaning to attention: positions are in the keys' rotation.)
+ *   layers     host array of n_layers layouts, fp16 / bf16 or INT4, of one type, block table and set of strides (an FP8 cache has
+ *              one scale per page, so its rows cannot leave their page: refused); changed in place.  The pages below the new
+ *              length must belong to one sequence alone
+ *   mass       [B, n_rows] fp32, rows mass_stride apart
+ *   token_positions  [B, n_rows] int32 (pos_stride apart), or NULL: the row's number (a cache that no row has left yet)
+ *   new_lens   [B] receives min(seq_lens[b], budget)
  *   mass_out / pos_out  [B, n_rows] (out_stride apart): the rows' weight and token position after the moves, 0 and -1 behind
- *              new_lens[b]; neither may be its input.  pos_out may be NULL; pos_in may be NULL (the row's number) */
-int kb200_evict_plan(const int32_t* keep, int64_t keep_stride, const int32_t* keep_count, const float* mass_in,
-                     int64_t mass_stride, const int32_t* pos_in, int64_t pos_stride, int32_t* moves, int64_t move_stride,
-                     int32_t* move_count, int32_t* new_lens, float* mass_out, int32_t* pos_out,
-                     int64_t out_stride, int batch, int n_rows, void* stream);
-
-/* Moves rows inside the caches of several layers.  All layers share the block table; fp16 / bf16 or INT4 caches (an FP8
- * cache has one scale per page, so its rows cannot leave their page: refused), one type and one set of strides per call.
- *   layers     host array of n_layers layouts
- *   max_moves  the most moves of a sequence (the grid's size) */
-int kb200_evict_move(const kb200_kv_layout* layers, int n_layers, const int32_t* moves, int64_t move_stride,
-                     const int32_t* move_count, int max_moves, int batch, int num_kv_heads, void* stream);
+ *              new_lens[b]; neither may be its input
+ *   workspace  16-byte aligned, kb200_evict_workspace_bytes bytes; two calls at once need two */
+size_t kb200_evict_workspace_bytes(int batch, int n_rows, int budget);
+int kb200_evict(const kb200_kv_layout* layers, int n_layers, const int32_t* seq_lens, const float* mass, int64_t mass_stride,
+                const int32_t* token_positions, int64_t pos_stride, int budget, int recent, int sinks, int32_t* new_lens,
+                float* mass_out, int32_t* pos_out, int64_t out_stride, void* workspace, size_t workspace_bytes, int batch,
+                int num_kv_heads, int n_rows, void* stream);
 
 /* ---- diagnostics ----------------------------------------------------------------------------- */
 

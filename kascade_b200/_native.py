@@ -30,8 +30,8 @@ EXPORTS = [
     "kb200_decode_sparse_paged_noalloc", "kb200_prefill_dense_fanout", "kb200_prefill_sparse_fanout",
     "kb200_kv_write", "kb200_prefill_dense_ragged", "kb200_prefill_pool_scores_ragged", "kb200_prefill_sparse_ragged",
     "kb200_prefill_budgets_ragged", "kb200_zero_padding", "kb200_peer_push", "kb200_stream_wait_events", "kb200_selftest_wait_timeout", "kb200_tensor_map_encodes", "kb200_decode_noalloc_splits",
-    "kb200_kv_write_at", "kb200_kv_read", "kb200_mass_add", "kb200_mass_add_prompt", "kb200_evict_keys", "kb200_evict_plan",
-    "kb200_evict_move",
+    "kb200_kv_write_at", "kb200_kv_read", "kb200_mass_add", "kb200_mass_add_prompt", "kb200_evict",
+    "kb200_evict_workspace_bytes",
 ]
 
 
@@ -165,9 +165,10 @@ def load() -> C.CDLL:
         lib.kb200_kv_read.argtypes = [C.POINTER(KvLayout), vp, vp, vp, i32, i32, i32, vp]
         lib.kb200_mass_add.argtypes = [vp, i64, vp, vp, vp, i64, i32, i32, i32, vp]
         lib.kb200_mass_add_prompt.argtypes = [vp, i64, vp, vp, vp, i64, i64, i32, i32, i32, i32, vp]
-        lib.kb200_evict_keys.argtypes = [vp, i64, vp, vp, i64, i32, i32, vp, i64, i32, i32, vp]
-        lib.kb200_evict_plan.argtypes = [vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i32, i32, vp]
-        lib.kb200_evict_move.argtypes = [C.POINTER(KvLayout), i32, vp, i64, vp, i32, i32, i32, vp]
+        lib.kb200_evict_workspace_bytes.restype = C.c_size_t
+        lib.kb200_evict_workspace_bytes.argtypes = [i32, i32, i32]
+        lib.kb200_evict.argtypes = [C.POINTER(KvLayout), i32, vp, vp, i64, vp, i64, i32, i32, i32, vp, vp, vp, i64, vp, C.c_size_t,
+                                    i32, i32, i32, vp]
         lib.kb200_selftest_umma.argtypes = [vp, vp, vp, vp, vp]
         lib.kb200_peer_push.argtypes = [C.POINTER(PushPlan), vp, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, vp, vp]
         lib.kb200_stream_wait_events.argtypes = [vp, C.POINTER(C.c_void_p), i32]
@@ -256,8 +257,9 @@ def _want(t: torch.Tensor, dtype, name: str):
 
 
 def _same_device(first: torch.Tensor, **others: Optional[torch.Tensor]):
+    where = first.get_device()
     for name, t in others.items():
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != where:
             raise KascadeNativeError(f"{name} is on {t.device}, expected {first.device}")
 
 
@@ -339,12 +341,25 @@ def is_int4(cache: torch.Tensor) -> bool:
 
 
 def _int4_params(k, v, k_param, v_param):
-    """The checks of an INT4 cache: codes [..., 64] uint8 and parameters [..., 8] fp16 of the same leading shape."""
-    if not k.is_cuda:
+    """The checks of an INT4 cache: codes [..., 64] uint8 and parameters [..., 8] fp16 of the same leading shape.  Returns the
+    strides of the codes and of the parameters."""
+    where, st = k.get_device(), k.stride()
+    if where >= 0 and len(st) == 4 and st[3] == 1 and k_param is not None:
+        ps, shape = k_param.stride(), k.shape
+        if ps[-1] == 1 and k_param.dtype is torch.float16 and k_param.get_device() == where \
+                and k_param.shape == (*shape[:3], 8):
+            if v is None:
+                return st, ps
+            if v_param is not None and v.shape == shape and v.stride() == st and v.dtype == k.dtype and v.get_device() == where \
+                    and v_param.dtype is torch.float16 and v_param.shape == k_param.shape and v_param.stride() == ps \
+                    and v_param.get_device() == where:
+                return st, ps
+    # something is wrong: say what
+    if where < 0:
         raise KascadeNativeError(f"k_cache: expected a CUDA uint8 tensor, got one on {k.device}")
-    if k.dim() != 4 or k.stride(3) != 1:
+    if len(st) != 4 or st[3] != 1:
         raise KascadeNativeError("an INT4 cache holds rows of 64 contiguous bytes: [num_pages, page_size, G, 64]")
-    if v is not None and (v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype):
+    if v is not None and (v.shape != k.shape or v.stride() != st or v.dtype != k.dtype):
         raise KascadeNativeError("k_cache and v_cache must have the same type, shape and strides")
     if k_param is None or (v is not None and v_param is None):
         raise KascadeNativeError("an INT4 cache needs k_scale (and v_scale): eight fp16 per row, four scales and four zeros")
@@ -355,9 +370,8 @@ def _int4_params(k, v, k_param, v_param):
         if par.shape != k.shape[:3] + (8,) or par.stride(3) != 1:
             raise KascadeNativeError(f"{name} of an INT4 cache: expected {tuple(k.shape[:3]) + (8,)}, the last dimension "
                                      f"contiguous, got {tuple(par.shape)}")
-    if v is not None and v_param.stride() != k_param.stride():
-        raise KascadeNativeError("k_scale and v_scale must have the same shape and strides")
     _same_device(k, v_cache=v, k_scale=k_param, v_scale=v_param)
+    raise KascadeNativeError("k_scale and v_scale must have the same shape and strides")
 
 
 def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], block_table: torch.Tensor,
@@ -368,17 +382,17 @@ def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], bloc
     [num_pages, page_size, G, 64]) with k_scale / v_scale [num_pages, page_size, G, 8] fp16 and `act_dtype`, the type of the
     queries, outputs and new rows."""
     if is_int4(k_cache):
-        _int4_params(k_cache, v_cache, k_scale, v_scale)
+        st, ps = _int4_params(k_cache, v_cache, k_scale, v_scale)
         if act_dtype not in DTYPES:
             raise KascadeNativeError(f"act_dtype of an INT4 cache: expected fp16 or bf16, got {act_dtype}")
-        _want(block_table, torch.int32, "block_table")
-        _same_device(k_cache, block_table=block_table)
-        if block_table.dim() != 2 or block_table.stride(1) != 1:
+        ts = block_table.stride()
+        if block_table.dtype is not torch.int32 or block_table.get_device() != k_cache.get_device() or len(ts) != 2 or ts[1] != 1:
+            _want(block_table, torch.int32, "block_table")
+            _same_device(k_cache, block_table=block_table)
             raise KascadeNativeError("block_table: expected [B, max_pages], the last dimension contiguous")
-        st, ps = k_cache.stride(), k_scale.stride()
-        return _holding(KvLayout(k_cache.data_ptr(), _ptr(v_cache), 0, st[0], st[1], st[2], block_table.data_ptr(),
-                                 block_table.stride(0), k_cache.shape[1], INT4, 0, 0, 0, 0, 0, k_scale.data_ptr(),
-                                 _ptr(v_scale) if v_cache is not None else 0, 0, ps[0], ps[1], ps[2], DTYPES[act_dtype]),
+        return _holding(KvLayout(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2],
+                                 block_table.data_ptr(), ts[0], k_cache.shape[1], INT4, 0, 0, 0, 0, 0, k_scale.data_ptr(),
+                                 0 if v_cache is None else v_scale.data_ptr(), 0, ps[0], ps[1], ps[2], DTYPES[act_dtype]),
                         k_cache, v_cache, block_table, k_scale, v_scale)
     if k_cache.dtype in FP8_TORCH:
         assert k_cache.is_cuda and k_cache.dim() == 4 and k_cache.stride(3) == 1
@@ -409,10 +423,9 @@ def kv_layout_contiguous(k: torch.Tensor, v: Optional[torch.Tensor], page_size: 
     """HF cache view [B, G, L, D] (any batch / head / token strides, D contiguous).  An FP8 cache comes with
     k_scale / v_scale [B, G, ceil(L / page_size)] fp32, an INT4 cache [B, G, L, 64] with [B, G, L, 8] fp16."""
     if is_int4(k):
-        _int4_params(k, v, k_scale, v_scale)
+        st, ps = _int4_params(k, v, k_scale, v_scale)
         if act_dtype not in DTYPES:
             raise KascadeNativeError(f"act_dtype of an INT4 cache: expected fp16 or bf16, got {act_dtype}")
-        st, ps = k.stride(), k_scale.stride()
         return _holding(KvLayout(k.data_ptr(), _ptr(v), st[0], st[2] * page_size, st[2], st[1], 0, 0, page_size, INT4, 0, 0, 0, 0,
                                  0, k_scale.data_ptr(), _ptr(v_scale) if v is not None else 0, ps[0], ps[2] * page_size, ps[2],
                                  ps[1], DTYPES[act_dtype]), k, v, k_scale, v_scale)
@@ -669,20 +682,23 @@ def kv_write(q_in, q_out, k_new, v_new, start_pos, n_new, kv: KvLayout, q_gain=N
         _want(inv_freq, torch.float32, "inv_freq")
         assert inv_freq.is_contiguous() and inv_freq.numel() == HEAD_DIM // 2
     if positions is not None:
-        _want(positions, torch.int32, "positions")
-        _want_opt(pair_axis, torch.int32, "pair_axis")
-        _want_opt(token_positions, torch.int32, "token_positions")
-        _same_device(k_new, positions=positions, pair_axis=pair_axis, token_positions=token_positions)
-        if positions.dim() != 3 or positions.shape[1:] != (B, T) or (T > 1 and positions.stride(2) != 1) or not positions.shape[0]:
+        where, ps = k_new.get_device(), positions.stride()
+        if positions.dtype is not torch.int32 or positions.get_device() != where or len(ps) != 3 or positions.shape[1:] != (B, T) \
+                or (T > 1 and ps[2] != 1) or not positions.shape[0]:
+            _want(positions, torch.int32, "positions")
+            _same_device(k_new, positions=positions)
             raise KascadeNativeError(f"positions: expected [axes, {B}, {T}], the last dimension contiguous, got "
                                      f"{tuple(positions.shape)}")
-        if pair_axis is not None and (pair_axis.shape != (HEAD_DIM // 2,) or not pair_axis.is_contiguous()):
-            raise KascadeNativeError(f"pair_axis: expected [{HEAD_DIM // 2}] contiguous, got {tuple(pair_axis.shape)}")
-        if token_positions is not None and (token_positions.dim() != 2 or token_positions.shape[0] != B
-                                            or token_positions.stride(1) != 1):
-            raise KascadeNativeError(f"token_positions: expected [{B}, rows], the last dimension contiguous, got "
-                                     f"{tuple(token_positions.shape)}")
-        at = Positions(positions.data_ptr(), positions.stride(0), positions.stride(1), _ptr(pair_axis), positions.shape[0],
+        if pair_axis is not None and (pair_axis.dtype is not torch.int32 or pair_axis.shape != (HEAD_DIM // 2,)
+                                      or not pair_axis.is_contiguous() or pair_axis.get_device() != where):
+            raise KascadeNativeError(f"pair_axis: expected [{HEAD_DIM // 2}] int32 contiguous on {k_new.device}, got "
+                                     f"{tuple(pair_axis.shape)} {pair_axis.dtype} on {pair_axis.device}")
+        if token_positions is not None and (token_positions.dtype is not torch.int32 or token_positions.dim() != 2
+                                            or token_positions.shape[0] != B or token_positions.stride(1) != 1
+                                            or token_positions.get_device() != where):
+            raise KascadeNativeError(f"token_positions: expected [{B}, rows] int32 on {k_new.device}, the last dimension "
+                                     f"contiguous, got {tuple(token_positions.shape)} {token_positions.dtype} on {token_positions.device}")
+        at = Positions(positions.data_ptr(), ps[0], ps[1], _ptr(pair_axis), positions.shape[0],
                        _ptr(token_positions), 0 if token_positions is None else token_positions.stride(0),
                        0 if token_positions is None else token_positions.shape[1])
         _check(lib.kb200_kv_write_at(C.byref(ql), _ptr(q_out), C.byref(kl), C.byref(vl), _ptr(start_pos), _ptr(n_new),
@@ -700,17 +716,16 @@ def kv_write(q_in, q_out, k_new, v_new, start_pos, n_new, kv: KvLayout, q_gain=N
 def kv_read(kv: KvLayout, seq_lens, k_out, v_out):
     """Rows 0 .. seq_lens[b] - 1 of an INT4 cache into k_out / v_out [B, max_len, G, D] (contiguous, of the layout's act_dtype);
     rows behind a sequence are written as zeros."""
-    lib = init(k_out.get_device())
-    B, T, G, _ = k_out.shape
+    where = k_out.get_device()
+    lib = init(where)
+    B, T, G, D = k_out.shape
     if kv.dtype != INT4:
         raise KascadeNativeError("kv_read: the cache is not INT4: its rows need no conversion")
-    _want(seq_lens, torch.int32, "seq_lens")
-    if _half_code(k_out, "k_out") != kv.act_dtype or v_out.dtype != k_out.dtype or v_out.shape != k_out.shape:
+    if _half_code(k_out, "k_out") != kv.act_dtype or v_out.dtype is not k_out.dtype or v_out.shape != k_out.shape:
         raise KascadeNativeError("kv_read: k_out and v_out must have one shape and the layout's act_dtype")
-    if not (k_out.is_contiguous() and v_out.is_contiguous() and seq_lens.is_contiguous()) or seq_lens.shape != (B,) \
-            or k_out.shape[3] != HEAD_DIM:
-        raise KascadeNativeError(f"kv_read: expected contiguous k_out / v_out [B, T, G, {HEAD_DIM}] and seq_lens [B]")
-    _same_device(k_out, v_out=v_out, seq_lens=seq_lens)
+    if not (k_out.is_contiguous() and v_out.is_contiguous() and seq_lens.is_contiguous()) or seq_lens.shape != (B,) or D != HEAD_DIM \
+            or seq_lens.dtype is not torch.int32 or seq_lens.get_device() != where or v_out.get_device() != where:
+        raise KascadeNativeError(f"kv_read: expected contiguous k_out / v_out [B, T, G, {HEAD_DIM}] and seq_lens [B] int32 on one device")
     _check(lib.kb200_kv_read(C.byref(kv), _ptr(seq_lens), _ptr(k_out), _ptr(v_out), B, T, G, _stream()), "kb200_kv_read")
     _launched(1 if k_out.numel() else 0)
 
@@ -764,70 +779,41 @@ def mass_add_prompt(pooled, mass, out, seq_len=None):
 
 
 @_on_device_of(0)
-def evict_keys(mass, seq_lens, token_positions, sinks: int, recent: int, keys):
-    """keys [B, key_stride >= rows] fp32: what the rows of a cache are ranked by, see kb200_evict_keys."""
+def evict(mass, layers, seq_lens, budget: int, recent: int, sinks: int, token_positions, num_kv_heads: int):
+    """Shortens the caches of `layers` (KvLayouts that share a block table, a type and strides) in place, see kb200_evict.  Returns
+    the new lengths [B], and the rows' weight and token position [B, rows] after the moves."""
     lib = init(mass.get_device())
+    if mass.dim() != 2:
+        raise KascadeNativeError(f"mass: expected [B, rows], got {tuple(mass.shape)}")
     B, rows = mass.shape
     _want_rows(mass, torch.float32, B, "mass")
-    _want(keys, torch.float32, "keys")
     _want(seq_lens, torch.int32, "seq_lens")
     if token_positions is not None:
         _want_rows(token_positions, torch.int32, B, "token_positions")
         if token_positions.shape[1] != rows:
             raise KascadeNativeError(f"token_positions: expected {(B, rows)}, got {tuple(token_positions.shape)}")
-    if seq_lens.shape != (B,) or not seq_lens.is_contiguous() or not keys.is_contiguous() or keys.shape[0] != B:
-        raise KascadeNativeError("evict_keys: seq_lens [B] and keys [B, key_stride] must be contiguous")
-    _same_device(mass, seq_lens=seq_lens, token_positions=token_positions, keys=keys)
-    _check(lib.kb200_evict_keys(_ptr(mass), mass.stride(0), _ptr(seq_lens), _ptr(token_positions),
-                                0 if token_positions is None else token_positions.stride(0), int(sinks), int(recent), _ptr(keys),
-                                keys.shape[1], B, rows, _stream()), "kb200_evict_keys")
-    _launched(1 if B and rows else 0)
-
-
-@_on_device_of(0)
-def evict_plan(keep, keep_count, mass, token_positions, moves, move_count, new_lens, mass_out, pos_out):
-    """keep [B, budget] int32 ascending and keep_count [B]: the rows that stay; moves [B, budget, 2], move_count, new_lens [B] int32
-    and the rows' weight and token position after the moves, see kb200_evict_plan."""
-    lib = init(keep.get_device())
-    B, rows = mass.shape
-    for name, t in (("keep", keep), ("keep_count", keep_count), ("moves", moves), ("move_count", move_count), ("new_lens", new_lens)):
-        _want(t, torch.int32, name)
-        if not t.is_contiguous() or t.shape[0] != B:
-            raise KascadeNativeError(f"evict_plan: {name} must be contiguous, with a row for each of {B} sequences")
-    _want_rows(mass, torch.float32, B, "mass")
-    _want(mass_out, torch.float32, "mass_out")
-    _want(pos_out, torch.int32, "pos_out")
-    if token_positions is not None:
-        _want_rows(token_positions, torch.int32, B, "token_positions")
-    if moves.shape != keep.shape + (2,) or mass_out.shape != mass.shape or pos_out.shape != mass.shape \
-            or not mass_out.is_contiguous() or not pos_out.is_contiguous() \
-            or (token_positions is not None and token_positions.shape != mass.shape):
-        raise KascadeNativeError("evict_plan: moves must be [B, budget, 2], the weights and positions [B, rows]")
-    _same_device(keep, keep_count=keep_count, mass=mass, token_positions=token_positions, moves=moves, move_count=move_count,
-                 new_lens=new_lens, mass_out=mass_out, pos_out=pos_out)
-    _check(lib.kb200_evict_plan(_ptr(keep), keep.shape[1], _ptr(keep_count), _ptr(mass), mass.stride(0), _ptr(token_positions),
-                                0 if token_positions is None else token_positions.stride(0), _ptr(moves), keep.shape[1],
-                                _ptr(move_count), _ptr(new_lens), _ptr(mass_out), _ptr(pos_out), rows, B, rows, _stream()),
-           "kb200_evict_plan")
-    _launched(1 if B and rows else 0)
-
-
-@_on_device_of(1)
-def evict_move(layers, moves, move_count, max_moves: int, num_kv_heads: int):
-    """Moves rows inside the caches of several layers (KvLayouts that share a block table, a type and strides)."""
-    lib = init(moves.get_device())
-    _want(moves, torch.int32, "moves")
-    _want(move_count, torch.int32, "move_count")
-    B, budget = moves.shape[:2]
-    if not moves.is_contiguous() or moves.shape[2:] != (2,) or move_count.shape != (B,) or not move_count.is_contiguous():
-        raise KascadeNativeError("evict_move: expected contiguous moves [B, budget, 2] and move_count [B]")
-    _same_device(moves, move_count=move_count)
+    if seq_lens.shape != (B,) or not seq_lens.is_contiguous():
+        raise KascadeNativeError("evict: seq_lens [B] must be contiguous")
+    _same_device(mass, seq_lens=seq_lens, token_positions=token_positions)
+    where = mass.get_device()
     for layer in layers:
-        _same_device(moves, **{f"cache {i}": t for i, t in enumerate(layer._keep)})
+        for t in layer._keep:
+            if t.get_device() != where:
+                raise KascadeNativeError(f"a cache is on {t.device}, expected {mass.device}")
+    dev = mass.device
+    lens = torch.empty(B, dtype=torch.int32, device=dev)
+    mass_out = torch.empty(B, rows, dtype=torch.float32, device=dev)
+    pos_out = torch.empty(B, rows, dtype=torch.int32, device=dev)
+    size = lib.kb200_evict_workspace_bytes(B, rows, budget)
+    workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
     array = (KvLayout * len(layers))(*layers)
-    _check(lib.kb200_evict_move(array, len(layers), _ptr(moves), budget, _ptr(move_count), max_moves, B, num_kv_heads, _stream()),
-           "kb200_evict_move")
-    _launched(-(-len(layers) // 32) if B and max_moves else 0)
+    _check(lib.kb200_evict(array, len(layers), seq_lens.data_ptr(), mass.data_ptr(), mass.stride(0), _ptr(token_positions),
+                           0 if token_positions is None else token_positions.stride(0), budget, recent, sinks, lens.data_ptr(),
+                           mass_out.data_ptr(), pos_out.data_ptr(), rows, workspace.data_ptr(), size, B, num_kv_heads, rows,
+                           _stream()), "kb200_evict")
+    if B and rows:
+        _launched(3 + (-(-len(layers) // 32) if rows > budget else 0))
+    return lens, mass_out, pos_out
 
 
 @_on_device_of(0)

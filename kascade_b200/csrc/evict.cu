@@ -103,59 +103,95 @@ static int mass_ctas(int64_t clusters) {
 }
 
 // ---- what stays ------------------------------------------------------------------------------------------------------
-// One CTA per sequence: the newest position, then the keys.
-__global__ void __launch_bounds__(1024) evict_keys_kernel(const float* mass, int64_t mass_stride, const int32_t* seq_lens,
-                                                          const int32_t* positions, int64_t pos_stride, int sinks, int recent,
-                                                          float* keys, int64_t key_stride, int n_rows) {
+// What the rows of a sequence are ranked by: +inf for protected ones, else their weight (a NaN counts as 0).  A cluster of CTAs
+// takes a sequence: the newest position first, over all of it, then the keys of its piece.
+constexpr int kKeyThreads = 1024;
+struct EvictKeysParams {
+  const float* mass; int64_t mass_stride;
+  const int32_t* seq_lens;
+  const int32_t* positions; int64_t pos_stride;
+  float* keys; int64_t key_stride;
+  int sinks, recent, n_rows;
+};
+__global__ void __launch_bounds__(kKeyThreads) evict_keys_kernel(const EvictKeysParams p) {
+  namespace cg = cooperative_groups;
   pdl_begin();
-  __shared__ int newest_of[32];
-  const int b = blockIdx.x, n = min(seq_lens[b], n_rows), tid = threadIdx.x;
-  int newest = -1;
+  __shared__ int newest_of[32], newest_s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x;
+  const int b = blockIdx.x / ctas, n = min(p.seq_lens[b], p.n_rows);
+  const float* mass = p.mass + b * p.mass_stride;
+  const int32_t* positions = p.positions ? p.positions + b * p.pos_stride : nullptr;
+  int newest = n - 1;
   if (positions) {
-    for (int j = tid; j < n; j += 1024) newest = max(newest, positions[b * pos_stride + j]);
+    newest = -1;
+    for (int j = rank * kKeyThreads + tid; j < n; j += ctas * kKeyThreads) newest = max(newest, positions[j]);
     newest = __reduce_max_sync(0xFFFFFFFFu, newest);
     if ((tid & 31) == 0) newest_of[tid >> 5] = newest;
     __syncthreads();
     newest = __reduce_max_sync(0xFFFFFFFFu, newest_of[tid & 31]);
-  } else {
-    newest = n - 1;
+    if (tid == 0) newest_s = newest;
+    cluster.sync();
+    for (int r = 0; r < ctas; ++r) newest = max(newest, *cluster.map_shared_rank(&newest_s, r));
   }
-  for (int j = tid; j < n; j += 1024) {
-    const int pos = positions ? positions[b * pos_stride + j] : j;
-    const float m = mass[b * mass_stride + j];
-    keys[b * key_stride + j] = pos < sinks || (int64_t)pos > (int64_t)newest - recent ? INFINITY : m == m ? m : 0.f;
+  for (int j = rank * kKeyThreads + tid; j < n; j += ctas * kKeyThreads) {
+    const int pos = positions ? positions[j] : j;
+    const float m = mass[j];
+    p.keys[b * p.key_stride + j] = pos < p.sinks || (int64_t)pos > (int64_t)newest - p.recent ? INFINITY : m == m ? m : 0.f;
   }
+  if (positions) cluster.sync();                                  // the other CTAs have read this one's newest position
 }
 
 struct EvictPlanParams {
   const int32_t* keep; int64_t keep_stride; const int32_t* keep_count;
   const float* mass_in; int64_t mass_stride;
   const int32_t* pos_in; int64_t pos_stride;
-  int2* moves; int64_t move_stride; int32_t* move_count; int32_t* new_lens;
+  int2* moves; int32_t* move_count; int32_t* new_lens;
   float* mass_out; int32_t* pos_out; int64_t out_stride;
   int n_rows;
 };
 
-// the first place of the ascending list a[0..n) whose value is not below x
-__device__ __forceinline__ int lower_bound(const int32_t* a, int n, int x) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (a[mid] < x) lo = mid + 1;
-    else hi = mid;
+// The first place of the ascending list a[0..n) whose value is not below x, by one warp: 32 probes at a time, four rounds for
+// a million entries instead of twenty loads one after the other.
+__device__ __forceinline__ int warp_lower_bound(const int32_t* a, int n, int x) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, len = n;                                            // the answer lies in [lo, lo + len]
+  while (len > 0) {
+    const int step = (len + 31) / 32, at = lo + lane * step;       // the last probe is the last of its piece, or beyond
+    const int last = min(at + step, lo + len) - 1;
+    const unsigned below = __ballot_sync(0xFFFFFFFFu, at < lo + len && a[max(last, 0)] < x);
+    const int whole = __popc(below);                               // pieces that lie below x as a whole: a prefix
+    const int end = lo + len;
+    lo = min(lo + whole * step, end);
+    len = min(step, end - lo);
+    if (step == 1) len = 0;
   }
   return lo;
 }
 
-// A thread per row i.  With the kept rows ascending, r = rank of i among them says whether i is kept (keep[r] == i); if it is
-// not, i - r rows below it are let go too, so it takes the (i - r)-th of the kept rows that lie behind the new length.
+// A CTA takes 256 rows.  The rank of a row among the kept ones comes from a bitmap of the kept rows among the 256 and the rank of
+// the first.  A row below the new length that is let go has i - rank others let go before it, and takes the (i - rank)-th of
+// the kept rows behind the new length.
 __global__ void __launch_bounds__(256) evict_plan_kernel(const EvictPlanParams p) {
   pdl_begin();
-  const int b = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.n_rows) return;
+  __shared__ uint32_t kept[8];
+  __shared__ int stay_s, rank_s;
+  const int b = blockIdx.y, i0 = blockIdx.x * 256, tid = threadIdx.x, i = i0 + tid, warp = tid >> 5;
   const int left = p.keep_count[b];
   const int32_t* keep = p.keep + b * p.keep_stride;
-  const int stay = lower_bound(keep, left, left);                  // kept rows below the new length
+  if (tid < 8) kept[tid] = 0u;
+  if (warp < 2) {
+    const int at = warp_lower_bound(keep, left, warp == 0 ? left : i0);
+    if ((tid & 31) == 0) (warp == 0 ? stay_s : rank_s) = at;
+  }
+  __syncthreads();
+  const int stay = stay_s, rank = rank_s;                          // kept rows below the new length; kept rows below i0
+  if (rank + tid < left) {
+    const int row = keep[rank + tid] - i0;
+    if (row < 256) atomicOr(&kept[row >> 5], 1u << (row & 31));
+  }
+  __syncthreads();
+  if (i >= p.n_rows) return;
   if (i == 0) {
     p.new_lens[b] = left;
     p.move_count[b] = left - stay;
@@ -163,17 +199,18 @@ __global__ void __launch_bounds__(256) evict_plan_kernel(const EvictPlanParams p
   float mass = 0.f;
   int pos = -1;
   if (i < left) {
-    const int r = lower_bound(keep, stay, i);
     int from = i;
-    if (r >= stay || keep[r] != i) {
+    if (!((kept[warp] >> (tid & 31)) & 1u)) {
+      int r = rank + __popc(kept[warp] & ((1u << (tid & 31)) - 1u));
+      for (int w = 0; w < warp; ++w) r += __popc(kept[w]);
       from = keep[stay + i - r];
-      p.moves[b * p.move_stride + i - r] = make_int2(from, i);
+      p.moves[b * p.keep_stride + i - r] = make_int2(from, i);
     }
     mass = p.mass_in[b * p.mass_stride + from];
     pos = p.pos_in ? p.pos_in[b * p.pos_stride + from] : from;
   }
   p.mass_out[b * p.out_stride + i] = mass;
-  if (p.pos_out) p.pos_out[b * p.out_stride + i] = pos;
+  p.pos_out[b * p.out_stride + i] = pos;
 }
 
 // ---- the moves -------------------------------------------------------------------------------------------------------
@@ -252,69 +289,50 @@ extern "C" int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, co
   return 0;
 }
 
-extern "C" int kb200_evict_keys(const float* mass, int64_t mass_stride, const int32_t* seq_lens,
-                                const int32_t* token_positions, int64_t pos_stride, int sinks, int recent, float* keys,
-                                int64_t key_stride, int batch, int n_rows, void* stream) {
-  using namespace kb200;
-  KB_ENTRY(mass, "evict_keys: mass");
-  KB_REQUIRE(mass && seq_lens && keys, "evict_keys: null pointer");
-  KB_REQUIRE(batch >= 0 && n_rows >= 0 && sinks >= 0 && recent >= 0, "evict_keys: negative size");
-  KB_REQUIRE(key_stride >= n_rows, "evict_keys: keys hold %lld rows, %d are needed", (long long)key_stride, n_rows);
-  if (batch == 0 || n_rows == 0) return 0;
-  KB_LAUNCH("evict_keys_kernel", launch_pdl(evict_keys_kernel, dim3(batch), 1024, 0, (cudaStream_t)stream, 1, mass, mass_stride,
-                                            seq_lens, token_positions, pos_stride, sinks, recent, keys, key_stride, n_rows));
-  return 0;
-}
+namespace kb200 {
+// the pieces of the workspace, in 4-byte words: keys [B, keys_row], kept rows [B, budget] and their count [B], moves [B, budget] pairs
+// and their count [B]
+struct EvictWorkspace {
+  int64_t keys_row, keep, keep_count, moves, move_count, words;
+  EvictWorkspace(int64_t batch, int64_t n_rows, int64_t budget) {
+    keys_row = (n_rows + 3) / 4 * 4;
+    moves = batch * keys_row;                                      // (8-byte aligned: a multiple of four words)
+    keep = moves + 2 * batch * budget;
+    keep_count = keep + batch * budget;
+    move_count = keep_count + batch;
+    words = move_count + batch;
+  }
+};
 
-extern "C" int kb200_evict_plan(const int32_t* keep, int64_t keep_stride, const int32_t* keep_count,
-                                const float* mass_in, int64_t mass_stride, const int32_t* pos_in, int64_t pos_stride,
-                                int32_t* moves, int64_t move_stride, int32_t* move_count, int32_t* new_lens, float* mass_out,
-                                int32_t* pos_out, int64_t out_stride, int batch, int n_rows, void* stream) {
-  using namespace kb200;
-  KB_ENTRY(keep, "evict_plan: keep");
-  KB_REQUIRE(keep && keep_count && mass_in && moves && move_count && new_lens && mass_out, "evict_plan: null pointer");
-  KB_REQUIRE(batch >= 0 && batch <= 65535 && n_rows >= 0 && out_stride >= n_rows, "evict_plan: bad sizes");
-  KB_REQUIRE((reinterpret_cast<uintptr_t>(moves) & 7) == 0, "evict_plan: moves must be 8-byte aligned");
-  KB_REQUIRE(move_stride >= keep_stride || move_stride >= n_rows, "evict_plan: %lld moves per sequence may not hold them all",
-             (long long)move_stride);
-  KB_REQUIRE(mass_out != mass_in && (!pos_out || pos_out != pos_in), "evict_plan: an output is its own input");
-  if (batch == 0 || n_rows == 0) return 0;
-  EvictPlanParams p{keep, keep_stride, keep_count, mass_in, mass_stride, pos_in, pos_stride,
-                    reinterpret_cast<int2*>(moves), move_stride, move_count, new_lens, mass_out, pos_out, out_stride, n_rows};
-  KB_LAUNCH("evict_plan_kernel",
-            launch_pdl(evict_plan_kernel, dim3(ceil_div(n_rows, 256), batch), 256, 0, (cudaStream_t)stream, 1, p));
-  return 0;
-}
-
-extern "C" int kb200_evict_move(const kb200_kv_layout* layers, int n_layers, const int32_t* moves, int64_t move_stride,
-                                const int32_t* move_count, int max_moves, int batch, int num_kv_heads, void* stream) {
-  using namespace kb200;
-  KB_REQUIRE(layers && moves && move_count, "evict_move: null pointer");
-  KB_REQUIRE(n_layers >= 0 && max_moves >= 0 && batch >= 0 && batch <= 65535 && num_kv_heads > 0, "evict_move: bad sizes");
-  KB_REQUIRE((reinterpret_cast<uintptr_t>(moves) & 7) == 0, "evict_move: moves must be 8-byte aligned");
-  KB_ENTRY(moves, "evict_move: moves");
-  if (n_layers == 0 || max_moves == 0 || batch == 0) return 0;
+static int check_layers(const kb200_kv_layout* layers, int n_layers) {
   const kb200_kv_layout& one = layers[0];
   const bool int4 = one.dtype == KB200_INT4;
   KB_REQUIRE(one.dtype == KB200_FP16 || one.dtype == KB200_BF16 || int4,
-             "evict_move: fp16, bf16 or INT4 caches (dtype code %d): an FP8 row is stored in the scale of its page and cannot leave it",
+             "evict: fp16, bf16 or INT4 caches (dtype code %d): an FP8 row is stored in the scale of its page and cannot leave it",
              one.dtype);
   KB_REQUIRE(one.page_size >= 1 && (one.page_size & (one.page_size - 1)) == 0,
-             "evict_move: page_size must be a power of two (got %d)", one.page_size);
+             "evict: page_size must be a power of two (got %d)", one.page_size);
   for (int i = 0; i < n_layers; ++i) {
     const kb200_kv_layout& l = layers[i];
-    KB_REQUIRE(l.k && l.v, "evict_move: null cache of layer %d", i);
+    KB_REQUIRE(l.k && l.v, "evict: null cache of layer %d", i);
     KB_REQUIRE(l.dtype == one.dtype && l.page_size == one.page_size && l.block_table == one.block_table &&
                    l.block_table_stride == one.block_table_stride && l.stride_batch == one.stride_batch &&
                    l.stride_page == one.stride_page && l.stride_token == one.stride_token && l.stride_head == one.stride_head &&
                    (!int4 || (l.param_stride_batch == one.param_stride_batch && l.param_stride_page == one.param_stride_page &&
                               l.param_stride_token == one.param_stride_token && l.param_stride_head == one.param_stride_head)),
-               "evict_move: layer %d has another type, block table or strides than layer 0", i);
+               "evict: layer %d has another type, block table or strides than layer 0", i);
     KB_REQUIRE(((reinterpret_cast<uintptr_t>(l.k) | reinterpret_cast<uintptr_t>(l.v)) & 15) == 0 &&
                    ((l.stride_batch | l.stride_page | l.stride_token | l.stride_head) & (int4 ? 15 : 7)) == 0,
-               "evict_move: caches must be 16-byte aligned, with strides that are multiples of 16 bytes");
-    if (int4 && check_int4(&l, true, "evict_move") != 0) return -1;
+               "evict: caches must be 16-byte aligned, with strides that are multiples of 16 bytes");
+    if (int4 && check_int4(&l, true, "evict") != 0) return -1;
   }
+  return 0;
+}
+
+static int move_rows(const kb200_kv_layout* layers, int n_layers, const int2* moves, int64_t move_stride, const int32_t* move_count,
+                     int max_moves, int batch, int num_kv_heads, cudaStream_t st) {
+  const kb200_kv_layout& one = layers[0];
+  const bool int4 = one.dtype == KB200_INT4;
   EvictMoveParams p{};
   const int64_t unit = int4 ? 1 : 2;
   p.sb = one.stride_batch * unit; p.sp = one.stride_page * unit; p.st = one.stride_token * unit; p.sh = one.stride_head * unit;
@@ -325,7 +343,7 @@ extern "C" int kb200_evict_move(const kb200_kv_layout* layers, int n_layers, con
   while ((1 << shift) < one.page_size) ++shift;
   p.page_shift = shift;
   p.page_mask = one.page_size - 1;
-  p.moves = reinterpret_cast<const int2*>(moves);
+  p.moves = moves;
   p.move_stride = move_stride;
   p.move_count = move_count;
   p.G = num_kv_heads;
@@ -339,8 +357,49 @@ extern "C" int kb200_evict_move(const kb200_kv_layout* layers, int n_layers, con
       p.kp[i] = int4 ? static_cast<uint8_t*>(const_cast<void*>(l.k_param)) : nullptr;
       p.vp[i] = int4 ? static_cast<uint8_t*>(const_cast<void*>(l.v_param)) : nullptr;
     }
-    KB_LAUNCH("evict_move_kernel",
-              launch_pdl(evict_move_kernel, dim3(ceil_div(max_moves, 8), n, batch), 256, 0, (cudaStream_t)stream, 1, p));
+    KB_LAUNCH("evict_move_kernel", launch_pdl(evict_move_kernel, dim3(ceil_div(max_moves, 8), n, batch), 256, 0, st, 1, p));
   }
   return 0;
+}
+}  // namespace kb200
+
+extern "C" size_t kb200_evict_workspace_bytes(int batch, int n_rows, int budget) {
+  if (batch <= 0 || n_rows <= 0 || budget <= 0) return 0;
+  return (size_t)kb200::EvictWorkspace(batch, n_rows, budget).words * 4;
+}
+
+extern "C" int kb200_evict(const kb200_kv_layout* layers, int n_layers, const int32_t* seq_lens, const float* mass,
+                           int64_t mass_stride, const int32_t* token_positions, int64_t pos_stride, int budget, int recent,
+                           int sinks, int32_t* new_lens, float* mass_out, int32_t* pos_out, int64_t out_stride, void* workspace,
+                           size_t workspace_bytes, int batch, int num_kv_heads, int n_rows, void* stream) {
+  using namespace kb200;
+  KB_ENTRY(mass, "evict: mass");
+  KB_REQUIRE(layers && seq_lens && mass && new_lens && mass_out && pos_out, "evict: null pointer");
+  KB_REQUIRE(n_layers >= 1 && batch >= 0 && batch <= 65535 && num_kv_heads > 0 && n_rows >= 0, "evict: bad sizes");
+  KB_REQUIRE(budget >= 1 && budget <= (n_rows > 1 ? n_rows : 1) && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget,
+             "evict: a budget of %d rows of %d, %d first and %d last ones protected", budget, n_rows, sinks, recent);
+  KB_REQUIRE(out_stride >= n_rows && mass_out != mass && pos_out != token_positions, "evict: outputs must hold %d rows and not be inputs", n_rows);
+  if (check_layers(layers, n_layers) != 0) return -1;
+  if (batch == 0 || n_rows == 0) return 0;
+  const EvictWorkspace at(batch, n_rows, budget);
+  KB_REQUIRE(workspace && workspace_bytes >= (size_t)at.words * 4 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+             "evict: a 16-byte aligned workspace of %lld bytes is required, got %zu", (long long)at.words * 4, workspace_bytes);
+  int32_t* ws = static_cast<int32_t*>(workspace);
+  float* keys = reinterpret_cast<float*>(ws);
+  cudaStream_t st = (cudaStream_t)stream;
+  // CTAs of a sequence: of 1024 rows at least, while there are SMs for them
+  int ctas = 1;
+  while (ctas < 8 && n_rows > ctas * 2048 && batch * ctas <= sm_count() / 2) ctas *= 2;
+  KB_LAUNCH("evict_keys_kernel",
+            launch_pdl(evict_keys_kernel, dim3(batch * ctas), kKeyThreads, 0, st, ctas,
+                       EvictKeysParams{mass, mass_stride, seq_lens, token_positions, pos_stride, keys, at.keys_row, sinks, recent, n_rows}));
+  if (kb200_topk_select(keys, at.keys_row, n_rows, seq_lens, nullptr, budget, ws + at.keep, budget, ws + at.keep_count, batch, stream) != 0)
+    return -1;
+  int2* moves = reinterpret_cast<int2*>(ws + at.moves);
+  KB_LAUNCH("evict_plan_kernel",
+            launch_pdl(evict_plan_kernel, dim3(ceil_div(n_rows, 256), batch), 256, 0, st, 1,
+                       EvictPlanParams{ws + at.keep, budget, ws + at.keep_count, mass, mass_stride, token_positions, pos_stride, moves,
+                                       ws + at.move_count, new_lens, mass_out, pos_out, out_stride, n_rows}));
+  const int max_moves = n_rows - budget < budget ? n_rows - budget : budget;
+  return max_moves > 0 ? move_rows(layers, n_layers, moves, budget, ws + at.move_count, max_moves, batch, num_kv_heads, st) : 0;
 }

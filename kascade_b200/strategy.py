@@ -684,19 +684,9 @@ class EfficientKascadeStrategy(Strategy):
             raise ValueError(f"attention_mass has {rows} rows, the block table {block_table.shape[1]} pages")
         if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
             seq_lens = seq_lens.to(torch.int32).contiguous()
-        budget = min(int(budget), rows)
         layouts = [nat.kv_layout_paged(c[0], c[1], block_table, *c[2:]) for c in caches]
-        dev = attention_mass.device
-        keys = torch.empty(B, -(-rows // 4) * 4, dtype=torch.float32, device=dev)
-        nat.evict_keys(attention_mass, seq_lens, token_positions, sinks, recent, keys)
-        keep = torch.empty(B, budget, dtype=torch.int32, device=dev)
-        counts = torch.empty(3, B, dtype=torch.int32, device=dev)
-        nat.topk_select(keys, seq_lens, None, budget, keep, counts[0], n_cols=rows)
-        moves = torch.empty(B, budget, 2, dtype=torch.int32, device=dev)
-        mass, positions = torch.empty(B, rows, dtype=torch.float32, device=dev), torch.empty(B, rows, dtype=torch.int32, device=dev)
-        nat.evict_plan(keep, counts[0], attention_mass, token_positions, moves, counts[1], counts[2], mass, positions)
-        nat.evict_move(layouts, moves, counts[1], min(budget, rows - budget), caches[0][0].shape[2])
-        return counts[2], mass, positions
+        return nat.evict(attention_mass, layouts, seq_lens, max(min(int(budget), rows), 1), int(recent), int(sinks), token_positions,
+                         caches[0][0].shape[2])
 
     def paged_decode_forward(self, layer_idx: int, query, key_cache, value_cache, block_table, seq_lens, scaling,
                              max_seq_len: Optional[int] = None, k_scale=None, v_scale=None,

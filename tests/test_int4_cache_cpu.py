@@ -98,9 +98,8 @@ def test_c_entry_points_refuse_before_they_launch():
     layout = nat.KvLayout()
     assert lib.kb200_mass_add(None, 0, None, None, None, 0, 0, 1, 0, None) != 0
     assert lib.kb200_mass_add_prompt(None, 0, None, None, None, 0, 0, 0, 1, 0, 0, None) != 0
-    assert lib.kb200_evict_keys(None, 0, None, None, 0, 0, 0, None, 0, 0, 0, None) != 0
-    assert lib.kb200_evict_plan(None, 0, None, None, 0, None, 0, None, 0, None, None, None, None, 0, 0, 0, None) != 0
-    assert lib.kb200_evict_move(C.byref(layout), 1, None, 0, None, 0, 0, 1, None) != 0
+    assert lib.kb200_evict(C.byref(layout), 1, None, None, 0, None, 0, 1, 0, 0, None, None, None, 0, None, 0, 0, 1, 0, None) != 0
+    assert lib.kb200_evict_workspace_bytes(2, 5, 3) == 4 * (2 * 8 + 2 * (3 + 6) + 4) and lib.kb200_evict_workspace_bytes(0, 5, 3) == 0
     assert lib.kb200_kv_read(C.byref(layout), None, None, None, 0, 0, 1, None) != 0
     act = nat.ActLayout()
     assert lib.kb200_kv_write_at(C.byref(act), None, C.byref(act), C.byref(act), None, None, C.byref(layout), None, None, 0.0, None, 1.0,
