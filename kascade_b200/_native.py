@@ -466,8 +466,19 @@ def decode_workspace(batch: int, heads: int, splits: int, device) -> torch.Tenso
     return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(maxsize=1024)                    # the layers of a step ask the same; the answer follows from the arguments
+def decode_workspace_bytes(batch: int, heads: int, splits: int) -> int:
+    return load().kb200_decode_workspace_bytes(batch, heads, splits)
+
+
+@functools.lru_cache(maxsize=1024)
+def _default_splits(batch: int, groups: int, max_keys: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return init(device).kb200_decode_default_splits(batch, groups, max_keys)
+
+
 def decode_default_splits(batch: int, groups: int, max_keys: int, device: Optional[int] = None) -> int:
-    return init(device).kb200_decode_default_splits(batch, groups, max_keys)
+    return _default_splits(batch, groups, max_keys, torch.cuda.current_device() if device is None else int(device))
 
 
 @functools.lru_cache(maxsize=None)
@@ -480,6 +491,8 @@ def _check_q(q, kv: KvLayout):
     if _half_code(q, "q") != want:
         raise KascadeNativeError(f"q is {q.dtype} but the KV cache has dtype code {kv.dtype} (an FP8 cache takes fp16 q, an INT4 "
                                  "cache the type given as act_dtype)")
+    if kv.dtype == INT4 and kv._keep[0].get_device() != q.get_device():
+        raise KascadeNativeError(f"q is on {q.device}, the KV cache on {kv._keep[0].device}")
 
 
 @_on_device_of(0)
@@ -674,6 +687,8 @@ def kv_write(q_in, q_out, k_new, v_new, start_pos, n_new, kv: KvLayout, q_gain=N
     if q_in is not None:
         _want(q_out, k_new.dtype, "q_out")
         assert q_out.is_contiguous() and q_out.shape == q_in.shape
+    if kv.dtype == INT4 and kv._keep[0].get_device() != k_new.get_device():
+        raise KascadeNativeError(f"the new rows are on {k_new.device}, the KV cache on {kv._keep[0].device}")
     _want(start_pos, torch.int32, "start_pos")
     _want_opt(n_new, torch.int32, "n_new")
     _want_opt(q_gain, k_new.dtype, "q_gain")
@@ -747,7 +762,7 @@ def mass_add(pooled, seq_lens, mass, out, max_len: int):
     B, G, stride = pooled.shape
     _want_rows(mass, torch.float32, B, "mass")
     _want_rows(out, torch.float32, B, "out")
-    if not pooled.is_contiguous() or not seq_lens.is_contiguous() or seq_lens.shape != (B,) or out.stride(0) != mass.stride(0):
+    if not pooled.is_contiguous() or not seq_lens.is_contiguous() or seq_lens.shape != (B,) or (B > 1 and out.stride(0) != mass.stride(0)):
         raise KascadeNativeError("mass_add: pooled and seq_lens must be contiguous, mass and out equally strided")
     if mass.shape[1] < max_len or out.shape[1] < max_len:
         raise KascadeNativeError(f"mass_add: mass holds {mass.shape[1]} rows, {max_len} are needed")
@@ -795,11 +810,13 @@ def evict(mass, layers, seq_lens, budget: int, recent: int, sinks: int, token_po
     if seq_lens.shape != (B,) or not seq_lens.is_contiguous():
         raise KascadeNativeError("evict: seq_lens [B] must be contiguous")
     _same_device(mass, seq_lens=seq_lens, token_positions=token_positions)
-    where = mass.get_device()
-    for layer in layers:
+    where, shape = mass.get_device(), layers[0]._keep[0].shape
+    for i, layer in enumerate(layers):
+        if layer._keep[0].shape != shape:
+            raise KascadeNativeError(f"the cache of layer {i} is {tuple(layer._keep[0].shape)}, that of layer 0 {tuple(shape)}")
         for t in layer._keep:
             if t.get_device() != where:
-                raise KascadeNativeError(f"a cache is on {t.device}, expected {mass.device}")
+                raise KascadeNativeError(f"the cache of layer {i} is on {t.device}, expected {mass.device}")
     dev = mass.device
     lens = torch.empty(B, dtype=torch.int32, device=dev)
     mass_out = torch.empty(B, rows, dtype=torch.float32, device=dev)

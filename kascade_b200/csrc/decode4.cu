@@ -384,11 +384,14 @@ static int init_one() {
 
 int init_decode4() { return init_one<false, true>() || init_one<true, true>() || init_one<true, false>() ? -1 : 0; }
 
-// CTAs of 16 warps, one per SM, while the grid is small; of 8, two per SM, from 1.5 CTAs per SM on, as in decode.cu.
+// CTAs of 16 warps, one per SM, while the grid is small; of 8, two per SM, from 1.5 CTAs per SM on, as in decode.cu; of 4, four per
+// SM, from 6 on: there one CTA's start (lengths -> index -> block table -> rows) and merge are hidden behind three others.  us with 8 /
+// 4 warps: reuse of 128 x 1606 rows 97.5 / 93.9, 256 x 787 102.7 / 94.2; dense passes of 256 x 2048 179 / 160, 16 of 5213..32768 rows in 7
+// splits 115 / 111; but 64 x 3244 rows, 3.5 CTAs per SM, 93 / 102.
 template <bool DENSE, bool HAS_V>
 static cudaError_t launch(const DecodeParams& p, dim3 grid, cudaStream_t st) {
-  const long long total = (long long)grid.x * grid.y * grid.z;
-  const int warps = total * 2 >= 3ll * sm_count() ? kWarps4 / 2 : kWarps4;
+  const long long total = (long long)grid.x * grid.y * grid.z, sms = sm_count();
+  const int warps = total >= 6 * sms ? kWarps4 / 4 : total * 2 >= 3 * sms ? kWarps4 / 2 : kWarps4;
   const size_t smem = (size_t)warps * stages4(HAS_V) * stage_bytes4(HAS_V);
   return launch_pdl(p.bf16 ? decode_attn4_kernel<DENSE, HAS_V, true> : decode_attn4_kernel<DENSE, HAS_V, false>, grid, warps * 32, smem,
                     st, 1, p);

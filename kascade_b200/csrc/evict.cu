@@ -18,13 +18,22 @@ __global__ void __launch_bounds__(128) mass_add_kernel(const float* pooled, int6
   const int j = (blockIdx.x * 128 + threadIdx.x) * 4;
   if (j >= n) return;
   const float* src = pooled + (int64_t)b * G * row_stride + j;
-  float4 a = *reinterpret_cast<const float4*>(src);
-  for (int g = 1; g < G; ++g) {
-    const float4 x = *reinterpret_cast<const float4*>(src + g * row_stride);   // (row_stride is a multiple of 4: readable)
-    a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+  float m[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m[e] = j + e < n ? mass_in[b * mass_stride + j + e] : 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int g0 = 0; g0 < G; g0 += 8) {                               // eight loads in flight
+    float4 x[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g)                                      // (row_stride is a multiple of 4: readable)
+      x[g] = g0 + g < G ? *reinterpret_cast<const float4*>(src + (g0 + g) * row_stride) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < 8; ++g) { a.x += x[g].x; a.y += x[g].y; a.z += x[g].z; a.w += x[g].w; }
   }
   const float s[4] = {a.x, a.y, a.z, a.w};
-  for (int e = 0; e < 4 && j + e < n; ++e) mass_out[b * mass_stride + j + e] = mass_in[b * mass_stride + j + e] + s[e];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j + e < n) mass_out[b * mass_stride + j + e] = m[e] + s[e];
 }
 
 // ---- weight of a prompt ----------------------------------------------------------------------------------------------
@@ -263,7 +272,7 @@ extern "C" int kb200_mass_add(const float* pooled, int64_t row_stride, const int
   KB_REQUIRE(batch >= 0 && batch <= 65535 && num_kv_heads > 0 && max_len >= 0, "mass_add: bad sizes");
   KB_REQUIRE(row_stride % 4 == 0 && row_stride >= max_len && (reinterpret_cast<uintptr_t>(pooled) & 15) == 0,
              "mass_add: pooled rows must be 16-byte aligned (row_stride %% 4 == 0) and hold max_len (%d) scores", max_len);
-  KB_REQUIRE(mass_stride >= max_len, "mass_add: mass holds %lld rows, %d are needed", (long long)mass_stride, max_len);
+  KB_REQUIRE(batch <= 1 || mass_stride >= max_len, "mass_add: mass holds %lld rows, %d are needed", (long long)mass_stride, max_len);
   if (batch == 0 || max_len == 0) return 0;
   KB_LAUNCH("mass_add_kernel", launch_pdl(mass_add_kernel, dim3(ceil_div(max_len, 512), batch), 128, 0, (cudaStream_t)stream, 1,
                                           pooled, row_stride, seq_lens, mass_in, mass_out, mass_stride, num_kv_heads, max_len));
@@ -280,6 +289,7 @@ extern "C" int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, co
   const int64_t need = num_tiles > 0 ? (int64_t)(num_tiles - 1) * kTile : 0;
   KB_REQUIRE(row_stride % 4 == 0 && row_stride >= need && (reinterpret_cast<uintptr_t>(pooled) & 15) == 0,
              "mass_add_prompt: pooled rows must be 16-byte aligned (row_stride %% 4 == 0) and hold %lld scores", (long long)need);
+  KB_REQUIRE(batch <= 1 || (mass_in_stride >= n_rows && mass_out_stride >= n_rows), "mass_add_prompt: rows of mass overlap");
   KB_REQUIRE(n_rows >= need, "mass_add_prompt: mass holds %d rows, %d tiles need %lld", n_rows, num_tiles, (long long)need);
   if (batch == 0 || n_rows == 0) return 0;
   PromptMassParams p{pooled, row_stride, seq_len, mass_in, mass_out, mass_in_stride, mass_out_stride, num_kv_heads, num_tiles, n_rows};

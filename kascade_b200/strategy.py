@@ -269,6 +269,14 @@ class EfficientKascadeStrategy(Strategy):
             y = y.contiguous()
         return y
 
+    @staticmethod
+    def _check_mass(mass, batch: int, rows: int, dev):
+        """attention_mass of a call, before anything is launched."""
+        if mass.dim() != 2 or mass.dtype != torch.float32 or mass.shape[0] != batch or mass.shape[1] < rows or mass.device != dev \
+                or (mass.shape[1] > 1 and mass.stride(1) != 1):
+            raise ValueError(f"attention_mass must be fp32 [{batch}, at least {rows}] on {dev}, the last dimension contiguous, got "
+                             f"{mass.dtype} {tuple(mass.shape)} on {mass.device}")
+
     # ------------------------------------------------------------------------------------------
     def attention_forward(self, module, query, key, value, attention_mask, scaling, dropout=0.0, **kwargs):
         """query [B,H,Lq,D], key/value [B,G,Lk,D] -> (out [B,Lq,H,D], None).
@@ -284,6 +292,8 @@ class EfficientKascadeStrategy(Strategy):
         mass = kwargs.get("attention_mass")
         if mass is not None and self._shard is not None:
             raise NotImplementedError("attention_mass is summed over all heads; a sharded strategy holds some of them")
+        if mass is not None:
+            self._check_mass(mass, query.shape[0], key.shape[2], query.device)
         if query.dtype not in nat.DTYPES or key.dtype != query.dtype or value.dtype != query.dtype:
             raise nat.KascadeNativeError(f"efficient_kascade takes fp16 or bf16 q / k / v of one type; got {query.dtype}, "
                                          f"{key.dtype}, {value.dtype}")
@@ -564,13 +574,13 @@ class EfficientKascadeStrategy(Strategy):
             q = q.contiguous()
         out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
         ragged = float(max_len) / mean_len if mean_len else 1.0
-        splits_a = self._splits(B, G, max_len, ragged, dev)
         if dense_only or self.is_anchor(layer):
+            splits_a = self._splits(B, G, max_len, ragged, dev)
             stride = -(-max_len // 4) * 4
             logits = self._scratch("dec_logits", (B, H, stride), torch.float32, dev)
             pooled = self._scratch("dec_pooled", (B, G, stride), torch.float32, dev)
             lse2 = self._scratch("dec_lse2", (B, H), torch.float32, dev)
-            ws = self._scratch("dec_ws", (nat.load().kb200_decode_workspace_bytes(B, H, splits_a),), torch.uint8, dev)
+            ws = self._scratch("dec_ws", (nat.decode_workspace_bytes(B, H, splits_a),), torch.uint8, dev)
             want_out = dense_only or layer == 0
             nat.decode_anchor_paged(q, kv, seq_lens, max_len, scaling, logits, pooled, out if want_out else None,
                                     lse2, ws, splits_a)
@@ -593,7 +603,7 @@ class EfficientKascadeStrategy(Strategy):
         rows, counts = (self._dec_idx, self._dec_count) if index_rows is None else index_rows
         kmax = rows.shape[2]
         splits = self._splits(B, G, kmax, ragged, dev)
-        ws = self._scratch("dec_ws_s", (nat.load().kb200_decode_workspace_bytes(B, H, splits),), torch.uint8, dev)
+        ws = self._scratch("dec_ws_s", (nat.decode_workspace_bytes(B, H, splits),), torch.uint8, dev)
         nat.decode_sparse_paged(q, kv, rows, counts, kmax, head_map, scaling, out, None, ws, splits)
         return out
 
@@ -615,7 +625,7 @@ class EfficientKascadeStrategy(Strategy):
         The reference has no counterpart (it receives rotated tensors and copies them per call,
         strategies/EfficientKascadeStrategy.py:144-150)."""
         if positions is not None:
-            if positions.dtype.is_floating_point or positions.dim() not in (2, 3):
+            if positions.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8) or positions.dim() not in (2, 3):
                 raise ValueError(f"positions must be integers [B, T] or [axes, B, T], got {positions.dtype} {tuple(positions.shape)}")
             positions = positions.to(torch.int32)
             positions = positions[None] if positions.dim() == 2 else positions
@@ -711,9 +721,13 @@ class EfficientKascadeStrategy(Strategy):
                 raise ValueError(f"layer {layer_idx} is an anchor layer: it selects its own rows")
             rows, counts = index_rows
             want = (query.shape[0], key_cache.shape[2])
-            if rows.dim() != 3 or tuple(rows.shape[:2]) != want or tuple(counts.shape) != want or not counts.is_contiguous():
-                raise ValueError(f"index_rows must be [{want[0]}, {want[1]}, k] and contiguous counts {want}, got "
-                                 f"{tuple(rows.shape)} and {tuple(counts.shape)}")
+            if rows.dim() != 3 or tuple(rows.shape[:2]) != want or tuple(counts.shape) != want or not counts.is_contiguous() \
+                    or rows.stride(2) != 1 or not rows.shape[2] or rows.dtype != torch.int32 or counts.dtype != torch.int32 \
+                    or rows.device != query.device or counts.device != query.device:
+                raise ValueError(f"index_rows must be int32 [{want[0]}, {want[1]}, k], the last dimension contiguous, and contiguous "
+                                 f"int32 counts {want} on {query.device}, got {tuple(rows.shape)} and {tuple(counts.shape)}")
+        if attention_mass is not None:
+            self._check_mass(attention_mass, query.shape[0], int(max_seq_len), query.device)
         kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, query.dtype)
         return self._decode(int(layer_idx), query, kv, seq_lens, int(max_seq_len), scaling, key_cache.shape[2],
                             mean_len=mean_seq_len, mass=attention_mass, index_rows=index_rows)

@@ -292,3 +292,65 @@ def test_a_conversation_in_a_4bit_cache_that_is_kept_short():
             assert all(set(range(int(seen[b]) - recent, int(seen[b]))) <= set(t) and set(range(4)) <= set(t)
                        for b, t in enumerate(tokens))
     assert evictions >= 1 and int(lens[1]) == 85
+
+
+def test_two_evictions_at_once_and_one_after_another():
+    """Two calls on two streams have workspaces of their own; a second eviction of what the first left, with other budgets."""
+    from kascade_b200 import EfficientKascadeStrategy
+    g = torch.Generator().manual_seed(23)
+    S, G = 900, 2
+    table, pages = _tables([S, S - 100], S, 16, 23)
+    masses = [torch.rand(2, S, generator=g) for _ in range(2)]
+    caches = [tuple(torch.randn(pages, 16, G, 128, generator=g).half().cuda() for _ in range(2)) for _ in range(2)]
+    before = [[x.cpu().clone() for x in c] for c in caches]
+    table_d, lens, dev = table.cuda(), torch.tensor([S, S - 100], dtype=torch.int32, device="cuda"), [m.cuda() for m in masses]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for st, cache, m, budget in zip(streams, caches, dev, (400, 650)):
+        with torch.cuda.stream(st):
+            got.append(EfficientKascadeStrategy.evict_kv([cache], table_d, lens, m, budget, recent=7, sinks=2))
+    torch.cuda.synchronize()
+    for i, budget in enumerate((400, 650)):
+        moves, left, want_mass, want_pos = _plain_evict([S, S - 100], masses[i], None, budget, 7, 2)
+        assert got[i][0].tolist() == left and torch.equal(got[i][1].cpu(), want_mass) and torch.equal(got[i][2].cpu(), want_pos)
+        for x, y in zip(before[i], caches[i]):
+            for b, pairs in enumerate(moves):
+                for s, t in pairs:
+                    x[int(table[b, t // 16]), t % 16] = x[int(table[b, s // 16]), s % 16]
+            assert torch.equal(y.cpu(), x)
+    # again, from the rows that are left
+    again = EfficientKascadeStrategy.evict_kv([caches[0]], table_d, got[0][0], got[0][1], 100, recent=7, sinks=2, token_positions=got[0][2])
+    moves, left, want_mass, want_pos = _plain_evict([400, 400], got[0][1].cpu(), got[0][2].cpu(), 100, 7, 2)
+    assert again[0].tolist() == left and torch.equal(again[1].cpu(), want_mass) and torch.equal(again[2].cpu(), want_pos)
+    for x, y in zip(before[0], caches[0]):
+        for b, pairs in enumerate(moves):
+            for s, t in pairs:
+                x[int(table[b, t // 16]), t % 16] = x[int(table[b, s // 16]), s % 16]
+        assert torch.equal(y.cpu(), x)
+
+
+def test_more_protected_rows_than_the_budget_holds():
+    """Rows that share a position (images on several axes) can be more than `recent`: the lowest of them stay."""
+    mass = torch.rand(1, 64, generator=torch.Generator().manual_seed(3))
+    positions = torch.full((1, 64), 5, dtype=torch.int32)
+    positions[0, 40:] = 9
+    _run_evict([64], 64, 10, 6, 0, 1, 16, 1, torch.float16, mass, positions)
+
+
+def test_refusals_of_attention_mass():
+    from kascade_b200 import EfficientKascadeStrategy
+    strat = EfficientKascadeStrategy([0], "x/y", k=20, tile_size=32, head_mapping=[[0, 1]] * 2, register=False)
+    k, v, kp, vp, table, _, _, _ = make_cache([200], 2, 16, seed=1)
+    q, lens = torch.zeros(1, 8, 128, dtype=torch.float16, device="cuda"), torch.tensor([200], device="cuda")
+    good = torch.zeros(1, 200, device="cuda")
+    for bad in (good[:, :199], good.double(), good.cpu(), torch.zeros(2, 200, device="cuda"), torch.zeros(1, 400, device="cuda")[:, ::2], good[0]):
+        with pytest.raises(ValueError, match="attention_mass"):
+            strat.paged_decode_forward(0, q, k, v, table, lens, 0.1, 200, kp, vp, attention_mass=bad)
+    x, kv = torch.zeros(1, 8, 140, 128, dtype=torch.float16, device="cuda"), torch.zeros(1, 2, 140, 128, dtype=torch.float16, device="cuda")
+
+    class M:
+        layer_idx = 0
+
+    with pytest.raises(ValueError, match="attention_mass"):
+        strat.attention_forward(M(), x, kv, kv, None, 0.1, attention_mass=good[:, :139])

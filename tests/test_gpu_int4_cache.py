@@ -415,3 +415,59 @@ def test_refusals_of_the_4bit_cache():
         strat.paged_decode_forward(0, q, k, v, table, torch.ones(1, device="cuda"), 0.1, 64, kp, vp, index_rows=(rows, rows[..., 0]))
     with pytest.raises(ValueError, match="index_rows"):
         strat.paged_decode_forward(1, q, k, v, table, torch.ones(1, device="cuda"), 0.1, 64, kp, vp, index_rows=(rows, rows))
+
+
+def test_many_sequences_take_small_ctas():
+    """Batches of 6 CTAs per SM and more run with four warps per CTA."""
+    from kascade_b200 import _native as nat
+    B, G = 112, 8
+    lens = [(37 * i) % 90 + 1 for i in range(B)]
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, 16, seed=81)
+    q = _queries(B, 4 * G, torch.float16, 82)
+    seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    rows = torch.arange(90, dtype=torch.int32, device="cuda").expand(B, G, 90)
+    counts = seq[:, None].expand(B, G).contiguous()
+    out, lse = torch.empty(B, 4 * G, 128, dtype=torch.float16, device="cuda"), torch.empty(B, 4 * G, device="cuda")
+    kv = nat.kv_layout_paged(k, v, table, kp, vp)
+    nat.decode_sparse_paged(q, kv, rows, counts, 90, None, 128 ** -0.5, out, lse, None, 1)
+    _check_attention(out[:20], lse[:20], q[:20], kf[:20], vf[:20], vc[:20], lambda b, h: list(range(lens[b])), 128 ** -0.5, torch.float16,
+                     "112 sequences, sparse")
+    ws = nat.decode_workspace(B, 4 * G, 2, q.device)
+    two = torch.empty_like(out)
+    nat.decode_sparse_paged(q, kv, rows, counts, 90, None, 128 ** -0.5, two, None, ws, 2)
+    logits, pooled = torch.empty(B, 4 * G, 92, device="cuda"), torch.empty(B, G, 92, device="cuda")
+    dense = torch.empty_like(out)
+    nat.decode_anchor_paged(q, kv, seq, 90, 128 ** -0.5, logits, pooled, dense, lse, None, 1)
+    for x in (two, dense):                                           # other splits and orders of sums: a step of fp16 apart at most
+        assert float((x.float() - out.float()).abs().max()) <= 2.0 ** -9 * float(out.abs().max())
+
+
+def test_rows_of_a_cache_beyond_32_bits():
+    """Rows whose byte offsets pass 2^31 and 2^32: written, read back and attended to."""
+    from kascade_b200 import _native as nat
+    G, page = 2, 16
+    strat = _strategy(G)
+    stride = 3 * 2 ** 20                                              # bytes from page to page: 1500 pages span 4.7 GB
+    pages = 1500
+    store = torch.empty(2, pages * stride, dtype=torch.uint8, device="cuda")
+    params = torch.empty(2, pages, page, G, 8, dtype=torch.float16, device="cuda")
+    k, v = (x.as_strided((pages, page, G, 64), (stride, G * 64, 64, 1)) for x in store)
+    table = torch.tensor([[0, 700, 1499, 1400]], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(91)
+    x = torch.randn(1, 60, 2 * G, 128, generator=g).half()
+    strat.append_kv(x[:, :, :G].cuda(), x[:, :, G:].cuda(), k, v, table, torch.zeros(1, dtype=torch.int32, device="cuda"), k_scale=params[0],
+                    v_scale=params[1])
+    n = torch.tensor([60], dtype=torch.int32, device="cuda")
+    ko, vo = strat.read_kv(k, v, table, n, 60, k_scale=params[0], v_scale=params[1])
+    want = []
+    for part, pieces in ((x[0, :, :G], K_PIECES), (x[0, :, G:], V_PIECES)):
+        codes, par = quantize(part)
+        want.append((unpack(pack(codes, pieces), par, pieces), unpack(pack(codes, pieces), par, pieces, False)))
+    for got, (w, _) in zip((ko, vo), want):
+        assert bool(((got[0].cpu().double() - w).abs() <= (2.0 ** -11 + 2.0 ** -23) * w.abs()).all())
+    q = _queries(1, 4 * G, torch.float16, 92)
+    out = torch.empty_like(q)
+    rows = torch.arange(60, dtype=torch.int32, device="cuda").expand(1, G, 60)
+    nat.decode_sparse_paged(q, nat.kv_layout_paged(k, v, table, params[0], params[1]), rows, None, 60, None, 0.08, out, None, None, 1)
+    kf, vf, vc = (y.transpose(0, 1)[None] for y in (want[0][0], want[1][0], want[1][1]))
+    _check_attention(out, None, q, kf, vf, vc, lambda b, h: list(range(60)), 0.08, torch.float16, "far pages")
