@@ -255,13 +255,13 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
         if (key0 + 16 * i + grp + 8 >= n) x[i][2] = x[i][3] = -INFINITY;
       }
     }
-    if (DENSE && quad < 2) {
-      float* lp = p.logits + ((int64_t)b * p.H + g * kHg + quad * 2) * p.logit_stride + key0 + grp;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (key0 + 16 * i + grp < n) { lp[16 * i] = x[i][0]; lp[p.logit_stride + 16 * i] = x[i][1]; }
-        if (key0 + 16 * i + grp + 8 < n) { lp[16 * i + 8] = x[i][2]; lp[p.logit_stride + 16 * i + 8] = x[i][3]; }
-      }
+    if (DENSE) {
+      // columns 4-7 are the same heads again: the lanes of quads 0, 1 write the first 16 keys, the others the last
+      const int half = quad >> 1;
+      float* lp = p.logits + ((int64_t)b * p.H + g * kHg + (quad & 1) * 2) * p.logit_stride + key0 + 16 * half + grp;
+      const int keys = n - (key0 + 16 * half + grp);
+      if (keys > 0) { lp[0] = half ? x[1][0] : x[0][0]; lp[p.logit_stride] = half ? x[1][1] : x[0][1]; }
+      if (keys > 8) { lp[8] = half ? x[1][2] : x[0][2]; lp[p.logit_stride + 8] = half ? x[1][3] : x[0][3]; }
     }
     // ---- exponentials against the reference of either head ---------------------------------------------
     float t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])), t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
