@@ -227,9 +227,10 @@ def _on_device_of(arg_index: int):
         @functools.wraps(fn)
         def wrapped(*args, **kwargs):
             t = args[arg_index]
-            if not t.is_cuda:
+            where = t.get_device()                               # (-1: not on a GPU)
+            if where < 0:
                 raise KascadeNativeError(f"{fn.__name__}: expected CUDA tensors, got one on {t.device}")
-            if t.get_device() == torch._C._cuda_getDevice():     # (a CUDA tensor exists: the runtime is up)
+            if where == torch._C._cuda_getDevice():              # (a CUDA tensor exists: the runtime is up)
                 return fn(*args, **kwargs)
             with torch.cuda.device(t.device):
                 return fn(*args, **kwargs)
@@ -239,7 +240,7 @@ def _on_device_of(arg_index: int):
 
 def _stream() -> int:
     """cudaStream_t of the current device's current stream (read as a handle, without building a torch.cuda.Stream)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())      # (a CUDA tensor exists: the runtime is up)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -252,7 +253,7 @@ def _want_opt(t: Optional[torch.Tensor], dtype, name: str):
 
 
 def _want(t: torch.Tensor, dtype, name: str):
-    if t.dtype != dtype or not t.is_cuda:
+    if t.dtype is not dtype or not t.is_cuda:
         raise KascadeNativeError(f"{name}: expected a CUDA {dtype} tensor, got {t.dtype} on {t.device}")
 
 
@@ -265,9 +266,10 @@ def _same_device(first: torch.Tensor, **others: Optional[torch.Tensor]):
 
 def _half_code(t: torch.Tensor, name: str) -> int:
     """KB200_FP16 / KB200_BF16 of a CUDA fp16 or bf16 tensor."""
-    if t.dtype not in DTYPES or not t.is_cuda:
+    code = DTYPES.get(t.dtype)
+    if code is None or not t.is_cuda:
         raise KascadeNativeError(f"{name}: expected a CUDA fp16 or bf16 tensor, got {t.dtype} on {t.device}")
-    return DTYPES[t.dtype]
+    return code
 
 
 # ------------------------------------------------------------------------------------------------
@@ -390,10 +392,11 @@ def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], bloc
             _want(block_table, torch.int32, "block_table")
             _same_device(k_cache, block_table=block_table)
             raise KascadeNativeError("block_table: expected [B, max_pages], the last dimension contiguous")
-        return _holding(KvLayout(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2],
-                                 block_table.data_ptr(), ts[0], k_cache.shape[1], INT4, 0, 0, 0, 0, 0, k_scale.data_ptr(),
-                                 0 if v_cache is None else v_scale.data_ptr(), 0, ps[0], ps[1], ps[2], DTYPES[act_dtype]),
-                        k_cache, v_cache, block_table, k_scale, v_scale)
+        layout = KvLayout(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2],
+                          block_table.data_ptr(), ts[0], k_cache.shape[1], INT4, 0, 0, 0, 0, 0, k_scale.data_ptr(),
+                          0 if v_cache is None else v_scale.data_ptr(), 0, ps[0], ps[1], ps[2], DTYPES[act_dtype])
+        layout._keep = (k_cache, block_table, k_scale) if v_cache is None else (k_cache, v_cache, block_table, k_scale, v_scale)
+        return layout
     if k_cache.dtype in FP8_TORCH:
         assert k_cache.is_cuda and k_cache.dim() == 4 and k_cache.stride(3) == 1
         assert block_table.dtype == torch.int32 and block_table.stride(1) == 1
@@ -407,14 +410,15 @@ def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], bloc
                                  0 if v_scale is None else v_scale.data_ptr(), 0, k_scale.stride(0), k_scale.stride(1)),
                         k_cache, v_cache, block_table, k_scale, v_scale)
     code = _half_code(k_cache, "k_cache")
-    st = k_cache.stride()
+    st, ts = k_cache.stride(), block_table.stride()
     assert len(st) == 4 and st[3] == 1
-    assert block_table.dtype == torch.int32 and block_table.stride(1) == 1
+    assert block_table.dtype is torch.int32 and ts[1] == 1
     if v_cache is not None:
-        assert v_cache.shape == k_cache.shape and v_cache.stride() == st and v_cache.dtype == k_cache.dtype
-    return _holding(KvLayout(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2],
-                             block_table.data_ptr(), block_table.stride(0), k_cache.shape[1], code),
-                    k_cache, v_cache, block_table)
+        assert v_cache.shape == k_cache.shape and v_cache.stride() == st and v_cache.dtype is k_cache.dtype
+    layout = KvLayout(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2],
+                      block_table.data_ptr(), ts[0], k_cache.shape[1], code)
+    layout._keep = (k_cache, block_table) if v_cache is None else (k_cache, v_cache, block_table)
+    return layout
 
 
 def kv_layout_contiguous(k: torch.Tensor, v: Optional[torch.Tensor], page_size: int = 16,
@@ -507,10 +511,11 @@ def decode_sparse_paged(q, kv: KvLayout, topk_idx, topk_count, k_max, head_map, 
     _want_opt(head_map, torch.int32, "head_map")
     B, H, D = q.shape
     G = topk_idx.shape[1]
-    assert D == HEAD_DIM and q.stride(2) == 1 and out.is_contiguous() and topk_idx.stride(2) == 1
+    qs, xs = q.stride(), topk_idx.stride()
+    assert D == HEAD_DIM and qs[2] == 1 and out.is_contiguous() and xs[2] == 1
     _check(lib.kb200_decode_sparse_paged(
-        _ptr(q), q.stride(0), q.stride(1), C.byref(kv), _ptr(topk_idx), topk_idx.stride(0), topk_idx.stride(1),
-        _ptr(topk_count), k_max, _ptr(head_map), float(scale), _ptr(out), _ptr(lse2), _ptr(workspace),
+        q.data_ptr(), qs[0], qs[1], C.byref(kv), topk_idx.data_ptr(), xs[0], xs[1], _ptr(topk_count), k_max, _ptr(head_map),
+        float(scale), out.data_ptr(), _ptr(lse2), _ptr(workspace),
         0 if workspace is None else workspace.numel() * workspace.element_size(), B, H, G, num_splits, _stream()),
         "kb200_decode_sparse_paged")
     ns = num_splits if num_splits else lib.kb200_decode_default_splits(B, G, k_max)
@@ -552,11 +557,12 @@ def decode_anchor_paged(q, kv: KvLayout, seq_lens, max_seq_len, scale, logits, p
     _want(logits, torch.float32, "logits")
     _want(pooled, torch.float32, "pooled")
     B, H, D = q.shape
-    G = pooled.shape[1]
-    assert logits.is_contiguous() and pooled.is_contiguous() and logits.shape[-1] == pooled.shape[-1]
+    G, stride = pooled.shape[1:]
+    qs = q.stride()
+    assert logits.is_contiguous() and pooled.is_contiguous() and logits.shape[-1] == stride
     _check(lib.kb200_decode_anchor_paged(
-        _ptr(q), q.stride(0), q.stride(1), C.byref(kv), _ptr(seq_lens), max_seq_len, float(scale), _ptr(logits),
-        _ptr(pooled), logits.shape[-1], _ptr(out), _ptr(lse2), _ptr(workspace),
+        q.data_ptr(), qs[0], qs[1], C.byref(kv), seq_lens.data_ptr(), max_seq_len, float(scale), logits.data_ptr(),
+        pooled.data_ptr(), stride, _ptr(out), _ptr(lse2), _ptr(workspace),
         0 if workspace is None else workspace.numel() * workspace.element_size(), B, H, G, num_splits, _stream()),
         "kb200_decode_anchor_paged")
     ns = num_splits if num_splits else lib.kb200_decode_default_splits(B, G, max_seq_len)
@@ -565,10 +571,9 @@ def decode_anchor_paged(q, kv: KvLayout, seq_lens, max_seq_len, scale, logits, p
 
 def act_layout(x: torch.Tensor) -> ActLayout:
     """x indexed [B, L, heads, D] (any strides, D contiguous)."""
-    code = _half_code(x, "activation")
-    st = x.stride()
-    assert len(st) == 4 and st[3] == 1 and x.shape[3] == HEAD_DIM
-    return ActLayout(x.data_ptr(), st[0], st[1], st[2], code)
+    b, t, h, d = x.stride()
+    assert d == 1 and x.shape[3] == HEAD_DIM
+    return ActLayout(x.data_ptr(), b, t, h, _half_code(x, "activation"))
 
 
 @_on_device_of(0)

@@ -570,7 +570,8 @@ class EfficientKascadeStrategy(Strategy):
                 mean_len: Optional[float] = None, mass=None, index_rows=None) -> torch.Tensor:
         B, H, D = q.shape
         dev = q.device
-        if q.stride(2) != 1 or q.stride(0) % 2 or q.stride(1) % 2:
+        sb, sh, sd = q.stride()
+        if sd != 1 or sb % 2 or sh % 2:
             q = q.contiguous()
         out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
         ragged = float(max_len) / mean_len if mean_len else 1.0
