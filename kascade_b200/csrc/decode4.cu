@@ -8,7 +8,7 @@
 // At 160 bytes a key the copies leave a warp scheduler some 230 issue slots per eight keys, so the rows are never turned into
 // fp16 values.  A code in the low bits of an fp16 word IS a number: the subnormal c 2^-24, or 16 c 2^-24 four bits further
 // up, and the tensor core takes subnormals as they are.  One AND therefore makes a pair of matrix operands from a word of
-// codes (two, after a shift by eight), and scales and zeros are applied where they are few:
+// codes (two, after a shift), and scales and zeros are applied where they are few:
 //   * S = K Q^T, keys as rows:  S = sum_g s_g (sum_{d in g} c_d q_d) + sum_g z_g (sum_{d in g} q_d).  Two products of 16 d for each
 //     group, whose sums are scaled by the key's s_g in fp32; the zeros are one more product, of the keys' parameters with the
 //     queries' sums over the groups (as two fp16 terms, exact to 2^-22).
@@ -29,8 +29,19 @@ constexpr int kCodeOne = 1 << 24;                          // 1 / (the value of 
 // most 4, so that their products with a scale (s <= 8734) stay in fp16's range, and the maximum over the lanes, the
 // factors and the rescaling of O are needed in a few steps per list only.
 constexpr float kSlack4 = 2.f;
+// The tensor core rounds its sums towards zero: by about 2^-24 of the accumulator per product, always the same way.  The codes' mean
+// is 7.5, so their share of O grows with the list while O itself, with the zeros' share taken off, does not: after 512 products that
+// was 0.4 % of O for 131072 keys.  (And it aligns products by their operands' exponent fields, so a subnormal loses what it lies below
+// 2^-14; V's codes are shifted two bits up for that.)  So every kFlush4 steps what the accumulators of a group have in common (one of them) is taken off
+// all of them and added up apart, rounded to nearest, in a few words per lane of shared memory.  Error of fp16 outputs against 64
+// bits, 131072 keys in 1 / 18 splits: 4.0e-3 / 5.3e-4 without, 6e-4 unshifted, 3.0e-4 / 2.8e-4 as it is (2.9e-4 is what the rounding
+// of probabilities and outputs to fp16 makes); every 8 steps 3.3e-4, every 16 4.6e-4.  It takes 1-2 % of a dense pass.
+constexpr int kFlush4 = 4;
+constexpr int kTracks4 = 10;                               // per lane: four groups and the zeros, two heads each
+constexpr int kTrackBytes4 = kTracks4 * 32 * 4;            // per warp
 __host__ __device__ constexpr int stages4(bool has_v) { return has_v ? 2 : 4; }
 __host__ __device__ constexpr int stage_bytes4(bool has_v) { return has_v ? 2 * kHalf4 : kHalf4; }
+__host__ __device__ constexpr int warp_bytes4(bool has_v) { return stages4(has_v) * stage_bytes4(has_v) + (has_v ? kTrackBytes4 : 0); }
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -198,6 +209,27 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
     for (int i = 0; i < 4; ++i) o_acc[e][0][i] = o_acc[e][1][i] = 0.f;
   }
   float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
+  float* track = reinterpret_cast<float*>(smem + WARPS * (kStages * kStage) + warp * kTrackBytes4) + lane;   // [10], 32 apart
+  if (HAS_V) {
+#pragma unroll
+    for (int i = 0; i < kTracks4; ++i) track[i * 32] = 0.f;
+  }
+  auto flush = [&] {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mean = o_acc[e][0][r];
+        track[(e * 2 + r) * 32] += mean;
+        o_acc[e][0][r] = 0.f;
+        o_acc[e][1][r] -= mean;
+        o_acc[e][0][2 + r] = fmaf(-16.f, mean, o_acc[e][0][2 + r]);
+        o_acc[e][1][2 + r] = fmaf(-16.f, mean, o_acc[e][1][2 + r]);
+      }
+      track[(8 + r) * 32] += o_zero[r];
+      o_zero[r] = 0.f;
+    }
+  };
 
   // p s in fp16 for columns 0-3, and for columns 4-7 (the same heads) what its rounding left, exactly: the products with the
   // codes, whose mean is far from zero, would carry the rounding of p s twice as far as that of p.  bf16 outputs are rounded
@@ -285,7 +317,9 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
             o_acc[e][f][0] *= alpha0; o_acc[e][f][1] *= alpha1; o_acc[e][f][2] *= alpha0; o_acc[e][f][3] *= alpha1;
           }
         }
-        o_zero[0] *= alpha0; o_zero[1] *= alpha1; o_zero[2] *= alpha0; o_zero[3] *= alpha1;
+        o_zero[0] *= alpha0; o_zero[1] *= alpha1;
+#pragma unroll
+        for (int i = 0; i < kTracks4; ++i) track[i * 32] *= i & 1 ? alpha1 : alpha0;
       }
     }
     float w[2][4];
@@ -315,14 +349,29 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
           const uint32_t hi = __byte_perm(e < 2 ? kc.x : kc.y, e < 2 ? kd.x : kd.y, sel);      // ... + 8
           const uint32_t sb0 = scaled(pb0, __shfl_sync(FULL, z0, e * 4 + quad));
           const uint32_t sb1 = scaled(pb1, __shfl_sync(FULL, z1, e * 4 + quad));
-          mma16816<false>(o_acc[e][0], lo & 0x000F000Fu, lo & 0x00F000F0u, hi & 0x000F000Fu, hi & 0x00F000F0u, sb0, sb1);
-          const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
-          mma16816<false>(o_acc[e][1], lo8 & 0x000F000Fu, lo8 & 0x00F000F0u, hi8 & 0x000F000Fu, hi8 & 0x00F000F0u, sb0, sb1);
+          const uint32_t lo2 = lo << 2, hi2 = hi << 2, lo6 = lo >> 6, hi6 = hi >> 6;
+          mma16816<false>(o_acc[e][0], lo2 & 0x003C003Cu, lo2 & 0x03C003C0u, hi2 & 0x003C003Cu, hi2 & 0x03C003C0u, sb0, sb1);
+          mma16816<false>(o_acc[e][1], lo6 & 0x003C003Cu, lo6 & 0x03C003C0u, hi6 & 0x003C003Cu, hi6 & 0x03C003C0u, sb0, sb1);
         }
       }
+      if ((j & (kFlush4 - 1)) == kFlush4 - 1) flush();
     }
   }
   cp_async_wait<0>();
+  if (HAS_V) {                         // what was taken off comes back, rounded to nearest like every sum of it
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mean = track[(e * 2 + r) * 32];
+        o_acc[e][0][r] += mean;
+        o_acc[e][1][r] += mean;
+        o_acc[e][0][2 + r] = fmaf(16.f, mean, o_acc[e][0][2 + r]);
+        o_acc[e][1][2 + r] = fmaf(16.f, mean, o_acc[e][1][2 + r]);
+      }
+      o_zero[r] += track[(8 + r) * 32];
+    }
+  }
   __syncthreads();
   pdl_trigger();                       // only the merge is left: most SMs have room by now
 
@@ -361,10 +410,10 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float4 o;
-          o.x = fmaf(o_acc[e][0][r], (float)kCodeOne, zero[e][r]);
-          o.y = fmaf(o_acc[e][0][2 + r], (float)(kCodeOne / 16), zero[e][r]);
-          o.z = fmaf(o_acc[e][1][r], (float)kCodeOne, zero[e][r]);
-          o.w = fmaf(o_acc[e][1][2 + r], (float)(kCodeOne / 16), zero[e][r]);
+          o.x = fmaf(o_acc[e][0][r], (float)(kCodeOne / 4), zero[e][r]);
+          o.y = fmaf(o_acc[e][0][2 + r], (float)(kCodeOne / 64), zero[e][r]);
+          o.z = fmaf(o_acc[e][1][r], (float)(kCodeOne / 4), zero[e][r]);
+          o.w = fmaf(o_acc[e][1][2 + r], (float)(kCodeOne / 64), zero[e][r]);
           *reinterpret_cast<float4*>(sm_o + (warp * kHg + h) * kD + 32 * e + 4 * grp) = o;
         }
       }
@@ -376,7 +425,7 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
 
 template <bool DENSE, bool HAS_V>
 static int init_one() {
-  const int bytes = kWarps4 * stages4(HAS_V) * stage_bytes4(HAS_V);
+  const int bytes = kWarps4 * warp_bytes4(HAS_V);
   KB_CUDA(cudaFuncSetAttribute(decode_attn4_kernel<DENSE, HAS_V, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   KB_CUDA(cudaFuncSetAttribute(decode_attn4_kernel<DENSE, HAS_V, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   return 0;
@@ -392,7 +441,7 @@ template <bool DENSE, bool HAS_V>
 static cudaError_t launch(const DecodeParams& p, dim3 grid, cudaStream_t st) {
   const long long total = (long long)grid.x * grid.y * grid.z, sms = sm_count();
   const int warps = total >= 6 * sms ? kWarps4 / 4 : total * 2 >= 3 * sms ? kWarps4 / 2 : kWarps4;
-  const size_t smem = (size_t)warps * stages4(HAS_V) * stage_bytes4(HAS_V);
+  const size_t smem = (size_t)warps * warp_bytes4(HAS_V);
   return launch_pdl(p.bf16 ? decode_attn4_kernel<DENSE, HAS_V, true> : decode_attn4_kernel<DENSE, HAS_V, false>, grid, warps * 32, smem,
                     st, 1, p);
 }

@@ -471,3 +471,22 @@ def test_rows_of_a_cache_beyond_32_bits():
     nat.decode_sparse_paged(q, nat.kv_layout_paged(k, v, table, params[0], params[1]), rows, None, 60, None, 0.08, out, None, None, 1)
     kf, vf, vc = (y.transpose(0, 1)[None] for y in (want[0][0], want[1][0], want[1][1]))
     _check_attention(out, None, q, kf, vf, vc, lambda b, h: list(range(60)), 0.08, torch.float16, "far pages")
+
+
+@pytest.mark.parametrize("splits", [1, 7])
+@pytest.mark.parametrize("n", [40000, 8191])
+def test_sums_over_long_lists_are_not_rounded_one_way(n, splits):
+    """All rows weigh the same (queries of zero), so every probability is exact and out is the mean of the values: small, while the
+    codes' and the zeros' shares of it are large and opposite.  Sums that are rounded towards zero would drift apart."""
+    from kascade_b200 import _native as nat
+    k, v, kp, vp, table, kf, vf, vc = make_cache([n], 1, 16, seed=101, spread=0.0)
+    q = torch.zeros(1, 4, 128, dtype=torch.float16, device="cuda")
+    rows = torch.arange(n, dtype=torch.int32, device="cuda").view(1, 1, n)
+    out, lse = torch.empty_like(q), torch.empty(1, 4, device="cuda")
+    ws = nat.decode_workspace(1, 4, splits, q.device)
+    nat.decode_sparse_paged(q, nat.kv_layout_paged(k, v, table, kp, vp), rows, None, n, None, 1.0, out, lse, ws, splits)
+    want = vf[0, 0].mean(0)
+    # the output's rounding, and 32-bit sums of either share: steps of 2^-24, at most 8 of them between two that are rounded to nearest
+    bound = 2.0 ** -11 * want.abs() + 2.0 ** -21 * (vc[0, 0].mean(0) + (vf - vc)[0, 0].abs().mean(0))
+    assert bool(((out[0].cpu().double() - want).abs() <= bound).all())
+    assert float((lse.cpu().double() - math.log2(n)).abs().max()) <= 2.0 ** -20 * math.log2(n)
