@@ -538,7 +538,8 @@ static void launch_kv_append(const KvWriteParams& p, int store, int64_t tokens, 
   else launch_kv_append<BF16, kSame, true>(p, tokens, st);
 }
 
-// Rows of a 4-bit cache in 16 bits: eight lanes per row, lane c the values 8c .. 8c+7 and 64+8c .. 64+8c+7 of K and of V.
+// Rows of a 4-bit cache in 16 bits: four lanes per row.  Lane q loads 16 bytes of the codes of K, which are the values 8q .. 8q+7 of
+// every group, and 16 of V, which are the same values in two pieces, and the eight parameters of either.
 struct KvReadParams {
   const uint8_t* k; const uint8_t* v; int64_t c_sb, c_sp, c_st, c_sh;
   const __half* k_param; const __half* v_param; int64_t pa_sb, pa_sp, pa_st, pa_sh;
@@ -548,6 +549,7 @@ struct KvReadParams {
   int T, G; int64_t rows;
 };
 
+// the eight values of a word of codes, the lowest nibble first
 template <bool BF16>
 __device__ __forceinline__ uint4 from_codes(uint32_t w, float s, float z) {
   using H2 = typename Pair<BF16>::T;
@@ -560,34 +562,34 @@ __device__ __forceinline__ uint4 from_codes(uint32_t w, float s, float z) {
 
 template <bool BF16>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
-  const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  const int c = threadIdx.x & 7, g4 = c >> 2, q = c & 3;
+  const int64_t row = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 2);
+  const int q = threadIdx.x & 3;
   if (row >= p.rows) return;
-  const int head = (int)(row % p.G);
   const int64_t token = row / p.G;
-  const int b = (int)(token / p.T), t = (int)(token - (int64_t)b * p.T);
-  uint4 kl = make_uint4(0u, 0u, 0u, 0u), kh = kl, vl = kl, vh = kl;     // rows behind a sequence read as zeros
-  if (t < p.seq_lens[b]) {
-    const int lp = t >> p.page_shift, slot = t & p.page_mask;
-    const int64_t page = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + lp] : lp;
-    const int64_t at = b * p.c_sb + page * p.c_sp + slot * p.c_st + head * p.c_sh;
-    const int64_t pa = b * p.pa_sb + page * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
-    const __half* kp = p.k_param + pa;
-    const __half* vp = p.v_param + pa;
-    const uint32_t* kw = reinterpret_cast<const uint32_t*>(p.k + at);
-    const uint16_t* vw = reinterpret_cast<const uint16_t*>(p.v + at);
-    auto v_word = [&](int g) { return (uint32_t)vw[2 * q * 4 + g] | ((uint32_t)vw[(2 * q + 1) * 4 + g] << 16); };
-    kl = from_codes<BF16>(kw[q * 4 + g4], __half2float(kp[g4]), __half2float(kp[4 + g4]));
-    kh = from_codes<BF16>(kw[q * 4 + g4 + 2], __half2float(kp[g4 + 2]), __half2float(kp[6 + g4]));
-    vl = from_codes<BF16>(v_word(g4), __half2float(vp[g4]), __half2float(vp[4 + g4]));
-    vh = from_codes<BF16>(v_word(g4 + 2), __half2float(vp[g4 + 2]), __half2float(vp[6 + g4]));
+  const int head = (int)(row - token * p.G), b = (int)(token / p.T), t = (int)(token - (int64_t)b * p.T);
+  uint4* ko = reinterpret_cast<uint4*>(p.k_out + row * kD) + q;          // group g: 16-byte piece 4 g + q
+  uint4* vo = reinterpret_cast<uint4*>(p.v_out + row * kD) + q;
+  if (t >= p.seq_lens[b]) {                                              // rows behind a sequence read as zeros
+#pragma unroll
+    for (int g = 0; g < 4; ++g) ko[4 * g] = vo[4 * g] = make_uint4(0u, 0u, 0u, 0u);
+    return;
   }
-  uint4* ko = reinterpret_cast<uint4*>(p.k_out + row * kD);
-  uint4* vo = reinterpret_cast<uint4*>(p.v_out + row * kD);
-  ko[c] = kl;
-  ko[c + 8] = kh;
-  vo[c] = vl;
-  vo[c + 8] = vh;
+  const int lp = t >> p.page_shift, slot = t & p.page_mask;
+  const int64_t page = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + lp] : lp;
+  const int64_t at = b * p.c_sb + page * p.c_sp + slot * p.c_st + head * p.c_sh + q * 16;
+  const int64_t pa = b * p.pa_sb + page * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
+  const uint4 kw = *reinterpret_cast<const uint4*>(p.k + at), vw = *reinterpret_cast<const uint4*>(p.v + at);
+  const uint4 kp = *reinterpret_cast<const uint4*>(p.k_param + pa), vp = *reinterpret_cast<const uint4*>(p.v_param + pa);
+  const uint32_t k_codes[4] = {kw.x, kw.y, kw.z, kw.w};
+  const uint32_t v_codes[4] = {__byte_perm(vw.x, vw.z, 0x5410), __byte_perm(vw.x, vw.z, 0x7632), __byte_perm(vw.y, vw.w, 0x5410),
+                               __byte_perm(vw.y, vw.w, 0x7632)};
+  const __half* ks = reinterpret_cast<const __half*>(&kp);
+  const __half* vs = reinterpret_cast<const __half*>(&vp);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    ko[4 * g] = from_codes<BF16>(k_codes[g], __half2float(ks[g]), __half2float(ks[4 + g]));
+    vo[4 * g] = from_codes<BF16>(v_codes[g], __half2float(vs[g]), __half2float(vs[4 + g]));
+  }
 }
 
 }  // namespace kb200
@@ -731,7 +733,7 @@ extern "C" int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens,
   KvReadParams p{};
   p.rows = (int64_t)batch * max_len * num_kv_heads;
   if (p.rows == 0) return 0;
-  KB_REQUIRE((p.rows + 31) / 32 < (1ll << 31), "kv_read: too many rows for one launch");
+  KB_REQUIRE((p.rows + 63) / 64 < (1ll << 31), "kv_read: too many rows for one launch");
   p.k = static_cast<const uint8_t*>(kv->k);
   p.v = static_cast<const uint8_t*>(kv->v);
   p.c_sb = kv->stride_batch; p.c_sp = kv->stride_page; p.c_st = kv->stride_token; p.c_sh = kv->stride_head;
@@ -749,7 +751,7 @@ extern "C" int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens,
   p.v_out = static_cast<__half*>(v_out);
   p.T = max_len;
   p.G = num_kv_heads;
-  const unsigned blocks = (unsigned)((p.rows + 31) / 32);
+  const unsigned blocks = (unsigned)((p.rows + 63) / 64);
   if (kv->act_dtype == KB200_BF16) kv_read_kernel<true><<<blocks, 256, 0, (cudaStream_t)stream>>>(p);
   else kv_read_kernel<false><<<blocks, 256, 0, (cudaStream_t)stream>>>(p);
   KB_CHECK_LAUNCH("kv_read_kernel");
