@@ -218,9 +218,6 @@ static void launch_kv_write(const KvWriteParams& p, int64_t blocks, cudaStream_t
 }
 
 // ---- appends that quantise to 4 bits, or whose tokens have positions of their own ---------------------
-// Eight lanes share a row; lane c has its values 8c .. 8c+7 (four pairs x[0..3], group c / 4) and 64+8c .. 64+8c+7 (x[4..7],
-// group 2 + c / 4), so a group of 32 lies in four lanes.
-
 // pairs of fp32 numbers, for the two-element instructions: these kernels are bound by issue slots
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
@@ -329,9 +326,10 @@ constexpr int kSame = 0, kFp8 = 1, kInt4 = 2;
 constexpr int kAppendThreads = 256;
 constexpr int kAppendTokens = 4;                                               // tokens of a CTA at most
 
-// Eight lanes take an item: the K and the V row of a (token, KV head), whose places in the cache are the same, or two Q rows of a
-// token.  A CTA takes p.tokens tokens and has, as a rule, eight lanes for each of their items: all rows are loaded at once,
-// before the angles are computed.  AT: positions of their own.
+// Four lanes take an item: the K and the V row of a (token, KV head), whose places in the cache are the same, or two Q rows of a
+// token.  Lane q has the values 8q .. 8q+7 of each of a row's four groups of 32: the two that a rotation pairs up are in groups g and
+// g + 2, and what it stores of a 4-bit row is one piece of 16 bytes.  A CTA takes p.tokens tokens; its first items are loaded before
+// the angles are computed.  AT: positions of their own.
 template <bool BF16, int STORE, bool AT>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWriteParams p) {
   using H2 = typename Pair<BF16>::T;
@@ -340,11 +338,11 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
   __shared__ __align__(16) Angle sin_s[kAppendTokens][kD / 2];
   __shared__ int64_t page_s[kAppendTokens];
   __shared__ int slot_s[kAppendTokens];
-  const int tid = threadIdx.x, c = tid & 7;
+  const int tid = threadIdx.x, q = tid & 3;
   const int per = p.G + (p.H + 1) / 2, items = p.tokens * per;       // items of a token: KV heads first, then pairs of Q heads
   const uint32_t first = blockIdx.x * (uint32_t)p.tokens, all = (uint32_t)p.B * p.T;
-  for (int item0 = 0; item0 < items; item0 += blockDim.x >> 3) {     // uniform for the CTA
-    const int item = item0 + (tid >> 3);
+  for (int item0 = 0; item0 < items; item0 += blockDim.x >> 2) {     // uniform for the CTA
+    const int item = item0 + (tid >> 2);
     const int i = (item >= per) + (item >= 2 * per) + (item >= 3 * per), h = item - i * per;
     static_assert(kAppendTokens == 4, "three comparisons");
     const uint32_t token = first + i;
@@ -353,16 +351,15 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
     const bool kv = h < p.G;
     const int head = kv ? h : 2 * (h - p.G);
     const bool two = kv || head + 1 < p.H;
-    uint4 row[2][2];                                                    // (all lanes take part in the shuffles)
+    uint4 row[2][4];                                                    // (all lanes take part in the shuffles)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      row[r][0] = row[r][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (!active || (r && !two)) continue;
       const __half* src = !kv ? p.q_in + b * p.q_sb + t * p.q_st + (head + r) * p.q_sh
                               : r == 0 ? p.k_new + b * p.k_sb + t * p.k_st + head * p.k_sh
                                        : p.v_new + b * p.v_sb + t * p.v_st + head * p.v_sh;
-      row[r][0] = reinterpret_cast<const uint4*>(src)[c];
-      row[r][1] = reinterpret_cast<const uint4*>(src + kD / 2)[c];
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        row[r][g] = active && (r == 0 || two) ? reinterpret_cast<const uint4*>(src)[4 * g + q] : make_uint4(0u, 0u, 0u, 0u);
     }
     if (item0 == 0) {
       // the tokens' places in the cache, and their angles
@@ -398,136 +395,142 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
     }
     const int64_t phys = active ? page_s[i] : 0, slot = active ? slot_s[i] : 0;
     const int64_t place = b * p.c_sb + phys * p.c_sp + slot * p.c_st + head * p.c_sh;
-    const int64_t params = b * p.pa_sb + phys * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const bool turn = p.inv_freq && (!kv || r == 0);
       const __half* gain = !kv ? p.q_gain : r == 0 ? p.k_gain : nullptr;
-      H2* lo = reinterpret_cast<H2*>(&row[r][0]);
-      H2* hi = reinterpret_cast<H2*>(&row[r][1]);
-      uint64_t x[8];                                                    // the row in fp32: pairs 0-3 from lo, 4-7 from hi
-      float ends[4];                                                    // the ends of its groups over the lane
+      const bool plain = AT && STORE != kInt4 && kv && r == 1;            // a V row that is stored as it is
+      uint64_t x[16];                                                     // the row in fp32, four pairs per group
       auto widen = [&] {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 a = to_f2(lo[e]), d2 = to_f2(hi[e]);
-          x[e] = pack2(a.x, a.y);
-          x[4 + e] = pack2(d2.x, d2.y);
+        for (int g = 0; g < 4; ++g) {
+          const H2* v = reinterpret_cast<const H2*>(&row[r][g]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = to_f2(v[e]);
+            x[4 * g + e] = pack2(f.x, f.y);
+          }
         }
       };
-      const bool plain = AT && STORE != kInt4 && kv && r == 1;            // a V row that is stored as it is
       float inv_rms = 1.f;
       if (AT && !plain) widen();
-      if (r == 0 ? p.q_gain || p.k_gain : p.q_gain != nullptr) {         // (uniform: the warp's rows are of either kind)
+      if (r == 0 ? p.q_gain || p.k_gain : p.q_gain != nullptr) {           // (uniform: the warp's rows are of either kind)
         uint64_t sq = 0;
         if constexpr (!AT) widen();
         if (!plain) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sq = fma2(x[e], x[e], sq);
+          for (int e = 0; e < 16; ++e) sq = fma2(x[e], x[e], sq);
         }
         float ss = unpack2(sq).x + unpack2(sq).y;
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+        ss += __shfl_xor_sync(0xFFFFFFFFu, ss, 1);
+        ss += __shfl_xor_sync(0xFFFFFFFFu, ss, 2);
         inv_rms = rsqrtf(ss / kD + p.eps);
       }
       if constexpr (AT) {
         if (!plain) {
           if (gain) {
-            const uint4 g_lo4 = reinterpret_cast<const uint4*>(gain)[c];
-            const uint4 g_hi4 = reinterpret_cast<const uint4*>(gain + kD / 2)[c];
-            const H2* g_lo = reinterpret_cast<const H2*>(&g_lo4);
-            const H2* g_hi = reinterpret_cast<const H2*>(&g_hi4);
             const uint64_t rms2 = pack2(inv_rms, inv_rms);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 a = to_f2(g_lo[e]), d2 = to_f2(g_hi[e]);
-              x[e] = mul2(x[e], mul2(pack2(a.x, a.y), rms2));
-              x[4 + e] = mul2(x[4 + e], mul2(pack2(d2.x, d2.y), rms2));
+            for (int g = 0; g < 4; ++g) {
+              const uint4 g4 = reinterpret_cast<const uint4*>(gain)[4 * g + q];
+              const H2* gv = reinterpret_cast<const H2*>(&g4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = to_f2(gv[e]);
+                x[4 * g + e] = mul2(x[4 * g + e], mul2(pack2(f.x, f.y), rms2));
+              }
             }
           }
           if (turn) {
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(&cos_s[i][c * 8 + 2 * e]);
-              const ulonglong2 sn = *reinterpret_cast<const ulonglong2*>(&sin_s[i][c * 8 + 2 * e]);
+            for (int g = 0; g < 2; ++g) {
 #pragma unroll
-              for (int f = 0; f < 2; ++f) {
-                const uint64_t l = x[e + f], h2 = x[4 + e + f], cv = f ? cs.y : cs.x, sv = f ? sn.y : sn.x;
-                x[e + f] = sub2(mul2(l, cv), mul2(h2, sv));
-                x[4 + e + f] = fma2(l, sv, mul2(h2, cv));
+              for (int e = 0; e < 4; e += 2) {
+                const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(&cos_s[i][32 * g + 8 * q + 2 * e]);
+                const ulonglong2 sn = *reinterpret_cast<const ulonglong2*>(&sin_s[i][32 * g + 8 * q + 2 * e]);
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                  const uint64_t l = x[4 * g + e + f], h2 = x[8 + 4 * g + e + f], cv = f ? cs.y : cs.x, sv = f ? sn.y : sn.x;
+                  x[4 * g + e + f] = sub2(mul2(l, cv), mul2(h2, sv));
+                  x[8 + 4 * g + e + f] = fma2(l, sv, mul2(h2, cv));
+                }
               }
             }
           }
           if (STORE != kInt4 || !kv) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 a = unpack2(x[e]), d2 = unpack2(x[4 + e]);
-              lo[e] = from_f2<BF16>(a.x, a.y);
-              hi[e] = from_f2<BF16>(d2.x, d2.y);
+            for (int g = 0; g < 4; ++g) {
+              H2* v = reinterpret_cast<H2*>(&row[r][g]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2(x[4 * g + e]);
+                v[e] = from_f2<BF16>(f.x, f.y);
+              }
             }
           }
         }
-        if constexpr (STORE == kInt4) {
-          group_ends(x, ends[0], ends[1]);
-          group_ends(x + 4, ends[2], ends[3]);
-        }
       } else {
-        if (gain) module_norm<BF16>(lo, hi, gain, inv_rms, c);
-        if (turn) module_rotate<BF16>(lo, hi, cos_s[i], sin_s[i], c);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          H2* lo = reinterpret_cast<H2*>(&row[r][g]);
+          H2* hi = reinterpret_cast<H2*>(&row[r][g + 2]);
+          if (gain) module_norm<BF16>(lo, hi, gain, inv_rms, 4 * g + q);
+          if (turn) module_rotate<BF16>(lo, hi, cos_s[i], sin_s[i], 4 * g + q);
+        }
         widen();
-        group_ends<BF16>(row[r][0], ends[0], ends[1]);
-        group_ends<BF16>(row[r][1], ends[2], ends[3]);
       }
-      uint32_t words[2];
-      __half scale[2], zero[2];
+      uint32_t words[4];
+      __half scale[4], zero[4];
       if constexpr (STORE == kInt4) {
-        words[0] = quantize_int4(x, ends[0], ends[1], scale[0], zero[0]);
-        words[1] = quantize_int4(x + 4, ends[2], ends[3], scale[1], zero[1]);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float mn, mx;
+          if constexpr (AT) group_ends(x + 4 * g, mn, mx);
+          else group_ends<BF16>(row[r][g], mn, mx);
+          words[g] = quantize_int4(x + 4 * g, mn, mx, scale[g], zero[g]);
+        }
       }
       if (!active || (r && !two)) continue;
-      if (!kv) {
-        __half* dst = p.q_out + (((int64_t)b * p.T + t) * p.H + head + r) * kD;
-        reinterpret_cast<uint4*>(dst)[c] = row[r][0];
-        reinterpret_cast<uint4*>(dst + kD / 2)[c] = row[r][1];
-        continue;
-      }
       __half* cache = r == 0 ? p.k_cache : p.v_cache;
-      if constexpr (STORE == kInt4) {
-        const int g = c >> 2, q = c & 3;                                 // groups g and g + 2, values 8q .. 8q+7 of either
-        uint8_t* dst = reinterpret_cast<uint8_t*>(cache) + place;
-        __half* pr = (r == 0 ? p.k_param : p.v_param) + params;
+      if (STORE == kSame || !kv) {
+        uint4* dst = reinterpret_cast<uint4*>(kv ? cache + place : p.q_out + (((int64_t)b * p.T + t) * p.H + head + r) * kD);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          if (r == 0) {
-            *reinterpret_cast<uint32_t*>(dst + q * 16 + (g + 2 * f) * 4) = words[f];
-          } else {
-            *reinterpret_cast<uint16_t*>(dst + (2 * q) * 8 + (g + 2 * f) * 2) = (uint16_t)words[f];
-            *reinterpret_cast<uint16_t*>(dst + (2 * q + 1) * 8 + (g + 2 * f) * 2) = (uint16_t)(words[f] >> 16);
-          }
-          if (q == 0) { pr[g + 2 * f] = scale[f]; pr[4 + g + 2 * f] = zero[f]; }
+        for (int g = 0; g < 4; ++g) dst[4 * g + q] = row[r][g];
+      } else if constexpr (STORE == kInt4) {
+        uint4 piece;                                                       // groups 0-3 of K; of V, whose pieces hold four values per
+        if (r == 0) {                                                      // group, the low halves of the words, then the high ones
+          piece = make_uint4(words[0], words[1], words[2], words[3]);
+        } else {
+          piece = make_uint4(__byte_perm(words[0], words[1], 0x5410), __byte_perm(words[2], words[3], 0x5410),
+                             __byte_perm(words[0], words[1], 0x7632), __byte_perm(words[2], words[3], 0x7632));
         }
-      } else if constexpr (STORE == kFp8) {
-        const float sc = (r == 0 ? p.k_scale : p.v_scale)[b * p.s_sb + phys * p.s_sp + head * p.s_sh];
-        uint8_t* d8 = reinterpret_cast<uint8_t*>(cache) + place;
-        reinterpret_cast<uint2*>(d8)[c] = quantize8(lo, sc);              // bytes 8c .. 8c+7
-        reinterpret_cast<uint2*>(d8 + kD / 2)[c] = quantize8(hi, sc);     // bytes 64+8c .. 64+8c+7
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(cache) + place + q * 16) = piece;
+        if (q == 0) {
+          __align__(16) const __half par[8] = {scale[0], scale[1], scale[2], scale[3], zero[0], zero[1], zero[2], zero[3]};
+          __half* dst = (r == 0 ? p.k_param : p.v_param) + b * p.pa_sb + phys * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(par);
+        }
       } else {
-        reinterpret_cast<uint4*>(cache + place)[c] = row[r][0];
-        reinterpret_cast<uint4*>(cache + place + kD / 2)[c] = row[r][1];
+        const float sc = (r == 0 ? p.k_scale : p.v_scale)[b * p.s_sb + phys * p.s_sp + head * p.s_sh];
+        uint2* dst = reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(cache) + place);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) dst[4 * g + q] = quantize8(reinterpret_cast<const H2*>(&row[r][g]), sc);
       }
     }
   }
 }
 
-// Two warps per CTA where there are many tokens: then a CTA makes several passes, and while one waits for its rows or computes its
-// angles the others on the SM work.  Few tokens: all items of a token at once.  us with CTAs for all items / of two warps: 16384 tokens
-// of 32 + 8 heads with norm 95 / 79, without 81 / 67; 64 tokens 5.7 / 8.1.
+// One warp per CTA where there are many tokens: then a CTA makes several passes, and while one waits for its rows or computes its angles
+// the others on the SM work.  Few tokens: all items of a token at once.  What bounds it is issue slots, the integer pipe above all:
+// us (and TB/s) for 32768 tokens of 8 KV heads to 4 bits 53 (3.3; with rotary 63), 16384 tokens of 32 + 8 heads with positions on three
+// axes 72 (5.6; with norm 77).  With two / three warps per CTA those two take 76 / 83 and 85 / 91, and with all items at once 81 and 95; 64
+// tokens of 32 + 8 heads 5.7 with all items at once, 8.1 with two warps.
 template <bool BF16, int STORE, bool AT>
 static void launch_kv_append(KvWriteParams p, int64_t tokens, cudaStream_t st) {
   const int per = p.G + (p.H + 1) / 2;
   p.tokens = 1;
   while (p.tokens < kAppendTokens && p.tokens * 2 * per <= 16 && tokens >= (int64_t)p.tokens * 2 * 8 * sm_count()) p.tokens *= 2;
-  const int threads = (p.tokens * per * 8 + 31) / 32 * 32, most = tokens > 8ll * sm_count() ? 64 : kAppendThreads;
+  const int threads = (p.tokens * per * 4 + 31) / 32 * 32, most = tokens > 8ll * sm_count() ? 32 : kAppendThreads;
   kv_append_kernel<BF16, STORE, AT><<<(unsigned)((tokens + p.tokens - 1) / p.tokens), threads < most ? threads : most, 0, st>>>(p);
 }
 template <bool BF16>
