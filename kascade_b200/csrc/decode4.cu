@@ -15,6 +15,9 @@
 //   * O^T = V^T P^T, values as rows:  sum_k (p_k s_gk) c_dk  with the scale on the probabilities, which are one row per head,
 //     not on the 128 values, and sum_k p_k z_gk as one product with the transposed parameters.
 // The orders of the codes in K and V rows are those in which a lane needs them: 16 bytes of a K row, 8 of a V row.
+// What bounds it: dense passes and rows in order, HBM (5.5-5.6 TB/s at 37 x 16384 and 64 x 32768 keys; 128 us of 144 for the former with the
+// cache in L2, with 57 % of the issue slots and 52 % of the integer pipe busy); reuse layers, lines: DRAM hands out 128 bytes at a
+// time, so random rows of 64 + 64 + 32 bytes move 304 bytes per key (64 x 3244 rows: 92 us, 5.4 TB/s of DRAM traffic).
 // Queries are brought to a largest element of 64..128 per head by a power of two, so that bf16 ones fit fp16 exactly.
 #include "decode.cuh"
 
