@@ -436,11 +436,14 @@ int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens, void* k_ou
  * head, because anchor layers hand their index rows to the reuse layers of other heads: a row has to mean the same token
  * in every layer and head.  The reference has no eviction. */
 
-/* Weight of a decode step (pooled [B, G, row_stride] of kb200_decode_anchor_paged), for the rows j < seq_lens[b] and j < max_len:
- *   mass_out[b, j] = mass_in[b, j] + sum_g pooled[b, g, j]        (added up in the order of g)
- * mass_out may be mass_in (rows mass_stride apart, both of them). */
-int kb200_mass_add(const float* pooled, int64_t row_stride, const int32_t* seq_lens, const float* mass_in, float* mass_out,
-                   int64_t mass_stride, int batch, int num_kv_heads, int max_len, void* stream);
+/* kb200_decode_anchor_paged that adds the step's weight to the rows', for j < seq_lens[b]:
+ *   mass[b, j] += sum_g pooled[b, g, j]        (added up in the order of g)
+ *   mass   [B, >= max_seq_len] fp32, rows mass_stride apart */
+int kb200_decode_anchor_paged_mass(const void* q, int64_t q_stride_b, int64_t q_stride_h, const kb200_kv_layout* kv,
+                                   const int32_t* seq_lens, int max_seq_len, float softmax_scale, float* logits, float* pooled,
+                                   int64_t logit_stride, float* mass, int64_t mass_stride, void* out, float* lse2_out,
+                                   void* workspace, size_t workspace_bytes, int batch, int num_q_heads, int num_kv_heads,
+                                   int num_splits, void* stream);
 
 /* Weight of a prompt (pooled [B, G, num_tiles, row_stride] of kb200_prefill_pool_scores[_ragged]):
  *   mass_out[b, j] = mass_in[b, j] + sum_g sum_{t : 32 t > j} pooled[b, g, t, j]     for 0 <= j < n_rows

@@ -30,7 +30,7 @@ EXPORTS = [
     "kb200_decode_sparse_paged_noalloc", "kb200_prefill_dense_fanout", "kb200_prefill_sparse_fanout",
     "kb200_kv_write", "kb200_prefill_dense_ragged", "kb200_prefill_pool_scores_ragged", "kb200_prefill_sparse_ragged",
     "kb200_prefill_budgets_ragged", "kb200_zero_padding", "kb200_peer_push", "kb200_stream_wait_events", "kb200_selftest_wait_timeout", "kb200_tensor_map_encodes", "kb200_decode_noalloc_splits",
-    "kb200_kv_write_at", "kb200_kv_read", "kb200_mass_add", "kb200_mass_add_prompt", "kb200_evict",
+    "kb200_kv_write_at", "kb200_kv_read", "kb200_decode_anchor_paged_mass", "kb200_mass_add_prompt", "kb200_evict",
     "kb200_evict_workspace_bytes",
 ]
 
@@ -163,7 +163,8 @@ def load() -> C.CDLL:
         lib.kb200_kv_write_at.argtypes = [AL, vp, AL, AL, vp, vp, C.POINTER(KvLayout), vp, vp, f32, vp, f32,
                                           C.POINTER(Positions), i32, i32, i32, i32, vp]
         lib.kb200_kv_read.argtypes = [C.POINTER(KvLayout), vp, vp, vp, i32, i32, i32, vp]
-        lib.kb200_mass_add.argtypes = [vp, i64, vp, vp, vp, i64, i32, i32, i32, vp]
+        lib.kb200_decode_anchor_paged_mass.argtypes = [vp, i64, i64, C.POINTER(KvLayout), vp, i32, f32, vp, vp, i64, vp, i64, vp, vp,
+                                                       vp, C.c_size_t, i32, i32, i32, i32, vp]
         lib.kb200_mass_add_prompt.argtypes = [vp, i64, vp, vp, vp, i64, i64, i32, i32, i32, i32, vp]
         lib.kb200_evict_workspace_bytes.restype = C.c_size_t
         lib.kb200_evict_workspace_bytes.argtypes = [i32, i32, i32]
@@ -549,8 +550,9 @@ def decode_sparse_paged_noalloc(q, kv: KvLayout, topk_idx, topk_count, k_max, he
 
 @_on_device_of(0)
 def decode_anchor_paged(q, kv: KvLayout, seq_lens, max_seq_len, scale, logits, pooled, out, lse2,
-                        workspace=None, num_splits=0):
-    """q [B,H,D]; logits [B,H,stride] fp32; pooled [B,G,stride] fp32; out [B,H,D] fp16 or None."""
+                        workspace=None, num_splits=0, mass=None):
+    """q [B,H,D]; logits [B,H,stride] fp32; pooled [B,G,stride] fp32; out [B,H,D] fp16 or None.  `mass` [B, at least max_seq_len] fp32:
+    the sum of pooled over the heads is added to it."""
     lib = init(q.get_device())
     _check_q(q, kv)
     _want_opt(out, q.dtype, "out")
@@ -560,11 +562,17 @@ def decode_anchor_paged(q, kv: KvLayout, seq_lens, max_seq_len, scale, logits, p
     G, stride = pooled.shape[1:]
     qs = q.stride()
     assert logits.is_contiguous() and pooled.is_contiguous() and logits.shape[-1] == stride
-    _check(lib.kb200_decode_anchor_paged(
-        q.data_ptr(), qs[0], qs[1], C.byref(kv), seq_lens.data_ptr(), max_seq_len, float(scale), logits.data_ptr(),
-        pooled.data_ptr(), stride, _ptr(out), _ptr(lse2), _ptr(workspace),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), B, H, G, num_splits, _stream()),
-        "kb200_decode_anchor_paged")
+    before = (q.data_ptr(), qs[0], qs[1], C.byref(kv), seq_lens.data_ptr(), max_seq_len, float(scale), logits.data_ptr(),
+              pooled.data_ptr(), stride)
+    after = (_ptr(out), _ptr(lse2), _ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), B, H, G,
+             num_splits, _stream())
+    if mass is None:
+        _check(lib.kb200_decode_anchor_paged(*before, *after), "kb200_decode_anchor_paged")
+    else:
+        _want_rows(mass, torch.float32, B, "mass")
+        if mass.shape[1] < max_seq_len or mass.get_device() != q.get_device():
+            raise KascadeNativeError(f"mass holds {mass.shape[1]} rows on {mass.device}, {max_seq_len} on {q.device} are needed")
+        _check(lib.kb200_decode_anchor_paged_mass(*before, mass.data_ptr(), mass.stride(0), *after), "kb200_decode_anchor_paged_mass")
     ns = num_splits if num_splits else lib.kb200_decode_default_splits(B, G, max_seq_len)
     _launched(2 + (ns > 1))
 
@@ -756,25 +764,6 @@ def _want_rows(t: torch.Tensor, dtype, batch: int, name: str):
     if t.dim() != 2 or t.shape[0] != batch or (t.shape[1] > 1 and t.stride(1) != 1):
         raise KascadeNativeError(f"{name}: expected [{batch}, rows], the last dimension contiguous, got {tuple(t.shape)} with strides "
                                  f"{t.stride()}")
-
-
-@_on_device_of(0)
-def mass_add(pooled, seq_lens, mass, out, max_len: int):
-    """out[b, j] = mass[b, j] + sum over the heads of pooled [B, G, row_stride], for j < seq_lens[b]; `out` may be `mass`."""
-    lib = init(pooled.get_device())
-    _want(pooled, torch.float32, "pooled")
-    _want(seq_lens, torch.int32, "seq_lens")
-    B, G, stride = pooled.shape
-    _want_rows(mass, torch.float32, B, "mass")
-    _want_rows(out, torch.float32, B, "out")
-    if not pooled.is_contiguous() or not seq_lens.is_contiguous() or seq_lens.shape != (B,) or (B > 1 and out.stride(0) != mass.stride(0)):
-        raise KascadeNativeError("mass_add: pooled and seq_lens must be contiguous, mass and out equally strided")
-    if mass.shape[1] < max_len or out.shape[1] < max_len:
-        raise KascadeNativeError(f"mass_add: mass holds {mass.shape[1]} rows, {max_len} are needed")
-    _same_device(pooled, seq_lens=seq_lens, mass=mass, out=out)
-    _check(lib.kb200_mass_add(_ptr(pooled), stride, _ptr(seq_lens), _ptr(mass), _ptr(out),
-                              mass.stride(0) if B > 1 else mass.shape[1], B, G, max_len, _stream()), "kb200_mass_add")
-    _launched(1 if B and max_len else 0)
 
 
 @_on_device_of(0)

@@ -447,6 +447,57 @@ __global__ void __launch_bounds__(256) decode_pool_kernel(const float* logits, c
   }
 }
 
+// The same, with the sum over the KV heads added to the weight that the rows have collected: mass[b,j] += sum_g pooled[b,g,j], in
+// the order of g.  grid (ceil(maxlen/128), B), the heads one after the other (so no sum depends on which CTA comes first), the
+// logits of the next head in flight meanwhile.  Next to the pooling kernel alone it takes 2-3 us more, at 8 KV heads and from one
+// sequence of 2048 keys to 64 of 4096; as a kernel of its own after it the addition took 6-8 us of an anchor layer.  Bound by
+// latency, so one warp per CTA: with 2, 4 and 8 warps it took 0.7-0.9 us more for one sequence of 2048 to 131072 keys.
+constexpr int kPoolMassThreads = 32;
+__global__ void __launch_bounds__(kPoolMassThreads) decode_pool_mass_kernel(const float* logits, const float* lse2,
+                                                                            const int32_t* seq_lens, float* __restrict__ pooled,
+                                                                            int64_t stride, float* mass, int64_t mass_stride, int H,
+                                                                            int G, int max_len) {
+  pdl_wait();
+  const int b = blockIdx.y;
+  const int n = min(seq_lens[b], max_len);
+  const int j = (blockIdx.x * kPoolMassThreads + threadIdx.x) * 4;
+  if (j >= n) return;
+  const float* src = logits + (int64_t)b * H * stride + j;
+  float m[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m[e] = j + e < n ? mass[b * mass_stride + j + e] : 0.f;
+  float4 x[kHg];
+#pragma unroll
+  for (int h = 0; h < kHg; ++h) x[h] = *reinterpret_cast<const float4*>(src + h * stride);   // padding beyond n is readable scratch
+  for (int g = 0; g < G; ++g) {
+    float4 next[kHg];
+#pragma unroll
+    for (int h = 0; h < kHg; ++h)
+      next[h] = g + 1 < G ? *reinterpret_cast<const float4*>(src + ((g + 1) * kHg + h) * stride) : x[h];
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < kHg; ++h) {
+      const float l = lse2[(int64_t)b * H + g * kHg + h];
+      a[0] += exp2f(x[h].x - l);
+      a[1] += exp2f(x[h].y - l);
+      a[2] += exp2f(x[h].z - l);
+      a[3] += exp2f(x[h].w - l);
+      x[h] = next[h];
+    }
+    float* dst = pooled + ((int64_t)b * G + g) * stride + j;
+    if (j + 3 < n) {
+      *reinterpret_cast<float4*>(dst) = make_float4(a[0], a[1], a[2], a[3]);
+    } else {
+      for (int e = 0; e < 4 && j + e < n; ++e) dst[e] = a[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += a[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j + e < n) mass[b * mass_stride + j + e] = m[e] + sum[e];
+}
+
 int init_decode() {
   KB_CUDA(cudaFuncSetAttribute(decode_attn_kernel<false, true, false, 0>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem));
@@ -677,13 +728,10 @@ extern "C" int kb200_decode_sparse_paged(const void* q, int64_t q_stride_b, int6
   return 0;
 }
 
-extern "C" int kb200_decode_anchor_paged(const void* q, int64_t q_stride_b, int64_t q_stride_h,
-                                         const kb200_kv_layout* kv, const int32_t* seq_lens,
-                                         int max_seq_len, float softmax_scale, float* logits,
-                                         float* pooled, int64_t logit_stride, void* out,
-                                         float* lse2_out, void* workspace, size_t workspace_bytes,
-                                         int batch, int num_q_heads, int num_kv_heads,
-                                         int num_splits, void* stream) {
+static int anchor_paged(const void* q, int64_t q_stride_b, int64_t q_stride_h, const kb200_kv_layout* kv, const int32_t* seq_lens,
+                        int max_seq_len, float softmax_scale, float* logits, float* pooled, int64_t logit_stride, float* mass,
+                        int64_t mass_stride, void* out, float* lse2_out, void* workspace, size_t workspace_bytes, int batch,
+                        int num_q_heads, int num_kv_heads, int num_splits, void* stream) {
   using namespace kb200;
   KB_ENTRY(q, "decode_anchor: q");
   KB_REQUIRE(q && seq_lens && logits && pooled && lse2_out, "decode_anchor: null pointer");
@@ -730,12 +778,39 @@ extern "C" int kb200_decode_anchor_paged(const void* q, int64_t q_stride_b, int6
   else rc = launch_attn<true, false, true, 0>(p, grid, max_seq_len, st);
   KB_LAUNCH("decode_attn_kernel<dense>", rc);
   if (splits > 1) KB_LAUNCH("decode_combine_kernel", launch_combine(p, has_v, batch, st));
-  if (max_seq_len > 0) {
+  if (max_seq_len > 0 && mass) {
+    KB_LAUNCH("decode_pool_mass_kernel",
+              launch_pdl(decode_pool_mass_kernel, dim3(ceil_div(max_seq_len, 4 * kPoolMassThreads), batch), kPoolMassThreads, 0, st, 1,
+                         logits, lse2_out, seq_lens, pooled, logit_stride, mass, mass_stride, num_q_heads, num_kv_heads, max_seq_len));
+  } else if (max_seq_len > 0) {
     dim3 pgrid(ceil_div(max_seq_len, 1024), num_kv_heads, batch);
     KB_LAUNCH("decode_pool_kernel", launch_pdl(decode_pool_kernel, pgrid, 256, 0, st, 1, logits, lse2_out, seq_lens, pooled,
                                                logit_stride, num_q_heads, num_kv_heads));
   }
   return 0;
+}
+
+extern "C" int kb200_decode_anchor_paged(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                                         const kb200_kv_layout* kv, const int32_t* seq_lens,
+                                         int max_seq_len, float softmax_scale, float* logits,
+                                         float* pooled, int64_t logit_stride, void* out,
+                                         float* lse2_out, void* workspace, size_t workspace_bytes,
+                                         int batch, int num_q_heads, int num_kv_heads,
+                                         int num_splits, void* stream) {
+  return anchor_paged(q, q_stride_b, q_stride_h, kv, seq_lens, max_seq_len, softmax_scale, logits, pooled, logit_stride, nullptr, 0,
+                      out, lse2_out, workspace, workspace_bytes, batch, num_q_heads, num_kv_heads, num_splits, stream);
+}
+
+extern "C" int kb200_decode_anchor_paged_mass(const void* q, int64_t q_stride_b, int64_t q_stride_h, const kb200_kv_layout* kv,
+                                              const int32_t* seq_lens, int max_seq_len, float softmax_scale, float* logits,
+                                              float* pooled, int64_t logit_stride, float* mass, int64_t mass_stride, void* out,
+                                              float* lse2_out, void* workspace, size_t workspace_bytes, int batch,
+                                              int num_q_heads, int num_kv_heads, int num_splits, void* stream) {
+  KB_REQUIRE(mass, "decode_anchor: null mass");
+  KB_REQUIRE(batch <= 1 || mass_stride >= max_seq_len, "decode_anchor: mass holds %lld rows, %d are needed", (long long)mass_stride,
+             max_seq_len);
+  return anchor_paged(q, q_stride_b, q_stride_h, kv, seq_lens, max_seq_len, softmax_scale, logits, pooled, logit_stride, mass,
+                      mass_stride, out, lse2_out, workspace, workspace_bytes, batch, num_q_heads, num_kv_heads, num_splits, stream);
 }
 
 // Same computation as kb200_decode_sparse_paged, for callers that must not allocate device memory and

@@ -15,9 +15,10 @@
 //   * O^T = V^T P^T, values as rows:  sum_k (p_k s_gk) c_dk  with the scale on the probabilities, which are one row per head,
 //     not on the 128 values, and sum_k p_k z_gk as one product with the transposed parameters.
 // The orders of the codes in K and V rows are those in which a lane needs them: 16 bytes of a K row, 8 of a V row.
-// What bounds it: dense passes and rows in order, HBM (5.5-5.6 TB/s at 37 x 16384 and 64 x 32768 keys; 128 us of 144 for the former with the
-// cache in L2, with 57 % of the issue slots and 52 % of the integer pipe busy); reuse layers, lines: DRAM hands out 128 bytes at a
-// time, so random rows of 64 + 64 + 32 bytes move 304 bytes per key (64 x 3244 rows: 92 us, 5.4 TB/s of DRAM traffic).
+// What bounds it: dense passes and rows in order, HBM (5.5-5.6 TB/s at 37 x 16384 and 64 x 32768 keys; 128 us of 144 for the
+// former with the cache in L2, with 57 % of the issue slots and 52 % of the integer pipe busy); reuse layers, lines: DRAM hands
+// out 128 bytes at a time, so random rows of 64 + 64 + 32 bytes move 304 bytes per key (64 x 3244 rows: 92 us, 5.4 TB/s of DRAM
+// traffic).
 // Queries are brought to a largest element of 64..128 per head by a power of two, so that bf16 ones fit fp16 exactly.
 #include "decode.cuh"
 
@@ -35,10 +36,11 @@ constexpr float kSlack4 = 2.f;
 // The tensor core rounds its sums towards zero: by about 2^-24 of the accumulator per product, always the same way.  The codes' mean
 // is 7.5, so their share of O grows with the list while O itself, with the zeros' share taken off, does not: after 512 products that
 // was 0.4 % of O for 131072 keys.  (And it aligns products by their operands' exponent fields, so a subnormal loses what it lies below
-// 2^-14; V's codes are shifted two bits up for that.)  So every kFlush4 steps what the accumulators of a group have in common (one of them) is taken off
-// all of them and added up apart, rounded to nearest, in a few words per lane of shared memory.  Error of fp16 outputs against 64
-// bits, 131072 keys in 1 / 18 splits: 4.0e-3 / 5.3e-4 without, 6e-4 unshifted, 3.0e-4 / 2.8e-4 as it is (2.9e-4 is what the rounding
-// of probabilities and outputs to fp16 makes); every 8 steps 3.3e-4, every 16 4.6e-4.  It takes 1-2 % of a dense pass.
+// 2^-14; V's codes are shifted two bits up for that.)  So every kFlush4 steps what the accumulators of a group have in common (one
+// of them) is taken off all of them and added up apart, rounded to nearest, in a few words per lane of shared memory.  Error of
+// fp16 outputs against 64 bits, 131072 keys in 1 / 18 splits: 4.0e-3 / 5.3e-4 without, 6e-4 unshifted, 3.0e-4 / 2.8e-4 as it is
+// (2.9e-4 is what the rounding of probabilities and outputs to fp16 makes); every 8 steps 3.3e-4, every 16 4.6e-4.  It takes 1-2 %
+// of a dense pass.
 constexpr int kFlush4 = 4;
 constexpr int kTracks4 = 10;                               // per lane: four groups and the zeros, two heads each
 constexpr int kTrackBytes4 = kTracks4 * 32 * 4;            // per warp
@@ -68,7 +70,8 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c) {
-  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                            *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 

@@ -1,40 +1,11 @@
-// Eviction from a KV cache by accumulated attention weight: the weight that rows collect in prompts and decode steps, the
-// choice of the rows that stay, and the moves that bring them together.  The declarations in kascade_b200.h say what each
-// entry point computes; the reference has no counterpart.
+// Eviction from a KV cache by accumulated attention weight: the weight that rows collect in prompts (that of decode steps is
+// added up where it is pooled, in decode.cu), the choice of the rows that stay, and the moves that bring them together.  The
+// declarations in kascade_b200.h say what each entry point computes; the reference has no counterpart.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
 
 namespace kb200 {
-
-// ---- weight of a decode step ---------------------------------------------------------------------------------------
-// Four rows per thread, eight heads' loads in flight: bound by the pooled scores' way out of L2, where the pooling kernel has just put
-// them (16 sequences, 300075 rows of 8 heads: 6 us).
-__global__ void __launch_bounds__(128) mass_add_kernel(const float* pooled, int64_t row_stride, const int32_t* seq_lens,
-                                                       const float* mass_in, float* mass_out, int64_t mass_stride, int G,
-                                                       int max_len) {
-  pdl_begin();
-  const int b = blockIdx.y, n = min(seq_lens[b], max_len);
-  const int j = (blockIdx.x * 128 + threadIdx.x) * 4;
-  if (j >= n) return;
-  const float* src = pooled + (int64_t)b * G * row_stride + j;
-  float m[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) m[e] = j + e < n ? mass_in[b * mass_stride + j + e] : 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int g0 = 0; g0 < G; g0 += 8) {                               // eight loads in flight
-    float4 x[8];
-#pragma unroll
-    for (int g = 0; g < 8; ++g)                                      // (row_stride is a multiple of 4: readable)
-      x[g] = g0 + g < G ? *reinterpret_cast<const float4*>(src + (g0 + g) * row_stride) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int g = 0; g < 8; ++g) { a.x += x[g].x; a.y += x[g].y; a.z += x[g].z; a.w += x[g].w; }
-  }
-  const float s[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (j + e < n) mass_out[b * mass_stride + j + e] = m[e] + s[e];
-}
 
 // ---- weight of a prompt ----------------------------------------------------------------------------------------------
 struct PromptMassParams {
@@ -180,8 +151,8 @@ __device__ __forceinline__ int warp_lower_bound(const int32_t* a, int n, int x) 
 }
 
 // A CTA takes 256 rows.  The rank of a row among the kept ones comes from a bitmap of the kept rows among the 256 and the rank of
-// the first (with a binary search for every row 12.7 us for 4 x 32768 rows, so 6.5).  A row below the new length that is let go has i - rank others let go before it, and takes the (i - rank)-th of
-// the kept rows behind the new length.
+// the first (with a binary search for every row 12.7 us for 4 x 32768 rows, so 6.5).  A row below the new length that is let go has
+// i - rank others let go before it, and takes the (i - rank)-th of the kept rows behind the new length.
 __global__ void __launch_bounds__(256) evict_plan_kernel(const EvictPlanParams p) {
   pdl_begin();
   __shared__ uint32_t kept[8];
@@ -264,21 +235,6 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
 }
 
 }  // namespace kb200
-
-extern "C" int kb200_mass_add(const float* pooled, int64_t row_stride, const int32_t* seq_lens, const float* mass_in,
-                              float* mass_out, int64_t mass_stride, int batch, int num_kv_heads, int max_len, void* stream) {
-  using namespace kb200;
-  KB_ENTRY(pooled, "mass_add: pooled");
-  KB_REQUIRE(pooled && seq_lens && mass_in && mass_out, "mass_add: null pointer");
-  KB_REQUIRE(batch >= 0 && batch <= 65535 && num_kv_heads > 0 && max_len >= 0, "mass_add: bad sizes");
-  KB_REQUIRE(row_stride % 4 == 0 && row_stride >= max_len && (reinterpret_cast<uintptr_t>(pooled) & 15) == 0,
-             "mass_add: pooled rows must be 16-byte aligned (row_stride %% 4 == 0) and hold max_len (%d) scores", max_len);
-  KB_REQUIRE(batch <= 1 || mass_stride >= max_len, "mass_add: mass holds %lld rows, %d are needed", (long long)mass_stride, max_len);
-  if (batch == 0 || max_len == 0) return 0;
-  KB_LAUNCH("mass_add_kernel", launch_pdl(mass_add_kernel, dim3(ceil_div(max_len, 512), batch), 128, 0, (cudaStream_t)stream, 1,
-                                          pooled, row_stride, seq_lens, mass_in, mass_out, mass_stride, num_kv_heads, max_len));
-  return 0;
-}
 
 extern "C" int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t* seq_len, const float* mass_in,
                                      float* mass_out, int64_t mass_in_stride, int64_t mass_out_stride, int batch,
@@ -389,7 +345,8 @@ extern "C" int kb200_evict(const kb200_kv_layout* layers, int n_layers, const in
   KB_REQUIRE(n_layers >= 1 && batch >= 0 && batch <= 65535 && num_kv_heads > 0 && n_rows >= 0, "evict: bad sizes");
   KB_REQUIRE(budget >= 1 && budget <= (n_rows > 1 ? n_rows : 1) && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget,
              "evict: a budget of %d rows of %d, %d first and %d last ones protected", budget, n_rows, sinks, recent);
-  KB_REQUIRE(out_stride >= n_rows && mass_out != mass && pos_out != token_positions, "evict: outputs must hold %d rows and not be inputs", n_rows);
+  KB_REQUIRE(out_stride >= n_rows && mass_out != mass && pos_out != token_positions,
+             "evict: outputs must hold %d rows and not be inputs", n_rows);
   if (check_layers(layers, n_layers) != 0) return -1;
   if (batch == 0 || n_rows == 0) return 0;
   const EvictWorkspace at(batch, n_rows, budget);

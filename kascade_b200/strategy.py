@@ -584,9 +584,7 @@ class EfficientKascadeStrategy(Strategy):
             ws = self._scratch("dec_ws", (nat.decode_workspace_bytes(B, H, splits_a),), torch.uint8, dev)
             want_out = dense_only or layer == 0
             nat.decode_anchor_paged(q, kv, seq_lens, max_len, scaling, logits, pooled, out if want_out else None,
-                                    lse2, ws, splits_a)
-            if mass is not None and self.is_anchor(layer):
-                nat.mass_add(pooled, seq_lens, mass, mass, max_len)
+                                    lse2, ws, splits_a, mass=mass if self.is_anchor(layer) else None)
             if dense_only:
                 return out
             self._dec_kmax = kmax = self._decode_row_length(max_len)
@@ -709,8 +707,9 @@ class EfficientKascadeStrategy(Strategy):
         either type.  `attention_mass` [B, rows >= max_seq_len] fp32: anchor layers add to it, in place, the attention that each
         row draws, summed over the heads (reuse layers do not see all rows and leave it as it is); ``evict_kv`` chooses by it.
         `index_rows` = (rows [B,G,k] int32, counts [B,G] int32): a reuse layer attends to these rows (of the KV head its mapping
-        names) instead of the last anchor layer's, for a layer whose anchor runs elsewhere.  `mean_seq_len` is a hint of the host for batches of very different
-        lengths (the work is then cut into more, smaller pieces); results do not depend on it beyond summation order.
+        names) instead of the last anchor layer's, for a layer whose anchor runs elsewhere.  `mean_seq_len` is a hint of the
+        host for batches of very different lengths (the work is then cut into more, smaller pieces); results do not depend
+        on it beyond summation order.
         The reference has no paged kernel (README.md:135); the nearest signature is
         kernels/flash_decoding/reuse_kascade_gqa_decode_with_kvcache.py:160-171."""
         if max_seq_len is None:

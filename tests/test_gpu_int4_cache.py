@@ -216,11 +216,13 @@ def test_dense_decode(dtype, splits, has_v, lens):
     ws = nat.decode_workspace(B, H, splits, q.device)
     seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
     nat.decode_anchor_paged(q, kv, seq, longest, 128 ** -0.5, logits, pooled, out, lse, ws, splits)
-    if has_v:
-        _check_attention(out, lse, q, kf, vf, vc, lambda b, h: list(range(lens[b])), 128 ** -0.5, dtype, f"dense, {splits} splits")
+    first = pooled.clone()
     mass = torch.rand(B, stride + 3, device="cuda")
     added = mass.clone()
-    nat.mass_add(pooled, seq, mass, added, longest)
+    nat.decode_anchor_paged(q, kv, seq, longest, 128 ** -0.5, logits, pooled.fill_(77.0), out, lse, ws, splits, mass=added)
+    assert torch.equal(pooled, first)                                 # the weight's sum changes nothing else
+    if has_v:
+        _check_attention(out, lse, q, kf, vf, vc, lambda b, h: list(range(lens[b])), 128 ** -0.5, dtype, f"dense, {splits} splits")
     for b, n in enumerate(lens):
         total = torch.zeros(n, dtype=torch.float64)
         for h in range(G):

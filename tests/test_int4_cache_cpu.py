@@ -96,7 +96,8 @@ def test_c_entry_points_refuse_before_they_launch():
         pytest.skip("the library is initialised there: tests of the GPU cover the messages")
     lib = nat.load()
     layout = nat.KvLayout()
-    assert lib.kb200_mass_add(None, 0, None, None, None, 0, 0, 1, 0, None) != 0
+    assert lib.kb200_decode_anchor_paged_mass(None, 0, 0, C.byref(layout), None, 0, 0.0, None, None, 0, None, 0, None, None, None,
+                                              0, 0, 4, 1, 0, None) != 0
     assert lib.kb200_mass_add_prompt(None, 0, None, None, None, 0, 0, 0, 1, 0, 0, None) != 0
     assert lib.kb200_evict(C.byref(layout), 1, None, None, 0, None, 0, 1, 0, 0, None, None, None, 0, None, 0, 0, 1, 0, None) != 0
     assert lib.kb200_evict_workspace_bytes(2, 5, 3) == 4 * (2 * 8 + 2 * (3 + 6) + 4) and lib.kb200_evict_workspace_bytes(0, 5, 3) == 0
