@@ -454,7 +454,7 @@ int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t
                           int num_tiles, int n_rows, void* stream);
 
 /* Shortens every sequence of a cache to at most `budget` rows, in all layers alike: those with the largest mass[b, j] stay
- * (j < seq_lens[b]; a NaN counts as 0; ties go to the lowest row), and in any case the rows whose token position is below
+ * (j < seq_lens[b] and j < n_rows; a NaN counts as 0, an infinite weight as the largest number; ties go to the lowest row), and in any case the rows whose token position is below
  * `sinks` or within the last `recent` of the sequence's positions.  Kept rows below the new length stay where they are, those
  * behind it fill the rows that were let go, the lowest into the lowest: the smallest number of moves, and no row is both source
  * and target.  (The order of rows in a cache has no meaning to attention: positions are in the keys' rotation.)

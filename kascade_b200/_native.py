@@ -709,6 +709,8 @@ def kv_write(q_in, q_out, k_new, v_new, start_pos, n_new, kv: KvLayout, q_gain=N
     if inv_freq is not None:
         _want(inv_freq, torch.float32, "inv_freq")
         assert inv_freq.is_contiguous() and inv_freq.numel() == HEAD_DIM // 2
+    if not B * T:
+        return
     if positions is not None:
         where, ps = k_new.get_device(), positions.stride()
         if positions.dtype is not torch.int32 or positions.get_device() != where or len(ps) != 3 or positions.shape[1:] != (B, T) \
@@ -754,8 +756,10 @@ def kv_read(kv: KvLayout, seq_lens, k_out, v_out):
     if not (k_out.is_contiguous() and v_out.is_contiguous() and seq_lens.is_contiguous()) or seq_lens.shape != (B,) or D != HEAD_DIM \
             or seq_lens.dtype is not torch.int32 or seq_lens.get_device() != where or v_out.get_device() != where:
         raise KascadeNativeError(f"kv_read: expected contiguous k_out / v_out [B, T, G, {HEAD_DIM}] and seq_lens [B] int32 on one device")
+    if not k_out.numel():
+        return
     _check(lib.kb200_kv_read(C.byref(kv), _ptr(seq_lens), _ptr(k_out), _ptr(v_out), B, T, G, _stream()), "kb200_kv_read")
-    _launched(1 if k_out.numel() else 0)
+    _launched(1)
 
 
 def _want_rows(t: torch.Tensor, dtype, batch: int, name: str):
@@ -781,10 +785,14 @@ def mass_add_prompt(pooled, mass, out, seq_len=None):
         raise KascadeNativeError("mass_add_prompt: pooled and seq_len [B] must be contiguous, out must have the shape of mass")
     _same_device(pooled, seq_len=seq_len, mass=mass, out=out)
     rows = mass.shape[1]
+    if not mass.numel() or not pooled.numel():                # nothing to add to, or nothing to add
+        if out is not mass:
+            out.copy_(mass)
+        return
     _check(lib.kb200_mass_add_prompt(_ptr(pooled), stride, _ptr(seq_len), _ptr(mass), _ptr(out),
                                      mass.stride(0) if B > 1 else rows, out.stride(0) if B > 1 else rows, B, G, T, rows,
                                      _stream()), "kb200_mass_add_prompt")
-    _launched(1 if B and rows else 0)
+    _launched(1)
 
 
 @_on_device_of(0)
@@ -812,6 +820,8 @@ def evict(mass, layers, seq_lens, budget: int, recent: int, sinks: int, token_po
             if t.get_device() != where:
                 raise KascadeNativeError(f"the cache of layer {i} is on {t.device}, expected {mass.device}")
     dev = mass.device
+    if not mass.numel():
+        return torch.zeros_like(seq_lens), torch.empty_like(mass), torch.empty(B, rows, dtype=torch.int32, device=dev)
     lens = torch.empty(B, dtype=torch.int32, device=dev)
     mass_out = torch.empty(B, rows, dtype=torch.float32, device=dev)
     pos_out = torch.empty(B, rows, dtype=torch.int32, device=dev)
@@ -822,8 +832,7 @@ def evict(mass, layers, seq_lens, budget: int, recent: int, sinks: int, token_po
                            0 if token_positions is None else token_positions.stride(0), budget, recent, sinks, lens.data_ptr(),
                            mass_out.data_ptr(), pos_out.data_ptr(), rows, workspace.data_ptr(), size, B, num_kv_heads, rows,
                            _stream()), "kb200_evict")
-    if B and rows:
-        _launched(3 + (-(-len(layers) // 32) if rows > budget else 0))
+    _launched(3 + (-(-len(layers) // 32) if rows > budget else 0))
     return lens, mass_out, pos_out
 
 

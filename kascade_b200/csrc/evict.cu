@@ -3,6 +3,8 @@
 // declarations in kascade_b200.h say what each entry point computes; the reference has no counterpart.
 #include <cooperative_groups.h>
 
+#include <cfloat>
+
 #include "common.cuh"
 
 namespace kb200 {
@@ -83,7 +85,8 @@ static int mass_ctas(int64_t clusters) {
 }
 
 // ---- what stays ------------------------------------------------------------------------------------------------------
-// What the rows of a sequence are ranked by: +inf for protected ones, else their weight (a NaN counts as 0).  A cluster of CTAs
+// What the rows of a sequence are ranked by: +inf for protected ones, else their weight (a NaN counts as 0, an infinite one as the
+// largest number, so that it stays behind the protected rows).  A cluster of CTAs
 // takes a sequence: the newest position first, over all of it, then the keys of its piece.  Latency is what counts: 4 sequences of 32768
 // rows 20.6 us with one CTA each, 7.8 with eight.
 constexpr int kKeyThreads = 1024;
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(kKeyThreads) evict_keys_kernel(const EvictKeys
   for (int j = rank * kKeyThreads + tid; j < n; j += ctas * kKeyThreads) {
     const int pos = positions ? positions[j] : j;
     const float m = mass[j];
-    p.keys[b * p.key_stride + j] = pos < p.sinks || (int64_t)pos > (int64_t)newest - p.recent ? INFINITY : m == m ? m : 0.f;
+    p.keys[b * p.key_stride + j] = pos < p.sinks || (int64_t)pos > (int64_t)newest - p.recent ? INFINITY : m == m ? fminf(m, FLT_MAX) : 0.f;
   }
   if (positions) cluster.sync();                                  // the other CTAs have read this one's newest position
 }
@@ -348,7 +351,11 @@ extern "C" int kb200_evict(const kb200_kv_layout* layers, int n_layers, const in
   KB_REQUIRE(out_stride >= n_rows && mass_out != mass && pos_out != token_positions,
              "evict: outputs must hold %d rows and not be inputs", n_rows);
   if (check_layers(layers, n_layers) != 0) return -1;
-  if (batch == 0 || n_rows == 0) return 0;
+  if (batch == 0) return 0;
+  if (n_rows == 0) {
+    KB_CUDA(cudaMemsetAsync(new_lens, 0, (size_t)batch * 4, (cudaStream_t)stream));
+    return 0;
+  }
   const EvictWorkspace at(batch, n_rows, budget);
   KB_REQUIRE(workspace && workspace_bytes >= (size_t)at.words * 4 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "evict: a 16-byte aligned workspace of %lld bytes is required, got %zu", (long long)at.words * 4, workspace_bytes);

@@ -269,9 +269,10 @@ class EfficientKascadeStrategy(Strategy):
             y = y.contiguous()
         return y
 
-    @staticmethod
-    def _check_mass(mass, batch: int, rows: int, dev):
+    def _check_mass(self, mass, batch: int, rows: int, dev):
         """attention_mass of a call, before anything is launched."""
+        if self._shard is not None:
+            raise NotImplementedError("attention_mass is summed over all heads; a sharded strategy holds some of them")
         if mass.dim() != 2 or mass.dtype != torch.float32 or mass.shape[0] != batch or mass.shape[1] < rows or mass.device != dev \
                 or (mass.shape[1] > 1 and mass.stride(1) != 1):
             raise ValueError(f"attention_mass must be fp32 [{batch}, at least {rows}] on {dev}, the last dimension contiguous, got "
@@ -290,8 +291,6 @@ class EfficientKascadeStrategy(Strategy):
         sequence draws, summed over the heads (and, in a prompt, over the query tiles behind the row's own): what
         ``evict_kv`` chooses by.  Rows are counted from the sequence's first token."""
         mass = kwargs.get("attention_mass")
-        if mass is not None and self._shard is not None:
-            raise NotImplementedError("attention_mass is summed over all heads; a sharded strategy holds some of them")
         if mass is not None:
             self._check_mass(mass, query.shape[0], key.shape[2], query.device)
         if query.dtype not in nat.DTYPES or key.dtype != query.dtype or value.dtype != query.dtype:
@@ -671,7 +670,8 @@ class EfficientKascadeStrategy(Strategy):
                  token_positions=None):
         """Shortens every sequence of a paged cache to at most `budget` rows: those with the largest `attention_mass` [B, rows]
         fp32 stay (ties: the lowest row), the first `sinks` token positions and the last `recent` ones in any case.  The rows
-        that go are the same in all layers and heads, because anchor layers hand index rows to other layers and heads.
+        that go are the same in all layers and heads, because anchor layers hand index rows to other layers and heads.  `rows`
+        must be as long as the longest sequence: what lies behind is not kept.
 
         caches: the layers' (key_cache, value_cache) or (key_cache, value_cache, k_scale, v_scale); fp16, bf16 or 4-bit, changed in
         place.  Kept rows behind the new length move into the places before it that became free, no other row moves; so
@@ -693,6 +693,8 @@ class EfficientKascadeStrategy(Strategy):
             raise ValueError(f"attention_mass has {rows} rows, the block table {block_table.shape[1]} pages")
         if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
             seq_lens = seq_lens.to(torch.int32).contiguous()
+        if budget >= rows:                              # every row stays, protected or not
+            recent = sinks = 0
         layouts = [nat.kv_layout_paged(c[0], c[1], block_table, *c[2:]) for c in caches]
         return nat.evict(attention_mass, layouts, seq_lens, max(min(int(budget), rows), 1), int(recent), int(sinks), token_positions,
                          caches[0][0].shape[2])
@@ -714,6 +716,8 @@ class EfficientKascadeStrategy(Strategy):
         kernels/flash_decoding/reuse_kascade_gqa_decode_with_kvcache.py:160-171."""
         if max_seq_len is None:
             max_seq_len = int(seq_lens.max().item())
+        if attention_mass is not None:
+            self._check_mass(attention_mass, query.shape[0], int(max_seq_len), query.device)
         if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():     # the kernels read contiguous int32
             seq_lens = seq_lens.to(torch.int32).contiguous()
         if index_rows is not None:
@@ -726,8 +730,6 @@ class EfficientKascadeStrategy(Strategy):
                     or rows.device != query.device or counts.device != query.device:
                 raise ValueError(f"index_rows must be int32 [{want[0]}, {want[1]}, k], the last dimension contiguous, and contiguous "
                                  f"int32 counts {want} on {query.device}, got {tuple(rows.shape)} and {tuple(counts.shape)}")
-        if attention_mass is not None:
-            self._check_mass(attention_mass, query.shape[0], int(max_seq_len), query.device)
         kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, query.dtype)
         return self._decode(int(layer_idx), query, kv, seq_lens, int(max_seq_len), scaling, key_cache.shape[2],
                             mean_len=mean_seq_len, mass=attention_mass, index_rows=index_rows)

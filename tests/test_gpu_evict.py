@@ -354,3 +354,71 @@ def test_refusals_of_attention_mass():
 
     with pytest.raises(ValueError, match="attention_mass"):
         strat.attention_forward(M(), x, kv, kv, None, 0.1, attention_mass=good[:, :139])
+
+
+@pytest.mark.parametrize("S", [100, 6000])
+@pytest.mark.parametrize("own", [False, True], ids=["in_order", "own_positions"])
+def test_infinite_weight_does_not_displace_protected_rows(S, own):
+    """Rows of infinite weight stay before others, the lowest first, but never in the place of a protected row."""
+    g = torch.Generator().manual_seed(9)
+    mass = torch.rand(1, S, generator=g)
+    mass[0, 3:60] = math.inf
+    mass[0, 61] = -math.inf
+    order = torch.randperm(S, generator=g) if own else torch.arange(S)              # the row of each position
+    positions = torch.empty(1, S, dtype=torch.int32)
+    positions[0, order] = torch.arange(S, dtype=torch.int32)
+    from kascade_b200 import EfficientKascadeStrategy
+    table, pages = _tables([S], S, 16, 1)
+    cache = tuple(torch.zeros(pages, 16, 1, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    lens, weight, at = EfficientKascadeStrategy.evict_kv([cache], table.cuda(), torch.tensor([S], dtype=torch.int32, device="cuda"),
+                                                         mass.cuda(), 30, recent=8, sinks=2,
+                                                         token_positions=positions.cuda() if own else None)
+    protected = {0, 1, *range(S - 8, S)}
+    others = [int(positions[0, j]) for j in range(3, 60) if int(positions[0, j]) not in protected][:20]
+    assert lens.tolist() == [30]
+    assert sorted(at[0, :30].tolist()) == sorted([*protected, *others])
+    assert torch.equal(weight[0, :30].cpu(), mass[0, order[at[0, :30].cpu().long()]])
+
+
+def test_a_budget_beyond_the_rows_keeps_them_all():
+    """Also where more rows are protected than there are."""
+    lens, mass = [64, 10, 0], torch.rand(3, 64, generator=torch.Generator().manual_seed(4))
+    got = _run_evict(lens, 64, 500, 100, 20, 2, 16, 1, torch.float16, mass, None)
+    for b, n in enumerate(lens):
+        assert got[2][b].tolist() == [*range(n), *[-1] * (64 - n)]
+
+
+def test_calls_on_nothing():
+    """No rows, no sequences, no tokens: results of that size, and no error."""
+    from kascade_b200 import EfficientKascadeStrategy as S, int4_kv_cache
+    k, v, kp, vp = int4_kv_cache(4, 2)
+    i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device="cuda")      # noqa: E731
+    for B, rows in ((2, 0), (0, 16), (0, 0)):
+        lens, mass, at = S.evict_kv([(k, v, kp, vp)], i32(B, 1), i32(B), torch.zeros(B, rows, device="cuda"), 8, recent=4)
+        assert lens.tolist() == [0] * B and mass.shape == at.shape == (B, rows)
+        key, value = S.read_kv(k, v, i32(B, 1), i32(B), rows, k_scale=kp, v_scale=vp)
+        assert key.shape == value.shape == (B, rows, 2, 128)
+    mass = torch.rand(1, 5, device="cuda")
+    assert torch.equal(S.prompt_mass(torch.zeros(1, 2, 0, 128, device="cuda"), mass), mass)
+    assert S.prompt_mass(torch.zeros(0, 2, 1, 128, device="cuda"), mass[:0]).shape == (0, 5)
+    new = torch.zeros(2, 0, 2, 128, dtype=torch.float16, device="cuda")
+    q = S.append_kv(new, new, k, v, i32(2, 1), i32(2), query=torch.zeros(2, 0, 8, 128, dtype=torch.float16, device="cuda"),
+                    k_scale=kp, v_scale=vp, positions=i32(2, 0))
+    assert q.shape == (2, 0, 8, 128) and not bool(k.any())
+
+
+def test_weight_of_a_prompt_replays_from_a_cuda_graph():
+    from kascade_b200 import EfficientKascadeStrategy as S
+    g = torch.Generator().manual_seed(2)
+    pooled, mass = torch.rand(2, 2, 5, 256, generator=g).cuda(), torch.rand(2, 160, generator=g).cuda()
+    lens = torch.tensor([160, 70], dtype=torch.int32, device="cuda")
+    S.prompt_mass(pooled, mass, lens)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = S.prompt_mass(pooled, mass, lens)
+    for _ in range(2):
+        pooled.copy_(torch.rand(2, 2, 5, 256, generator=g))
+        mass.copy_(torch.rand(2, 160, generator=g))
+        lens.copy_(torch.tensor([33, 160], dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(out, S.prompt_mass(pooled, mass, lens))

@@ -492,3 +492,77 @@ def test_sums_over_long_lists_are_not_rounded_one_way(n, splits):
     bound = 2.0 ** -11 * want.abs() + 2.0 ** -21 * (vc[0, 0].mean(0) + (vf - vc)[0, 0].abs().mean(0))
     assert bool(((out[0].cpu().double() - want).abs() <= bound).all())
     assert float((lse.cpu().double() - math.log2(n)).abs().max()) <= 2.0 ** -20 * math.log2(n)
+
+
+def test_the_same_row_twice():
+    """An index row may name a row more than once; it then counts as often."""
+    from kascade_b200 import _native as nat
+    lens, G = [90], 2
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, 16, seed=71)
+    rows = torch.randint(0, 90, (1, G, 257), generator=torch.Generator().manual_seed(72), dtype=torch.int32)
+    rows[0, 1] = 89
+    q = _queries(1, 4 * G, torch.float16, 73)
+    out = torch.empty(1, 4 * G, 128, dtype=torch.float16, device="cuda")
+    kv = nat.kv_layout_paged(k, v, table, kp, vp)
+    nat.decode_sparse_paged(q, kv, rows.cuda(), None, 257, None, 128 ** -0.5, out, None, nat.decode_workspace(1, 8, 2, q.device), 2)
+    _check_attention(out, None, q, kf, vf, vc, lambda b, h: rows[b, h].tolist(), 128 ** -0.5, torch.float16, "repeated rows")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_kv_heads(dtype):
+    """70 KV heads: appended, read back, attended to."""
+    from kascade_b200 import _native as nat
+    G, B, T = 70, 2, 37
+    g = torch.Generator().manual_seed(81)
+    k, v, kp, vp, table = _empty_cache(B, T, G, 16)
+    new = torch.randn(B, T, 2 * G, 128, generator=g).to(dtype).cuda()
+    strat = _strategy(G)
+    starts, lens = torch.zeros(B, dtype=torch.int32, device="cuda"), torch.full((B,), T, dtype=torch.int32, device="cuda")
+    strat.append_kv(new[:, :, :G], new[:, :, G:], k, v, table, starts, k_scale=kp, v_scale=vp)
+    for b in range(B):
+        for cache, par, x, pieces in ((k, kp, new[b, :, :G], K_PIECES), (v, vp, new[b, :, G:], V_PIECES)):
+            got, got_par = _written(cache, par, table, 16, b, range(T))
+            codes, want_par = quantize(x.cpu())
+            assert torch.equal(got_par, want_par) and torch.equal(got, pack(codes, pieces))
+    key, value = strat.read_kv(k, v, table, lens, T, k_scale=kp, v_scale=vp, dtype=dtype)
+    flat = lambda c, p, pieces, zeros=True: torch.stack([                               # noqa: E731
+        unpack(*_written(c, p, table, 16, b, range(T)), pieces, zeros) for b in range(B)]).transpose(1, 2)
+    kf, vf, vc = flat(k, kp, K_PIECES), flat(v, vp, V_PIECES), flat(v, vp, V_PIECES, False)
+    for got, want in ((key, kf), (value, vf)):
+        off = (got.cpu().double().transpose(1, 2) - want).abs() - (HALF_STEP[dtype] + 2.0 ** -23) * want.abs() - 2.0 ** -25
+        assert bool((off <= 0).all())
+    q = _queries(B, 4 * G, dtype, 82)
+    out = torch.empty(B, 4 * G, 128, dtype=dtype, device="cuda")
+    rows = torch.arange(T, dtype=torch.int32, device="cuda").expand(B, G, T)
+    nat.decode_sparse_paged(q, nat.kv_layout_paged(k, v, table, kp, vp, dtype), rows, None, T, None, 0.1, out, None, None, 1)
+    _check_attention(out, None, q, kf, vf, vc, lambda b, h: list(range(T)), 0.1, dtype, "70 heads")
+
+
+def test_two_strategies_on_two_streams():
+    """Steps over one cache at once, each strategy with scratch of its own: the results of one after the other."""
+    lens, G = [3000, 500], 8
+    k, v, kp, vp, table, _, _, _ = make_cache(lens, G, 16, seed=91)
+    seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    strats, queries = [_strategy(G) for _ in range(2)], [_queries(2, 4 * G, torch.float16, 92 + i) for i in range(2)]
+    masses = [torch.zeros(2, 3000, device="cuda") for _ in range(2)]
+
+    def step(i):
+        return [strats[i].paged_decode_forward(layer, queries[i], k, v, table, seq, 128 ** -0.5, 3000, kp, vp, attention_mass=masses[i])
+                for layer in (0, 1)]
+
+    alone = []
+    for i in range(2):
+        alone.append([x.clone() for x in step(i)] + [masses[i].clone()])
+        masses[i].zero_()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                masses[i].zero_()
+                last = step(i)
+                if i == 0:
+                    first = last
+    torch.cuda.synchronize()
+    for got, want, mass in ((first, alone[0], masses[0]), (last, alone[1], masses[1])):
+        assert all(torch.equal(x, y) for x, y in zip([*got, mass], want))

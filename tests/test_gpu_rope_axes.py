@@ -184,3 +184,26 @@ def test_refusals_of_positions():
         call(positions=pos, token_positions=torch.zeros(2, 16, dtype=torch.int32, device="cuda"))
     with pytest.raises(nat.KascadeNativeError, match="cpu"):
         call(positions=pos.cpu())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,T", [(1, 1, 1), (3, 2, 9), (5, 1, 700)])
+def test_odd_numbers_of_query_heads(dtype, H, G, T):
+    from kascade_b200 import EfficientKascadeStrategy
+    g = torch.Generator().manual_seed(H)
+    k, v, table = _paged(2, T, G, 16, dtype, 6)
+    q, new = (torch.randn(2, T, n, 128, generator=g).to(dtype).cuda() for n in (H, 2 * G))
+    inv_freq = 10000.0 ** (-torch.arange(0, 128, 2).float() / 128)
+    positions = torch.randint(0, 100000, (1, 2, T), generator=g)
+    gain = (1 + 0.1 * torch.randn(128, generator=g)).to(dtype)
+    got = EfficientKascadeStrategy.append_kv(new[:, :, :G], new[:, :, G:], k, v, table, torch.zeros(2, dtype=torch.int32, device="cuda"),
+                                             query=q, q_norm_weight=gain.cuda(), inv_freq=inv_freq.cuda(), positions=positions[0].cuda())
+    want, slack = _turned(q.cpu(), gain, positions, None, inv_freq, 1e-6)
+    _check(got, want, slack, dtype, "q")
+    want, slack = _turned(new[:, :, :G].cpu(), None, positions, None, inv_freq, 1e-6)
+    k, v, table = k.cpu(), v.cpu(), table.cpu().long()
+    for b in range(2):
+        for t in range(T):
+            at = int(table[b, t // 16]), t % 16
+            _check(k[at], want[b, t], slack[b, t], dtype, "k")
+            assert torch.equal(v[at], new[b, t, G:].cpu())

@@ -106,3 +106,12 @@ def test_c_entry_points_refuse_before_they_launch():
     assert lib.kb200_kv_write_at(C.byref(act), None, C.byref(act), C.byref(act), None, None, C.byref(layout), None, None, 0.0, None, 1.0,
                                  None, 0, 0, 0, 1, None) != 0
     assert b"null pointer" in lib.kb200_last_error()
+
+
+def test_sharded_strategies_refuse_attention_mass_in_a_paged_step():
+    from kascade_b200 import EfficientKascadeStrategy
+    strat = EfficientKascadeStrategy([0], "x/y", k=10, tile_size=32, head_mapping=[[0, 1]] * 2, register=False, shard=(0, 2))
+    cache, table = torch.zeros(4, 16, 1, 128, dtype=torch.float16), torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(NotImplementedError, match="all heads"):
+        strat.paged_decode_forward(0, torch.zeros(1, 4, 128, dtype=torch.float16), cache, cache, table, torch.tensor([9]), 0.1, 9,
+                                   attention_mass=torch.zeros(1, 9))
