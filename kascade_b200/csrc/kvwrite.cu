@@ -250,14 +250,32 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// the ends of the two groups over a lane's eight values of either, as the row's own type or in fp32; a value that is not finite
-// makes the upper end infinite or a NaN
+// What four lanes hold as four pieces each, exchanged: piece i of lane q becomes piece q of lane i.
+template <typename T>
+__device__ __forceinline__ void exchange4(T& a0, T& a1, T& a2, T& a3, int q) {
+  auto swap = [](T& low, T& high, bool up, int with) {               // the lower lane's high piece for the upper lane's low one
+    const T got = __shfl_xor_sync(0xFFFFFFFFu, up ? low : high, with);
+    low = up ? got : low;
+    high = up ? high : got;
+  };
+  swap(a0, a1, q & 1, 1);
+  swap(a2, a3, q & 1, 1);
+  swap(a0, a2, q & 2, 2);
+  swap(a1, a3, q & 2, 2);
+}
+
+// the ends of a group of 32, as the row's own type or in fp32; a value that is not finite makes the upper end infinite or a NaN
 template <bool BF16>
-__device__ __forceinline__ void group_ends(const uint4& v, float& mn, float& mx) {
+__device__ __forceinline__ void group_ends(const uint4* v, float& mn, float& mx) {
   using H2 = typename Pair<BF16>::T;
-  const H2* h = reinterpret_cast<const H2*>(&v);
-  const float2 lo = to_f2(__hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3])));
-  const float2 hi = to_f2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+  const H2* h = reinterpret_cast<const H2*>(v);
+  H2 least = h[0], most = h[0];
+#pragma unroll
+  for (int e = 1; e < 16; ++e) {
+    least = __hmin2(least, h[e]);
+    most = __hmax2_nan(most, h[e]);
+  }
+  const float2 lo = to_f2(least), hi = to_f2(most);
   mn = fminf(lo.x, lo.y);
   mx = hi.x == hi.x && hi.y == hi.y && mn > -INFINITY ? fmaxf(hi.x, hi.y) : INFINITY;
 }
@@ -266,7 +284,7 @@ __device__ __forceinline__ void group_ends(const uint64_t* x, float& mn, float& 
   mn = INFINITY;
   mx = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 16; ++e) {
     const float2 v = unpack2(x[e]);
     mn = fminf(mn, fminf(v.x, v.y));
     mx = fmaxf(mx, fmaxf(v.x, v.y));
@@ -276,20 +294,15 @@ __device__ __forceinline__ void group_ends(const uint64_t* x, float& mn, float& 
   if (!(b.x + b.y == 0.f)) mx = INFINITY;
 }
 
-// The 4-bit form of a lane's eight values x of a group whose ends over the lane are mn, mx:
+// The 4-bit form of a group of 32 values x whose ends are mn, mx:
 //   z = fp16(min), s = fp16((max - z) / 15), c = round((x - z) / s) clamped to 0..15, half to even.
-// Values saturate at +-65504, what fp16 can hold; a group with a value that is not finite gets z = NaN.  Returns the eight
-// codes, the lowest nibble first.
+// Values saturate at +-65504, what fp16 can hold; a group with a value that is not finite gets z = NaN.  words: eight
+// codes each, the lowest nibble first.
 // A quotient is a product with 1 / s (good to 2^-22) and one step of correction by the remainder, which is exact: so quotients that
 // are a number of 24 bits come out as that number, halves among them, and are rounded by adding 1.5 2^23.  (Halves are not rare,
 // 0.07 % of bf16 values, because x, z and s have few bits; testing for them took as long as the division.)  The eight sums add up
 // to the packed codes and a constant.  Clamping is needed only where fp16 rounds an end by a good part of a step.
-__device__ __forceinline__ uint32_t quantize_int4(const uint64_t* x, float mn, float mx, __half& sh, __half& zh) {
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    mn = fminf(mn, __shfl_xor_sync(0xFFFFFFFFu, mn, o));
-    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-  }
+__device__ __forceinline__ void quantize_int4(const uint64_t* x, float mn, float mx, uint32_t* words, __half& sh, __half& zh) {
   const bool fine = mx < INFINITY;
   zh = __float2half_rn(fine ? fminf(fmaxf(mn, -65504.f), 65504.f) : NAN);
   const float z = __half2float(zh);
@@ -302,9 +315,9 @@ __device__ __forceinline__ uint32_t quantize_int4(const uint64_t* x, float mn, f
   constexpr float kMagic = 12582912.f;                                          // 1.5 2^23: sums are rounded to whole numbers
   const uint64_t z2 = pack2(z, z), inv2 = pack2(inv, inv), magic2 = pack2(kMagic, kMagic), minus_s2 = pack2(-s, -s);
   const bool clamp = !(mn - z > -0.4f * s && mx - z < 15.4f * s);               // (also where s is 0, or z a NaN)
-  float u[8];
+  float u[32];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 16; ++e) {
     const uint64_t a = sub2(x[e], z2), q = mul2(a, inv2);
     const float2 v = unpack2(add2(fma2(fma2(q, minus_s2, a), inv2, q), magic2));
     u[2 * e] = v.x;
@@ -312,13 +325,16 @@ __device__ __forceinline__ uint32_t quantize_int4(const uint64_t* x, float mn, f
   }
   if (__any_sync(0xFFFFFFFFu, clamp)) {                                         // (a branch: rarely taken, and long)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)                                                 // a NaN becomes 0, and so does all of it where s is 0
+    for (int e = 0; e < 32; ++e)                                                // a NaN becomes 0, and so does all of it where s is 0
       if (clamp) u[e] = fminf(fmaxf(s > 0.f ? u[e] : 0.f, kMagic), kMagic + 15.f);
   }
-  uint32_t w = 0u - 0x4B400000u * 0x11111111u;                                  // 0x4B400000: the bits of kMagic
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w += __float_as_uint(u[e]) << (4 * e);
-  return w;
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w = 0u - 0x4B400000u * 0x11111111u;                                // 0x4B400000: the bits of kMagic
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w += __float_as_uint(u[8 * i + e]) << (4 * e);
+    words[i] = w;
+  }
 }
 
 // How a row is stored
@@ -327,9 +343,11 @@ constexpr int kAppendThreads = 256;
 constexpr int kAppendTokens = 4;                                               // tokens of a CTA at most
 
 // Four lanes take an item: the K and the V row of a (token, KV head), whose places in the cache are the same, or two Q rows of a
-// token.  Lane q has the values 8q .. 8q+7 of each of a row's four groups of 32: the two that a rotation pairs up are in groups g and
-// g + 2, and what it stores of a 4-bit row is one piece of 16 bytes.  A CTA takes p.tokens tokens; its first items are loaded before
-// the angles are computed.  AT: positions of their own.
+// token.  To be normalised and rotated, lane q has the values 8q .. 8q+7 of each of a row's four groups of 32: the two that a rotation
+// pairs up are in groups g and g + 2.  To be quantised, it has group q: what is done per group is then done once (with every group
+// spread over the four lanes 32768 rows took 53 us).  Rows that nothing turns are loaded that way, the others are exchanged, and so are the
+// codes, of which a lane stores one piece of 16 bytes per row.  A CTA takes p.tokens tokens; its first items are loaded before the
+// angles are computed.  AT: positions of their own.
 template <bool BF16, int STORE, bool AT>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWriteParams p) {
   using H2 = typename Pair<BF16>::T;
@@ -341,6 +359,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
   const int tid = threadIdx.x, q = tid & 3;
   const int per = p.G + (p.H + 1) / 2, items = p.tokens * per;       // items of a token: KV heads first, then pairs of Q heads
   const uint32_t first = blockIdx.x * (uint32_t)p.tokens, all = (uint32_t)p.B * p.T;
+  const bool turns = p.k_gain || p.inv_freq;                          // K rows are normalised or rotated
   for (int item0 = 0; item0 < items; item0 += blockDim.x >> 2) {     // uniform for the CTA
     const int item = item0 + (tid >> 2);
     const int i = (item >= per) + (item >= 2 * per) + (item >= 3 * per), h = item - i * per;
@@ -357,9 +376,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
       const __half* src = !kv ? p.q_in + b * p.q_sb + t * p.q_st + (head + r) * p.q_sh
                               : r == 0 ? p.k_new + b * p.k_sb + t * p.k_st + head * p.k_sh
                                        : p.v_new + b * p.v_sb + t * p.v_st + head * p.v_sh;
+      const bool whole = STORE == kInt4 && kv && !(r == 0 && turns);
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        row[r][g] = active && (r == 0 || two) ? reinterpret_cast<const uint4*>(src)[4 * g + q] : make_uint4(0u, 0u, 0u, 0u);
+        row[r][g] = active && (r == 0 || two) ? reinterpret_cast<const uint4*>(src)[whole ? 4 * q + g : 4 * g + q] : make_uint4(0u, 0u, 0u, 0u);
     }
     if (item0 == 0) {
       // the tokens' places in the cache, and their angles
@@ -477,18 +497,41 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
           if (gain) module_norm<BF16>(lo, hi, gain, inv_rms, 4 * g + q);
           if (turn) module_rotate<BF16>(lo, hi, cos_s[i], sin_s[i], 4 * g + q);
         }
-        widen();
       }
-      uint32_t words[4];
-      __half scale[4], zero[4];
+      uint32_t words[4], scale01 = 0u, scale23 = 0u, zero01 = 0u, zero23 = 0u;
       if constexpr (STORE == kInt4) {
+        float mn, mx;
+        if constexpr (AT) {
+          if (r == 0 && turns) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float mn, mx;
-          if constexpr (AT) group_ends(x + 4 * g, mn, mx);
-          else group_ends<BF16>(row[r][g], mn, mx);
-          words[g] = quantize_int4(x + 4 * g, mn, mx, scale[g], zero[g]);
+            for (int e = 0; e < 4; ++e) exchange4(x[e], x[4 + e], x[8 + e], x[12 + e], q);
+          }
+          group_ends(x, mn, mx);
+        } else {
+          if (r == 0 && turns) {                                          // (Q rows, which are stored as they are, keep theirs)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t w[4];
+#pragma unroll
+              for (int g = 0; g < 4; ++g) w[g] = reinterpret_cast<const uint32_t*>(&row[r][g])[e];
+              exchange4(w[0], w[1], w[2], w[3], q);
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                if (kv) reinterpret_cast<uint32_t*>(&row[r][g])[e] = w[g];
+            }
+          }
+          widen();
+          group_ends<BF16>(row[r], mn, mx);
         }
+        __half scale, zero;
+        quantize_int4(x, mn, mx, words, scale, zero);
+        exchange4(words[0], words[1], words[2], words[3], q);
+        const uint32_t par = (uint32_t)__half_as_ushort(scale) | (uint32_t)__half_as_ushort(zero) << 16;
+        const uint32_t next = __shfl_xor_sync(0xFFFFFFFFu, par, 1);
+        scale01 = __byte_perm(par, next, 0x5410);                         // (as lanes 0 and 2 see them)
+        zero01 = __byte_perm(par, next, 0x7632);
+        scale23 = __shfl_xor_sync(0xFFFFFFFFu, scale01, 2);
+        zero23 = __shfl_xor_sync(0xFFFFFFFFu, zero01, 2);
       }
       if (!active || (r && !two)) continue;
       __half* cache = r == 0 ? p.k_cache : p.v_cache;
@@ -506,9 +549,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
         }
         *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(cache) + place + q * 16) = piece;
         if (q == 0) {
-          __align__(16) const __half par[8] = {scale[0], scale[1], scale[2], scale[3], zero[0], zero[1], zero[2], zero[3]};
           __half* dst = (r == 0 ? p.k_param : p.v_param) + b * p.pa_sb + phys * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(par);
+          *reinterpret_cast<uint4*>(dst) = make_uint4(scale01, scale23, zero01, zero23);
         }
       } else {
         const float sc = (r == 0 ? p.k_scale : p.v_scale)[b * p.s_sb + phys * p.s_sp + head * p.s_sh];
