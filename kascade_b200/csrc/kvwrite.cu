@@ -45,7 +45,7 @@ struct KvWriteParams {
   // the first axis is noted per cache row, [B, rows], or null
   const int32_t* positions; int64_t ps_axis, ps_b; const int32_t* pair_axis; int axes;
   int32_t* token_positions; int64_t tp_sb; int tp_rows;
-  int tokens;                                                         // kv_append_kernel: tokens of a CTA
+  int tokens, chunks;                                                 // kv_append_kernel: tokens of a CTA, CTAs of a sequence
 };
 
 // One CTA per (sequence, new token): the token's 64 (cos, sin) pairs are computed once and shared by all
@@ -298,10 +298,10 @@ __device__ __forceinline__ void group_ends(const uint64_t* x, float& mn, float& 
 //   z = fp16(min), s = fp16((max - z) / 15), c = round((x - z) / s) clamped to 0..15, half to even.
 // Values saturate at +-65504, what fp16 can hold; a group with a value that is not finite gets z = NaN.  words: eight
 // codes each, the lowest nibble first.
-// A quotient is a product with 1 / s (good to 2^-22) and one step of correction by the remainder, which is exact: so quotients that
-// are a number of 24 bits come out as that number, halves among them, and are rounded by adding 1.5 2^23.  (Halves are not rare,
-// 0.07 % of bf16 values, because x, z and s have few bits; testing for them took as long as the division.)  The eight sums add up
-// to the packed codes and a constant.  Clamping is needed only where fp16 rounds an end by a good part of a step.
+// A quotient is a product with 1 / s in two parts (good to 2^-44 together), rounded once: so quotients that are a number of 24 bits
+// come out as that number, halves among them, and are rounded by adding 1.5 2^23.  (Halves are not rare, 0.07 % of bf16 values,
+// because x, z and s have few bits; testing for them took as long as the division.)  The eight sums add up to the packed codes
+// and a constant.  Clamping is needed only where fp16 rounds an end by a good part of a step.
 __device__ __forceinline__ void quantize_int4(const uint64_t* x, float mn, float mx, uint32_t* words, __half& sh, __half& zh) {
   const bool fine = mx < INFINITY;
   zh = __float2half_rn(fine ? fminf(fmaxf(mn, -65504.f), 65504.f) : NAN);
@@ -313,13 +313,14 @@ __device__ __forceinline__ void quantize_int4(const uint64_t* x, float mn, float
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(s));
   constexpr float kMagic = 12582912.f;                                          // 1.5 2^23: sums are rounded to whole numbers
-  const uint64_t z2 = pack2(z, z), inv2 = pack2(inv, inv), magic2 = pack2(kMagic, kMagic), minus_s2 = pack2(-s, -s);
+  const float rest = fmaf(-s, inv, 1.f) * inv;                                  // (of s = 0 both are no numbers: clamped)
+  const uint64_t minus_z2 = pack2(-z, -z), inv2 = pack2(inv, inv), rest2 = pack2(rest, rest), magic2 = pack2(kMagic, kMagic);
   const bool clamp = !(mn - z > -0.4f * s && mx - z < 15.4f * s);               // (also where s is 0, or z a NaN)
   float u[32];
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const uint64_t a = sub2(x[e], z2), q = mul2(a, inv2);
-    const float2 v = unpack2(add2(fma2(fma2(q, minus_s2, a), inv2, q), magic2));
+    const uint64_t a = add2(x[e], minus_z2);
+    const float2 v = unpack2(add2(fma2(a, inv2, mul2(a, rest2)), magic2));
     u[2 * e] = v.x;
     u[2 * e + 1] = v.y;
   }
@@ -347,9 +348,10 @@ constexpr int kAppendTokens = 4;                                               /
 // pairs up are in groups g and g + 2.  To be quantised, it has group q: what is done per group is then done once (with every group
 // spread over the four lanes 32768 rows took 53 us).  Rows that nothing turns are loaded that way, the others are exchanged, and so are the
 // codes, of which a lane stores one piece of 16 bytes per row.  A CTA takes p.tokens tokens; its first items are loaded before the
-// angles are computed.  AT: positions of their own.
+// angles are computed.  AT: positions of their own.  Quantising is bounded to 80 registers: with 64 / 118, 32768 rows take 52 / 46
+// us, so 44.
 template <bool BF16, int STORE, bool AT>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWriteParams p) {
+__global__ void __launch_bounds__(kAppendThreads, STORE == kInt4 ? 3 : 0) kv_append_kernel(const KvWriteParams p) {
   using H2 = typename Pair<BF16>::T;
   using Angle = typename std::conditional<AT, float, typename Pair<BF16>::S>::type;
   __shared__ __align__(16) Angle cos_s[kAppendTokens][kD / 2];
@@ -358,15 +360,15 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
   __shared__ int slot_s[kAppendTokens];
   const int tid = threadIdx.x, q = tid & 3;
   const int per = p.G + (p.H + 1) / 2, items = p.tokens * per;       // items of a token: KV heads first, then pairs of Q heads
-  const uint32_t first = blockIdx.x * (uint32_t)p.tokens, all = (uint32_t)p.B * p.T;
+  const int b = blockIdx.x / p.chunks, t0 = (blockIdx.x - b * p.chunks) * p.tokens;
+  const int t_end = p.n_new ? min(p.n_new[b], p.T) : p.T;
   const bool turns = p.k_gain || p.inv_freq;                          // K rows are normalised or rotated
   for (int item0 = 0; item0 < items; item0 += blockDim.x >> 2) {     // uniform for the CTA
     const int item = item0 + (tid >> 2);
     const int i = (item >= per) + (item >= 2 * per) + (item >= 3 * per), h = item - i * per;
     static_assert(kAppendTokens == 4, "three comparisons");
-    const uint32_t token = first + i;
-    const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * p.T);
-    const bool active = item < items && token < all && (!p.n_new || t < p.n_new[b]);
+    const int t = t0 + i;
+    const bool active = item < items && t < t_end;
     const bool kv = h < p.G;
     const int head = kv ? h : 2 * (h - p.G);
     const bool two = kv || head + 1 < p.H;
@@ -379,22 +381,21 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
       const bool whole = STORE == kInt4 && kv && !(r == 0 && turns);
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        row[r][g] = active && (r == 0 || two) ? reinterpret_cast<const uint4*>(src)[whole ? 4 * q + g : 4 * g + q] : make_uint4(0u, 0u, 0u, 0u);
+        row[r][g] = active && (r == 0 || two) ? reinterpret_cast<const uint4*>(src)[whole ? 4 * q + g : 4 * g + q]
+                                              : make_uint4(0u, 0u, 0u, 0u);
     }
     if (item0 == 0) {
       // the tokens' places in the cache, and their angles
       for (int at = tid; at < p.tokens * (p.inv_freq ? kD / 2 : 1); at += blockDim.x) {
         const int j = p.inv_freq ? at / (kD / 2) : at, pair = p.inv_freq ? at % (kD / 2) : 0;
-        const uint32_t tk = first + j;
-        const int tb = (int)(tk / (uint32_t)p.T), tt = (int)(tk - (uint32_t)tb * p.T);
-        if (tk >= all || (p.n_new && tt >= p.n_new[tb])) continue;
-        const int pos = p.start_pos[tb] + tt;
-        const int32_t* own = AT ? p.positions + tb * p.ps_b + tt : nullptr;
+        if (t0 + j >= t_end) continue;
+        const int pos = p.start_pos[b] + t0 + j;
+        const int32_t* own = AT ? p.positions + b * p.ps_b + t0 + j : nullptr;
         if (pair == 0) {
           const int page = pos >> p.page_shift;
-          page_s[j] = p.block_table ? (int64_t)p.block_table[(int64_t)tb * p.bt_stride + page] : page;
+          page_s[j] = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + page] : page;
           slot_s[j] = pos & p.page_mask;
-          if (AT && p.token_positions && pos < p.tp_rows) p.token_positions[tb * p.tp_sb + pos] = own[0];
+          if (AT && p.token_positions && pos < p.tp_rows) p.token_positions[b * p.tp_sb + pos] = own[0];
         }
         if (!p.inv_freq) continue;
         float sn, cs;
@@ -563,17 +564,20 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvWrite
 }
 
 // One warp per CTA where there are many tokens: then a CTA makes several passes, and while one waits for its rows or computes its angles
-// the others on the SM work.  Few tokens: all items of a token at once.  What bounds it is issue slots, the integer pipe above all:
-// us (and TB/s) for 32768 tokens of 8 KV heads to 4 bits 53 (3.3; with rotary 63), 16384 tokens of 32 + 8 heads with positions on three
-// axes 72 (5.6; with norm 77).  With two / three warps per CTA those two take 76 / 83 and 85 / 91, and with all items at once 81 and 95; 64
-// tokens of 32 + 8 heads 5.7 with all items at once, 8.1 with two warps.
+// the others on the SM work.  Few tokens: all items of a token at once.  us (and TB/s) for 32768 tokens of 8 KV heads to 4 bits 44
+// (4.0; with rotary 53), of which quantising is 10 (storing sums of the values instead: 34).  16384 tokens of 32 + 8 heads with
+// positions on three axes 71 (5.7; with norm 76).  With two / three warps per CTA those two take 76 / 83 and 85 / 91, and with all
+// items at once 81 and 95; 64 tokens of 32 + 8 heads 5.7 with all items at once, 8.1 with two warps.
 template <bool BF16, int STORE, bool AT>
 static void launch_kv_append(KvWriteParams p, int64_t tokens, cudaStream_t st) {
   const int per = p.G + (p.H + 1) / 2;
   p.tokens = 1;
-  while (p.tokens < kAppendTokens && p.tokens * 2 * per <= 16 && tokens >= (int64_t)p.tokens * 2 * 8 * sm_count()) p.tokens *= 2;
+  while (p.tokens < kAppendTokens && p.tokens * 2 * per <= 16 && p.tokens * 2 <= p.T &&
+         tokens >= (int64_t)p.tokens * 2 * 8 * sm_count())
+    p.tokens *= 2;
+  p.chunks = (p.T + p.tokens - 1) / p.tokens;
   const int threads = (p.tokens * per * 4 + 31) / 32 * 32, most = tokens > 8ll * sm_count() ? 32 : kAppendThreads;
-  kv_append_kernel<BF16, STORE, AT><<<(unsigned)((tokens + p.tokens - 1) / p.tokens), threads < most ? threads : most, 0, st>>>(p);
+  kv_append_kernel<BF16, STORE, AT><<<(unsigned)p.B * (unsigned)p.chunks, threads < most ? threads : most, 0, st>>>(p);
 }
 template <bool BF16>
 static void launch_kv_append(const KvWriteParams& p, int store, int64_t tokens, cudaStream_t st) {
