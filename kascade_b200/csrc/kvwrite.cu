@@ -19,6 +19,7 @@
 // (a few instructions of 64 of the threads of a CTA), norm and rotation are computed in fp32 and rounded once.
 #include <cuda_bf16.h>
 
+#include <climits>
 #include <type_traits>
 
 #include "common.cuh"
@@ -595,49 +596,56 @@ struct KvReadParams {
   const int32_t* block_table; int bt_stride; int page_shift, page_mask;
   const int32_t* seq_lens;
   __half* k_out; __half* v_out;                                       // [B, T, G, D]
-  int T, G; int64_t rows;
+  int G, rows, chunks;                                                // rows of a sequence (T G), CTAs that share them
 };
 
-// the eight values of a word of codes, the lowest nibble first
+// the eight values of a word of codes, the lowest nibble first: a code in the low bits of 2^23 is that number and the code
 template <bool BF16>
-__device__ __forceinline__ uint4 from_codes(uint32_t w, float s, float z) {
+__device__ __forceinline__ uint4 from_codes(uint32_t w, uint64_t s2, uint64_t z2) {
   using H2 = typename Pair<BF16>::T;
+  const uint64_t minus = pack2(-8388608.f, -8388608.f);
   H2 out[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    out[e] = from_f2<BF16>(fmaf((float)((w >> (8 * e)) & 15u), s, z), fmaf((float)((w >> (8 * e + 4)) & 15u), s, z));
+  for (int e = 0; e < 4; ++e) {
+    const uint64_t c = pack2(__uint_as_float(((w >> (8 * e)) & 15u) | 0x4B000000u),
+                             __uint_as_float(((w >> (8 * e + 4)) & 15u) | 0x4B000000u));
+    const float2 v = unpack2(fma2(add2(c, minus), s2, z2));
+    out[e] = from_f2<BF16>(v.x, v.y);
+  }
   return *reinterpret_cast<uint4*>(out);
 }
 
+constexpr int kReadThreads = 256;
+constexpr int kReadBlock = kReadThreads / 4;                              // rows of a CTA; a CTA stays within a sequence
+// Bound by HBM: 32768 rows of 8 KV heads 31.4 us, 5.6 TB/s, the same with two or four rows per thread and with 64 or 128 threads.
 template <bool BF16>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
-  const int64_t row = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 2);
-  const int q = threadIdx.x & 3;
+__global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const KvReadParams p) {
+  const int b = blockIdx.x / p.chunks, row = (blockIdx.x - b * p.chunks) * kReadBlock + (threadIdx.x >> 2), q = threadIdx.x & 3;
   if (row >= p.rows) return;
-  const int64_t token = row / p.G;
-  const int head = (int)(row - token * p.G), b = (int)(token / p.T), t = (int)(token - (int64_t)b * p.T);
-  uint4* ko = reinterpret_cast<uint4*>(p.k_out + row * kD) + q;          // group g: 16-byte piece 4 g + q
-  uint4* vo = reinterpret_cast<uint4*>(p.v_out + row * kD) + q;
-  if (t >= p.seq_lens[b]) {                                              // rows behind a sequence read as zeros
-#pragma unroll
-    for (int g = 0; g < 4; ++g) ko[4 * g] = vo[4 * g] = make_uint4(0u, 0u, 0u, 0u);
-    return;
+  const int t = row / p.G, head = row - t * p.G;
+  uint4 kw = make_uint4(0u, 0u, 0u, 0u), vw = kw, kp = kw, vp = kw;        // rows behind a sequence read as zeros
+  if (t < p.seq_lens[b]) {
+    const int lp = t >> p.page_shift, slot = t & p.page_mask;
+    const int64_t page = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + lp] : lp;
+    const int64_t at = b * p.c_sb + page * p.c_sp + slot * p.c_st + head * p.c_sh + q * 16;
+    const int64_t pa = b * p.pa_sb + page * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
+    kw = *reinterpret_cast<const uint4*>(p.k + at);
+    vw = *reinterpret_cast<const uint4*>(p.v + at);
+    kp = *reinterpret_cast<const uint4*>(p.k_param + pa);
+    vp = *reinterpret_cast<const uint4*>(p.v_param + pa);
   }
-  const int lp = t >> p.page_shift, slot = t & p.page_mask;
-  const int64_t page = p.block_table ? (int64_t)p.block_table[(int64_t)b * p.bt_stride + lp] : lp;
-  const int64_t at = b * p.c_sb + page * p.c_sp + slot * p.c_st + head * p.c_sh + q * 16;
-  const int64_t pa = b * p.pa_sb + page * p.pa_sp + slot * p.pa_st + head * p.pa_sh;
-  const uint4 kw = *reinterpret_cast<const uint4*>(p.k + at), vw = *reinterpret_cast<const uint4*>(p.v + at);
-  const uint4 kp = *reinterpret_cast<const uint4*>(p.k_param + pa), vp = *reinterpret_cast<const uint4*>(p.v_param + pa);
+  uint4* ko = reinterpret_cast<uint4*>(p.k_out + ((int64_t)b * p.rows + row) * kD) + q;      // group g: 16-byte piece 4 g + q
+  uint4* vo = reinterpret_cast<uint4*>(p.v_out + ((int64_t)b * p.rows + row) * kD) + q;
   const uint32_t k_codes[4] = {kw.x, kw.y, kw.z, kw.w};
   const uint32_t v_codes[4] = {__byte_perm(vw.x, vw.z, 0x5410), __byte_perm(vw.x, vw.z, 0x7632), __byte_perm(vw.y, vw.w, 0x5410),
                                __byte_perm(vw.y, vw.w, 0x7632)};
   const __half* ks = reinterpret_cast<const __half*>(&kp);
   const __half* vs = reinterpret_cast<const __half*>(&vp);
+  auto twice = [](__half x) { return pack2(__half2float(x), __half2float(x)); };
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    ko[4 * g] = from_codes<BF16>(k_codes[g], __half2float(ks[g]), __half2float(ks[4 + g]));
-    vo[4 * g] = from_codes<BF16>(v_codes[g], __half2float(vs[g]), __half2float(vs[4 + g]));
+    ko[4 * g] = from_codes<BF16>(k_codes[g], twice(ks[g]), twice(ks[4 + g]));
+    vo[4 * g] = from_codes<BF16>(v_codes[g], twice(vs[g]), twice(vs[4 + g]));
   }
 }
 
@@ -780,9 +788,11 @@ extern "C" int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens,
   KB_REQUIRE(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0,
              "kv_read: k_out and v_out must be 16-byte aligned");
   KvReadParams p{};
-  p.rows = (int64_t)batch * max_len * num_kv_heads;
-  if (p.rows == 0) return 0;
-  KB_REQUIRE((p.rows + 63) / 64 < (1ll << 31), "kv_read: too many rows for one launch");
+  if (batch == 0 || max_len == 0) return 0;
+  const int64_t rows = (int64_t)max_len * num_kv_heads, chunks = (rows + kReadBlock - 1) / kReadBlock;
+  KB_REQUIRE(rows <= INT_MAX - kReadBlock && batch * chunks < (1ll << 31), "kv_read: too many rows for one launch");
+  p.rows = (int)rows;
+  p.chunks = (int)chunks;
   p.k = static_cast<const uint8_t*>(kv->k);
   p.v = static_cast<const uint8_t*>(kv->v);
   p.c_sb = kv->stride_batch; p.c_sp = kv->stride_page; p.c_st = kv->stride_token; p.c_sh = kv->stride_head;
@@ -798,11 +808,10 @@ extern "C" int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens,
   p.seq_lens = seq_lens;
   p.k_out = static_cast<__half*>(k_out);
   p.v_out = static_cast<__half*>(v_out);
-  p.T = max_len;
   p.G = num_kv_heads;
-  const unsigned blocks = (unsigned)((p.rows + 63) / 64);
-  if (kv->act_dtype == KB200_BF16) kv_read_kernel<true><<<blocks, 256, 0, (cudaStream_t)stream>>>(p);
-  else kv_read_kernel<false><<<blocks, 256, 0, (cudaStream_t)stream>>>(p);
+  const unsigned blocks = (unsigned)(batch * chunks);
+  if (kv->act_dtype == KB200_BF16) kv_read_kernel<true><<<blocks, kReadThreads, 0, (cudaStream_t)stream>>>(p);
+  else kv_read_kernel<false><<<blocks, kReadThreads, 0, (cudaStream_t)stream>>>(p);
   KB_CHECK_LAUNCH("kv_read_kernel");
   return 0;
 }
