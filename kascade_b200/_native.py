@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import os
+import struct
 from typing import Optional
 
 import torch
@@ -49,6 +50,10 @@ class KvLayout(C.Structure):
                 ("k_param", C.c_void_p), ("v_param", C.c_void_p), ("param_stride_batch", C.c_int64),
                 ("param_stride_page", C.c_int64), ("param_stride_token", C.c_int64), ("param_stride_head", C.c_int64),
                 ("act_dtype", C.c_int32)]
+
+
+_LAYOUT = struct.Struct("PPqqqqPiiiPPqqqPPqqqqi0P")      # the same: packing costs half of what the fields of a KvLayout do
+assert _LAYOUT.size == C.sizeof(KvLayout)
 
 
 class Positions(C.Structure):
@@ -348,13 +353,13 @@ def _int4_params(k, v, k_param, v_param):
     strides of the codes and of the parameters."""
     where, st = k.get_device(), k.stride()
     if where >= 0 and len(st) == 4 and st[3] == 1 and k_param is not None:
-        ps, shape = k_param.stride(), k.shape
-        if ps[-1] == 1 and k_param.dtype is torch.float16 and k_param.get_device() == where \
-                and k_param.shape == (*shape[:3], 8):
+        ps, shape, pshape = k_param.stride(), k.shape, k_param.shape
+        if len(ps) == 4 and ps[3] == 1 and k_param.dtype is torch.float16 and k_param.get_device() == where and pshape[:3] == shape[:3] \
+                and pshape[-1] == 8:
             if v is None:
                 return st, ps
-            if v_param is not None and v.shape == shape and v.stride() == st and v.dtype == k.dtype and v.get_device() == where \
-                    and v_param.dtype is torch.float16 and v_param.shape == k_param.shape and v_param.stride() == ps \
+            if v_param is not None and v.shape == shape and v.stride() == st and v.dtype is k.dtype and v.get_device() == where \
+                    and v_param.dtype is torch.float16 and v_param.shape == pshape and v_param.stride() == ps \
                     and v_param.get_device() == where:
                 return st, ps
     # something is wrong: say what
@@ -393,9 +398,10 @@ def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], bloc
             _want(block_table, torch.int32, "block_table")
             _same_device(k_cache, block_table=block_table)
             raise KascadeNativeError("block_table: expected [B, max_pages], the last dimension contiguous")
-        layout = KvLayout(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2],
-                          block_table.data_ptr(), ts[0], k_cache.shape[1], INT4, 0, 0, 0, 0, 0, k_scale.data_ptr(),
-                          0 if v_cache is None else v_scale.data_ptr(), 0, ps[0], ps[1], ps[2], DTYPES[act_dtype])
+        layout = KvLayout.from_buffer_copy(_LAYOUT.pack(
+            k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2], block_table.data_ptr(), ts[0],
+            k_cache.shape[1], INT4, 0, 0, 0, 0, 0, k_scale.data_ptr(), 0 if v_cache is None else v_scale.data_ptr(), 0, ps[0], ps[1],
+            ps[2], DTYPES[act_dtype]))
         layout._keep = (k_cache, block_table, k_scale) if v_cache is None else (k_cache, v_cache, block_table, k_scale, v_scale)
         return layout
     if k_cache.dtype in FP8_TORCH:

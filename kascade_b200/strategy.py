@@ -572,7 +572,7 @@ class EfficientKascadeStrategy(Strategy):
         sb, sh, sd = q.stride()
         if sd != 1 or sb % 2 or sh % 2:
             q = q.contiguous()
-        out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         ragged = float(max_len) / mean_len if mean_len else 1.0
         if dense_only or self.is_anchor(layer):
             splits_a = self._splits(B, G, max_len, ragged, dev)
@@ -724,10 +724,10 @@ class EfficientKascadeStrategy(Strategy):
             if self.is_anchor(int(layer_idx)):
                 raise ValueError(f"layer {layer_idx} is an anchor layer: it selects its own rows")
             rows, counts = index_rows
-            want = (query.shape[0], key_cache.shape[2])
-            if rows.dim() != 3 or tuple(rows.shape[:2]) != want or tuple(counts.shape) != want or not counts.is_contiguous() \
-                    or rows.stride(2) != 1 or not rows.shape[2] or rows.dtype != torch.int32 or counts.dtype != torch.int32 \
-                    or rows.device != query.device or counts.device != query.device:
+            want, shape, where = (query.shape[0], key_cache.shape[2]), rows.shape, query.get_device()
+            if len(shape) != 3 or shape[:2] != want or not shape[2] or counts.shape != want or not counts.is_contiguous() \
+                    or rows.stride(2) != 1 or rows.dtype is not torch.int32 or counts.dtype is not torch.int32 \
+                    or rows.get_device() != where or counts.get_device() != where:
                 raise ValueError(f"index_rows must be int32 [{want[0]}, {want[1]}, k], the last dimension contiguous, and contiguous "
                                  f"int32 counts {want} on {query.device}, got {tuple(rows.shape)} and {tuple(counts.shape)}")
         kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, query.dtype)
