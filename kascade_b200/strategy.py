@@ -553,16 +553,20 @@ class EfficientKascadeStrategy(Strategy):
         return max(max_len if max_len <= 128 else max(topk_budget(self.k, max_len, self.tile_size), 128), 1)
 
     @staticmethod
-    def _splits(B: int, G: int, keys_max: int, raggedness: float, dev) -> int:
+    def _splits(B: int, G: int, keys_max: int, raggedness: float, dev, int4: bool = False) -> int:
         """Splits per (sequence, KV head).  The library's own choice assumes sequences of one length; in a batch whose
         longest sequence is `raggedness` times the mean the CTAs of the long ones would set the kernel's time, so
         they are cut until the longest CTA is about the batch's work divided by three CTAs per SM (measured on
-        batches of 32-128 sequences of 4k-65k tokens: 10-19 % faster at 32 and 64 sequences, no change at 128)."""
+        batches of 32-128 sequences of 4k-65k tokens: 10-19 % faster at 32 and 64 sequences, no change at 128).
+        Dense passes over a 4-bit cache have smaller CTAs, so the longest is cut to a sixth of an SM's share, of 1024 keys at
+        least (ragged batches, us by the other rule / by this: 8 x 32768 70 / 66, 16 x 32768 118 / 113, 32 x 16384 124 / 120, 64 x
+        8192 125 / 113, 128 x 4096 118 / 116).  Their reuse layers, where a CTA reads few keys anyway, are not cut for it (8
+        x 3244 keys 23.0 / 16.6, 16 x 3244 24.5 / 22.5, 32 x 1606 25.3 / 21.9, 64 x 3244 69 / 67)."""
         s = nat.decode_default_splits(B, G, keys_max, dev.index)
         if raggedness > 1.25:
-            slots = 3 * nat.sm_count(dev.index)
+            slots = (6 if int4 else 3) * nat.sm_count(dev.index)
             want = -(-int(raggedness * slots) // max(B * G, 1))
-            s = max(s, min(want, max(keys_max // 256, 1), 32))
+            s = max(s, min(want, max(keys_max // (1024 if int4 else 256), 1), 32))
         return s
 
     def _decode(self, layer: int, q, kv, seq_lens, max_len: int, scaling, G: int, dense_only=False,
@@ -574,8 +578,9 @@ class EfficientKascadeStrategy(Strategy):
             q = q.contiguous()
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         ragged = float(max_len) / mean_len if mean_len else 1.0
+        int4 = kv.dtype == nat.INT4
         if dense_only or self.is_anchor(layer):
-            splits_a = self._splits(B, G, max_len, ragged, dev)
+            splits_a = self._splits(B, G, max_len, ragged, dev, int4)
             stride = -(-max_len // 4) * 4
             logits = self._scratch("dec_logits", (B, H, stride), torch.float32, dev)
             pooled = self._scratch("dec_pooled", (B, G, stride), torch.float32, dev)
@@ -600,7 +605,7 @@ class EfficientKascadeStrategy(Strategy):
             head_map = self._mapping(layer, dev)
         rows, counts = (self._dec_idx, self._dec_count) if index_rows is None else index_rows
         kmax = rows.shape[2]
-        splits = self._splits(B, G, kmax, ragged, dev)
+        splits = self._splits(B, G, kmax, 1.0 if int4 else ragged, dev)
         ws = self._scratch("dec_ws_s", (nat.decode_workspace_bytes(B, H, splits),), torch.uint8, dev)
         nat.decode_sparse_paged(q, kv, rows, counts, kmax, head_map, scaling, out, None, ws, splits)
         return out
