@@ -75,6 +75,28 @@ __device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// The sequence of rank r by length, the longest first (equal lengths by position), found by all threads of the CTA; `lens` is n + 1
+// words of shared memory, free again when it returns.  A long sequence whose CTAs start last runs alone at the end.  us of a dense pass
+// with sequences as they come / the longest first, in the best number of splits of either: 8 of up to 32768 keys 60.7 / 62.4, 16 109
+// / 104, 64 434 / 376, 24 and 32 and 48 of up to 16384 93.5 / 88.4, 114 / 102 and 167 / 143, 64 of up to 8192 108 / 99.5.  Sequences
+// of one length pay for it: 64 x 4096 96.0 / 97.5, 64 x 16384 332.8 / 333.3; 200 x 2048, which are not ranked, 129 / 147.
+constexpr int kRankMax4 = 64;
+__device__ __forceinline__ int longest_first4(int r, int n, const int32_t* seq_lens, int* lens) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) lens[i] = seq_lens[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int mine = lens[i];
+    int before = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) before += lens[j] > mine || (lens[j] == mine && j < i);
+    if (before == r) lens[n] = i;
+  }
+  __syncthreads();
+  const int b = lens[n];
+  __syncthreads();
+  return b;
+}
+
 template <bool DENSE, bool HAS_V, bool BF16>
 __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const DecodeParams p) {
   pdl_wait();
@@ -82,7 +104,9 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
   constexpr int kStages = stages4(HAS_V), kStage = stage_bytes4(HAS_V);
   const int WARPS = blockDim.x >> 5;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  const int split = blockIdx.x, g = blockIdx.y;
+  const int b = DENSE && p.by_length ? longest_first4(blockIdx.z, gridDim.z, p.seq_lens, reinterpret_cast<int*>(smem))
+                                     : (int)blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = lane >> 2, quad = lane & 3;
 
@@ -444,9 +468,10 @@ int init_decode4() { return init_one<false, true>() || init_one<true, true>() ||
 // 4 warps: reuse of 128 x 1606 rows 97.5 / 93.9, 256 x 787 102.7 / 94.2; dense passes of 256 x 2048 179 / 160, 16 of 5213..32768 rows in 7
 // splits 115 / 111; but 64 x 3244 rows, 3.5 CTAs per SM, 93 / 102.
 template <bool DENSE, bool HAS_V>
-static cudaError_t launch(const DecodeParams& p, dim3 grid, cudaStream_t st) {
+static cudaError_t launch(DecodeParams p, dim3 grid, cudaStream_t st) {
   const long long total = (long long)grid.x * grid.y * grid.z, sms = sm_count();
   const int warps = total >= 6 * sms ? kWarps4 / 4 : total * 2 >= 3 * sms ? kWarps4 / 2 : kWarps4;
+  p.by_length = DENSE && grid.z > 1 && grid.z <= kRankMax4 && total > 2 * sms;      // more CTAs than start at once
   const size_t smem = (size_t)warps * warp_bytes4(HAS_V);
   return launch_pdl(p.bf16 ? decode_attn4_kernel<DENSE, HAS_V, true> : decode_attn4_kernel<DENSE, HAS_V, false>, grid, warps * 32, smem,
                     st, 1, p);

@@ -558,15 +558,15 @@ class EfficientKascadeStrategy(Strategy):
         longest sequence is `raggedness` times the mean the CTAs of the long ones would set the kernel's time, so
         they are cut until the longest CTA is about the batch's work divided by three CTAs per SM (measured on
         batches of 32-128 sequences of 4k-65k tokens: 10-19 % faster at 32 and 64 sequences, no change at 128).
-        Dense passes over a 4-bit cache have smaller CTAs, so the longest is cut to a sixth of an SM's share, of 1024 keys at
-        least (ragged batches, us by the other rule / by this: 8 x 32768 70 / 66, 16 x 32768 118 / 113, 32 x 16384 124 / 120, 64 x
-        8192 125 / 113, 128 x 4096 118 / 116).  Their reuse layers, where a CTA reads few keys anyway, are not cut for it (8
-        x 3244 keys 23.0 / 16.6, 16 x 3244 24.5 / 22.5, 32 x 1606 25.3 / 21.9, 64 x 3244 69 / 67)."""
+        Dense passes over a 4-bit cache start with the longest sequences, so about three CTAs per SM do, of 2048 keys at least
+        (us by the other rule / by this: 8 of up to 32768 keys 66 / 63, 16 108 / 105, 32 of up to 16384 108 / 105, 16 of up to 8192
+        39.4 / 38.6).  Their reuse layers, where a CTA reads few keys anyway, are not cut for it (8 x 3244 keys 23.0 / 16.6, 16 x
+        3244 24.5 / 22.5, 32 x 1606 25.3 / 21.9, 64 x 3244 69 / 67)."""
         s = nat.decode_default_splits(B, G, keys_max, dev.index)
         if raggedness > 1.25:
-            slots = (6 if int4 else 3) * nat.sm_count(dev.index)
-            want = -(-int(raggedness * slots) // max(B * G, 1))
-            s = max(s, min(want, max(keys_max // (1024 if int4 else 256), 1), 32))
+            slots = 3 * nat.sm_count(dev.index)
+            want = -(-int(slots if int4 else raggedness * slots) // max(B * G, 1))
+            s = max(s, min(want, max(keys_max // (2048 if int4 else 256), 1), 32))
         return s
 
     def _decode(self, layer: int, q, kv, seq_lens, max_len: int, scaling, G: int, dense_only=False,

@@ -566,3 +566,25 @@ def test_two_strategies_on_two_streams():
     torch.cuda.synchronize()
     for got, want, mass in ((first, alone[0], masses[0]), (last, alone[1], masses[1])):
         assert all(torch.equal(x, y) for x, y in zip([*got, mass], want))
+
+
+@pytest.mark.parametrize("B", [5, 33, 64])
+def test_dense_passes_of_ragged_batches_in_many_pieces(B):
+    """More CTAs than start at once: the longest sequences come first, equal and empty ones among them."""
+    from kascade_b200 import _native as nat
+    G, splits = 8, 9
+    g = torch.Generator().manual_seed(B)
+    lens = [int(x) for x in torch.randint(0, 400, (B,), generator=g)]
+    lens[0] = lens[B - 1] = 333
+    lens[B // 2] = 0
+    k, v, kp, vp, table, kf, vf, vc = make_cache(lens, G, 16, seed=95)
+    q = _queries(B, 4 * G, torch.float16, 96)
+    stride = 400
+    logits, pooled = torch.zeros(B, 4 * G, stride, device="cuda"), torch.zeros(B, G, stride, device="cuda")
+    out, lse = torch.empty(B, 4 * G, 128, dtype=torch.float16, device="cuda"), torch.zeros(B, 4 * G, device="cuda")
+    seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    kv = nat.kv_layout_paged(k, v, table, kp, vp)
+    nat.decode_anchor_paged(q, kv, seq, 400, 128 ** -0.5, logits, pooled, out, lse, nat.decode_workspace(B, 4 * G, splits, q.device), splits)
+    _check_attention(out, lse, q, kf, vf, vc, lambda b, h: list(range(lens[b])), 128 ** -0.5, torch.float16, f"{B} ragged sequences")
+    for b in (0, B // 2, B - 1):
+        assert bool((logits[b, :, lens[b]:] == 0).all()) and bool((pooled[b, :, lens[b]:] == 0).all())
