@@ -422,8 +422,9 @@ def kv_layout_paged(k_cache: torch.Tensor, v_cache: Optional[torch.Tensor], bloc
     assert block_table.dtype is torch.int32 and ts[1] == 1
     if v_cache is not None:
         assert v_cache.shape == k_cache.shape and v_cache.stride() == st and v_cache.dtype is k_cache.dtype
-    layout = KvLayout(k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2],
-                      block_table.data_ptr(), ts[0], k_cache.shape[1], code)
+    layout = KvLayout.from_buffer_copy(_LAYOUT.pack(
+        k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), 0, st[0], st[1], st[2], block_table.data_ptr(), ts[0],
+        k_cache.shape[1], code, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))
     layout._keep = (k_cache, block_table) if v_cache is None else (k_cache, v_cache, block_table)
     return layout
 
@@ -828,8 +829,7 @@ def evict(mass, layers, seq_lens, budget: int, recent: int, sinks: int, token_po
     dev = mass.device
     if not mass.numel():
         return torch.zeros_like(seq_lens), torch.empty_like(mass), torch.empty(B, rows, dtype=torch.int32, device=dev)
-    lens = torch.empty(B, dtype=torch.int32, device=dev)
-    mass_out = torch.empty(B, rows, dtype=torch.float32, device=dev)
+    lens, mass_out = torch.empty_like(seq_lens), torch.empty_like(mass, memory_format=torch.contiguous_format)
     pos_out = torch.empty(B, rows, dtype=torch.int32, device=dev)
     size = lib.kb200_evict_workspace_bytes(B, rows, budget)
     workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)

@@ -657,9 +657,9 @@ class EfficientKascadeStrategy(Strategy):
         if block_table.shape[0] != B:
             raise ValueError(f"block_table has rows for {block_table.shape[0]} sequences, seq_lens for {B}")
         kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, dtype)
-        out = torch.empty(2, B, max_seq_len, G, nat.HEAD_DIM, dtype=dtype, device=key_cache.device)
-        nat.kv_read(kv, seq_lens, out[0], out[1])
-        return out[0], out[1]
+        key, value = torch.empty(2, B, max_seq_len, G, nat.HEAD_DIM, dtype=dtype, device=key_cache.device).unbind()
+        nat.kv_read(kv, seq_lens, key, value)
+        return key, value
 
     @staticmethod
     def prompt_mass(pooled, attention_mass, seq_lens=None) -> torch.Tensor:
