@@ -17,70 +17,84 @@ struct PromptMassParams {
   int G, T, n_rows;
 };
 
-// 128 rows of the cache, four per lane, are a block; the pooled scores of a block are one piece of 512 bytes per head and later
-// tile, which a cluster of CTAs deals to its warps, eight loads in flight each.  The first rows have the most later tiles and the
+// 256 rows of the cache, twice four per lane, are a block; the pooled scores of a block are one piece of 1024 bytes per head and later
+// tile, which a cluster of CTAs deals to its warps, four pieces in flight each.  The first rows have the most later tiles and the
 // last none, so a cluster takes the i-th block from the front and the i-th from the back: equal work everywhere.  A lane
 // adds its pieces up one after the other, the warps' and the CTAs' sums meet in the order of their numbers, so a call
-// gives the same bits every time.
+// gives the same bits every time.  us with 128 / 256 / 512 rows in a block: one prompt of 32768 rows 94.6 / 90.9 / 88.3, 16384 30.6 / 28.7
+// / 35.8, 8192 13.6 / 14.6 / 19.8, 8 x 4096 18.8 / 17.8 / 18.7.
 constexpr int kMassWarps = 16;
-constexpr int kMassUnroll = 8;
+constexpr int kMassVec = 2;                                       // pieces of 512 bytes beside each other that a warp reads at once
+constexpr int kMassUnroll = 4;
+constexpr int kMassRows = 128 * kMassVec;                         // of a block
 __global__ void __launch_bounds__(kMassWarps * 32) mass_prompt_kernel(const PromptMassParams p) {
   namespace cg = cooperative_groups;
   pdl_begin();
-  __shared__ float4 sums[kMassWarps][32];
-  __shared__ float total[2][128];
+  __shared__ float4 sums[kMassWarps][kMassVec * 32];
+  __shared__ float total[2][kMassRows];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tiles = p.seq_len ? min((max(p.seq_len[b], 0) + kTile - 1) / kTile, p.T) : p.T;
-  const int blocks = (p.n_rows + 127) / 128, front = blockIdx.x / ctas, back = blocks - 1 - front;
+  const int blocks = (p.n_rows + kMassRows - 1) / kMassRows, front = blockIdx.x / ctas, back = blocks - 1 - front;
 #pragma unroll 1
   for (int half = 0; half < 2; ++half) {
     const int block = half ? back : front;
-    const int j = block * 128 + lane * 4, own = j / kTile;         // (the same tile for a lane's four rows)
-    const int first = block * 4 + 1;                                // the first tile behind the first of these rows
+    const int j = block * kMassRows + lane * 4;
+    const int first = block * (kMassRows / kTile) + 1;              // the first tile behind the first of these rows
     const int later = half && back == front ? 0 : max(tiles - first, 0), pieces = later * p.G, step = ctas * kMassWarps;
     const float* rows = p.pooled + (int64_t)b * p.G * p.T * p.row_stride + j;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 a[kMassVec];
+#pragma unroll
+    for (int v = 0; v < kMassVec; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = rank * kMassWarps + warp; i0 < pieces; i0 += step * kMassUnroll) {
-      float4 x[kMassUnroll];
+      float4 x[kMassUnroll][kMassVec];
 #pragma unroll
       for (int u = 0; u < kMassUnroll; ++u) {
         const int i = i0 + u * step, g = i / later, t = first + i - g * later;
-        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < pieces && t > own) x[u] = *reinterpret_cast<const float4*>(rows + ((int64_t)g * p.T + t) * p.row_stride);
+        const float* src = rows + ((int64_t)g * p.T + t) * p.row_stride;
+#pragma unroll
+        for (int v = 0; v < kMassVec; ++v) {
+          x[u][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i < pieces && t > (j + v * 128) / kTile) x[u][v] = *reinterpret_cast<const float4*>(src + v * 128);
+        }
       }
 #pragma unroll
-      for (int u = 0; u < kMassUnroll; ++u) { a.x += x[u].x; a.y += x[u].y; a.z += x[u].z; a.w += x[u].w; }
+      for (int u = 0; u < kMassUnroll; ++u)
+#pragma unroll
+        for (int v = 0; v < kMassVec; ++v) { a[v].x += x[u][v].x; a[v].y += x[u][v].y; a[v].z += x[u][v].z; a[v].w += x[u][v].w; }
     }
-    sums[warp][lane] = a;
+#pragma unroll
+    for (int v = 0; v < kMassVec; ++v) sums[warp][v * 32 + lane] = a[v];
     __syncthreads();
-    if (threadIdx.x < 128) {
+    for (int i = threadIdx.x; i < kMassRows; i += kMassWarps * 32) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < kMassWarps; ++w) s += reinterpret_cast<const float*>(sums[w])[threadIdx.x];
-      total[half][threadIdx.x] = s;
+      for (int w = 0; w < kMassWarps; ++w) s += reinterpret_cast<const float*>(sums[w])[i];
+      total[half][i] = s;
     }
     __syncthreads();
   }
   cluster.sync();
-  const int half = threadIdx.x >> 7, at = threadIdx.x & 127;
-  if (rank == 0 && half < (back == front ? 1 : 2)) {
-    float s = total[half][at];
-    for (int r = 1; r < ctas; ++r) s += cluster.map_shared_rank(&total[0][0], r)[half * 128 + at];
-    const int i = (half ? back : front) * 128 + at;
-    if (i < p.n_rows) p.mass_out[b * p.out_stride + i] = p.mass_in[b * p.in_stride + i] + s;
+  if (rank == 0) {
+    for (int i0 = threadIdx.x; i0 < kMassRows * (back == front ? 1 : 2); i0 += kMassWarps * 32) {
+      const int half = i0 / kMassRows, at = i0 - half * kMassRows;
+      float s = total[half][at];
+      for (int r = 1; r < ctas; ++r) s += cluster.map_shared_rank(&total[0][0], r)[half * kMassRows + at];
+      const int i = (half ? back : front) * kMassRows + at;
+      if (i < p.n_rows) p.mass_out[b * p.out_stride + i] = p.mass_in[b * p.in_stride + i] + s;
+    }
   }
   cluster.sync();                                                  // the sums have been read
 }
 
 // CTAs that share two blocks: doubled while all of them together are at most two per SM.  512 threads with eight loads each
-// keep enough in flight then, and a second round of CTAs would leave SMs idle at its end.  us with at most two / four CTAs per
-// SM: one prompt of 32768 rows 95 / 102 (5.7 TB/s, 0.88 of the copy), 16384 30.5 / 38.4, 8192 13.8 / 13.6, 8 x 4096 18.8 / 24.6,
-// 4 x 3001 11.9 / 17.3.  (A thread per four rows, over all heads and tiles: 1995 us for 32768 rows.)
+// keep enough in flight then, and a second round of CTAs would leave SMs idle at its end (with blocks of 128 rows and at most two
+// / four CTAs per SM: one prompt of 32768 rows 95 / 102 us, 16384 30.5 / 38.4, 8192 13.8 / 13.6, 8 x 4096 18.8 / 24.6, 4 x 3001 11.9 /
+// 17.3).  32768 rows: 5.9 TB/s, 0.92 of the copy.  (A thread per four rows, over all heads and tiles: 1995 us.)
 static int mass_ctas(int64_t clusters) {
   int c = 1;
-  while (c < 8 && clusters * c <= sm_count()) c *= 2;
+    while (c < 8 && clusters * c <= sm_count()) c *= 2;
   return c;
 }
 
@@ -253,7 +267,7 @@ extern "C" int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, co
   KB_REQUIRE(n_rows >= need, "mass_add_prompt: mass holds %d rows, %d tiles need %lld", n_rows, num_tiles, (long long)need);
   if (batch == 0 || n_rows == 0) return 0;
   PromptMassParams p{pooled, row_stride, seq_len, mass_in, mass_out, mass_in_stride, mass_out_stride, num_kv_heads, num_tiles, n_rows};
-  const int clusters = ceil_div(n_rows, 256), ctas = mass_ctas((int64_t)clusters * batch);
+  const int clusters = ceil_div(n_rows, 2 * kMassRows), ctas = mass_ctas((int64_t)clusters * batch);
   KB_LAUNCH("mass_prompt_kernel", launch_pdl(mass_prompt_kernel, dim3(clusters * ctas, batch), kMassWarps * 32, 0, (cudaStream_t)stream,
                                              ctas, p));
   return 0;
