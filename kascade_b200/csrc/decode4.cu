@@ -29,10 +29,18 @@ constexpr int kKeys4 = 32;                                 // keys of a step, on
 constexpr int kCodes4 = kKeys4 * kD / 2;                   // bytes of the codes of a step's K or V rows
 constexpr int kHalf4 = kCodes4 + kKeys4 * 16;              // ... with their parameters
 constexpr int kCodeOne = 1 << 24;                          // 1 / (the value of code 1 as an fp16 subnormal)
-// A row's reference point for its exponentials moves only when a logit exceeds it by more than 2^kSlack4: probabilities are at
-// most 4, so that their products with a scale (s <= 8734) stay in fp16's range, and the maximum over the lanes, the
-// factors and the rescaling of O are needed in a few steps per list only.
-constexpr float kSlack4 = 2.f;
+// A row's reference point for its exponentials lies kBase4 below the largest logit (in units of log2) when it is set, and moves only
+// when a logit exceeds it by more than kTop4: the maximum over the lanes, the factors and the rescaling of O are needed in a
+// few steps per list only.  So the probabilities p are at most 2^13 and the largest of a warp is 2^11 at least, and fp16 holds
+// all that are more than 2^-25 of the largest with all of its bits.
+constexpr float kBase4 = 11.f, kTop4 = 13.f;
+// Scales get a power of two of their own, per warp and group: 2^up brings the largest scale so far to [2, 4), so that p s 2^up stays
+// below 2^15 and, like p, keeps its bits down to 2^-26 of the largest, whatever the size of V.  It moves as the reference does.
+// (Without it p s falls below 2^-14, where fp16 has steps of 2^-24, wherever V is small or one key dominates: for 8192 keys with
+// one 9 above the others and V of a standard deviation of 0.03 outputs were off by 17 %.)  Scales below 2^-15 are taken
+// times 2^15, the largest power of two in fp16.
+constexpr int kMaxUp4 = 15;
+constexpr float kUnbase4 = 1.f / 2048.f;                   // 2^-kBase4: the results are relative to the largest logit again
 // The tensor core rounds its sums towards zero: by about 2^-24 of the accumulator per product, always the same way.  The codes' mean
 // is 7.5, so their share of O grows with the list while O itself, with the zeros' share taken off, does not: after 512 products that
 // was 0.4 % of O for 131072 keys.  (And it aligns products by their operands' exponent fields, so a subnormal loses what it lies below
@@ -239,6 +247,7 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
     for (int i = 0; i < 4; ++i) o_acc[e][0][i] = o_acc[e][1][i] = 0.f;
   }
   float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
+  int up = grp < 4 ? kMaxUp4 : 0;                                // lane (e, quad): the power of two of group e's scales (the zeros have none)
   float* track = reinterpret_cast<float*>(smem + WARPS * (kStages * kStage) + warp * kTrackBytes4) + lane;   // [10], 32 apart
   if (HAS_V) {
 #pragma unroll
@@ -261,9 +270,9 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
     }
   };
 
-  // p s in fp16 for columns 0-3, and for columns 4-7 (the same heads) what its rounding left, exactly: the products with the
-  // codes, whose mean is far from zero, would carry the rounding of p s twice as far as that of p.  bf16 outputs are rounded
-  // ten times as coarsely and do without.
+  // p s in fp16 for columns 0-3, and for columns 4-7 (the same heads) what its rounding left (exactly where p s, which goes up to 2^15,
+  // is 2^-3 or more): the products with the codes, whose mean is far from zero, would carry the rounding of p s twice as far as
+  // that of p.  bf16 outputs are rounded ten times as coarsely and do without.
   const uint32_t rest = grp < kHg ? 0u : 0xFFFFFFFFu;
   auto scaled = [&](uint32_t pb, uint32_t s) -> uint32_t {
     const uint32_t ps = mul_half2(pb, s);
@@ -327,29 +336,49 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
     }
     // ---- exponentials against the reference of either head ---------------------------------------------
     float t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])), t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
-    if (__any_sync(FULL, t0 > m_run[0] + kSlack4 || t1 > m_run[1] + kSlack4)) {     // (the first step: it has a valid key)
+    uint32_t z[2][2];                                        // lane (r, quad): parameter r of keys 2 quad, 2 quad + 1 / + 8 of either 16
+    __half2 top = __half2half2(__ushort_as_half(0));
+    if (HAS_V) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ldmatrix_x2_trans(z[i][0], z[i][1], buf + kHalf4 + kCodes4 + i * 256 + (lane & 15) * 16);
+        top = __hmax2(top, __hmax2(__habs2(*reinterpret_cast<__half2*>(&z[i][0])), __habs2(*reinterpret_cast<__half2*>(&z[i][1]))));
+      }
+    }
+    // (a scale of 2^(2 - up) or more; the first step moves in any case: it has a valid key)
+    const bool grown = HAS_V && grp < 4 && !__hblt2(top, __half2half2(__float2half_rn(__uint_as_float((uint32_t)(129 - up) << 23))));
+    if (__any_sync(FULL, grown || t0 > m_run[0] + kTop4 || t1 > m_run[1] + kTop4)) {
 #pragma unroll
       for (int sh = 4; sh <= 16; sh <<= 1) {
         t0 = fmaxf(t0, __shfl_xor_sync(FULL, t0, sh));
         t1 = fmaxf(t1, __shfl_xor_sync(FULL, t1, sh));
       }
-      const float m0 = t0 > m_run[0] + kSlack4 ? t0 : m_run[0], m1 = t1 > m_run[1] + kSlack4 ? t1 : m_run[1];
+      const float m0 = t0 > m_run[0] + kTop4 ? t0 - kBase4 : m_run[0], m1 = t1 > m_run[1] + kTop4 ? t1 - kBase4 : m_run[1];
       const float alpha0 = ex2(m_run[0] - m0), alpha1 = ex2(m_run[1] - m1);
       m_run[0] = m0;
       m_run[1] = m1;
       l_part[0] *= alpha0;
       l_part[1] *= alpha1;
       if (HAS_V) {
+        float s_top = fmaxf(__low2float(top), __high2float(top));
+        s_top = fmaxf(s_top, __shfl_xor_sync(FULL, s_top, 1));
+        s_top = fmaxf(s_top, __shfl_xor_sync(FULL, s_top, 2));
+        const int to = grp < 4 ? max(min(up, 128 - (int)(__float_as_uint(s_top) >> 23)), -14) : up;
+        const float ratio = __uint_as_float((uint32_t)(127 + to - up) << 23);
+        up = to;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+          const float r = __shfl_sync(FULL, ratio, e * 4 + quad), r0 = alpha0 * r, r1 = alpha1 * r;
 #pragma unroll
           for (int f = 0; f < 2; ++f) {
-            o_acc[e][f][0] *= alpha0; o_acc[e][f][1] *= alpha1; o_acc[e][f][2] *= alpha0; o_acc[e][f][3] *= alpha1;
+            o_acc[e][f][0] *= r0; o_acc[e][f][1] *= r1; o_acc[e][f][2] *= r0; o_acc[e][f][3] *= r1;
           }
+          track[(2 * e) * 32] *= r0;
+          track[(2 * e + 1) * 32] *= r1;
         }
         o_zero[0] *= alpha0; o_zero[1] *= alpha1;
-#pragma unroll
-        for (int i = 0; i < kTracks4; ++i) track[i * 32] *= i & 1 ? alpha1 : alpha0;
+        track[8 * 32] *= alpha0;
+        track[9 * 32] *= alpha1;
       }
     }
     float w[2][4];
@@ -362,13 +391,15 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
     l_part[1] += (w[0][1] + w[0][3]) + (w[1][1] + w[1][3]);
     if (HAS_V) {
       // ---- O^T += V^T P^T -------------------------------------------------------------------------------
+      const __half up_h = __float2half_rn(__uint_as_float((uint32_t)(127 + up) << 23));
+      const __half2 up2_h = __half2half2(up_h);
+      const uint32_t up2 = *reinterpret_cast<const uint32_t*>(&up2_h);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         // B operand P^T[key][head]: column = head grp, rows = keys 2 quad, 2 quad + 1 (pb0) and + 8 (pb1)
         const uint32_t pb0 = movmatrix_trans(pack_half2<false>(w[i][0], w[i][1]));
         const uint32_t pb1 = movmatrix_trans(pack_half2<false>(w[i][2], w[i][3]));
-        uint32_t z0, z1;                                       // lane (r, quad): parameter r of keys 2 quad, 2 quad + 1 / + 8
-        ldmatrix_x2_trans(z0, z1, buf + kHalf4 + kCodes4 + i * 256 + (lane & 15) * 16);
+        const uint32_t z0 = mul_half2(z[i][0], up2), z1 = mul_half2(z[i][1], up2);
         mma16816<false>(o_zero, z0, 0u, z1, 0u, pb0, pb1);
         const uint32_t v = buf + kHalf4 + i * 1024 + v_at;
         const uint2 ka = lds64(v), kb = lds64(v ^ 64u), kc = lds64(v + 512), kd = lds64((v + 512) ^ 64u);
@@ -413,7 +444,7 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
   float* sm_m = reinterpret_cast<float*>(smem);                  // [warps][4]
   float* sm_l = sm_m + WARPS * kHg;                              // [warps][4]
   float* sm_o = sm_l + WARPS * kHg;                              // [warps][4][128]
-  float zero[4][2];
+  float zero[4][2], unit[4];                                     // what group e's sums of p s c are multiplied by in the end
   if (HAS_V && !BF16) {                                          // the rests, columns 4-7, to their heads
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -427,23 +458,24 @@ __global__ void __launch_bounds__(kWarps4 * 32, 1) decode_attn4_kernel(const Dec
   if (HAS_V) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      zero[e][0] = __shfl_sync(FULL, o_zero[0], (4 + e) * 4 + quad);
-      zero[e][1] = __shfl_sync(FULL, o_zero[1], (4 + e) * 4 + quad);
+      zero[e][0] = __shfl_sync(FULL, o_zero[0], (4 + e) * 4 + quad) * kUnbase4;
+      zero[e][1] = __shfl_sync(FULL, o_zero[1], (4 + e) * 4 + quad) * kUnbase4;
+      unit[e] = __uint_as_float((uint32_t)(127 + 22 - (int)kBase4 - __shfl_sync(FULL, up, e * 4 + quad)) << 23);
     }
   }
   if (quad < 2) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int h = quad * 2 + r;
-      if (grp == 0) { sm_m[warp * kHg + h] = m_run[r]; sm_l[warp * kHg + h] = l_part[r]; }
+      if (grp == 0) { sm_m[warp * kHg + h] = m_run[r] + kBase4; sm_l[warp * kHg + h] = l_part[r] * kUnbase4; }
       if (HAS_V) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float4 o;
-          o.x = fmaf(o_acc[e][0][r], (float)(kCodeOne / 4), zero[e][r]);
-          o.y = fmaf(o_acc[e][0][2 + r], (float)(kCodeOne / 64), zero[e][r]);
-          o.z = fmaf(o_acc[e][1][r], (float)(kCodeOne / 4), zero[e][r]);
-          o.w = fmaf(o_acc[e][1][2 + r], (float)(kCodeOne / 64), zero[e][r]);
+          o.x = fmaf(o_acc[e][0][r], unit[e], zero[e][r]);
+          o.y = fmaf(o_acc[e][0][2 + r], unit[e] / 16, zero[e][r]);
+          o.z = fmaf(o_acc[e][1][r], unit[e], zero[e][r]);
+          o.w = fmaf(o_acc[e][1][2 + r], unit[e] / 16, zero[e][r]);
           *reinterpret_cast<float4*>(sm_o + (warp * kHg + h) * kD + 32 * e + 4 * grp) = o;
         }
       }
