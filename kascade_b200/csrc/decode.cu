@@ -48,8 +48,14 @@ __device__ __forceinline__ uint32_t swz8(int r, int c) { return (uint32_t)(r * 1
 //     (V[2q][d], V[2q][d+1], V[2q+1][d], V[2q+1][d+1]); a byte permute splits that into the operand of the
 //     even and of the odd columns, so a lane ends up with 4 contiguous d per 16-byte chunk.
 // The scales are applied in fp32 where a row's contribution appears: on the logit of its key and on its
-// probability before P.V.  q and the output are fp16 then.
+// probability before P.V.  q and the output are fp16 then.  The product of a probability and V's scale is an operand in fp16:
+// scales are taken times a power of two that brings the largest of the warp so far to [2^14, 2^15), so that products keep their
+// bits down to 2^-28 of the largest, however small V is (as they are, they would lie below 2^-14, where fp16 has steps of 2^-24,
+// wherever V is small or one key dominates).  Powers of two leave results as they are where nothing was lost before.
 constexpr int kRawStage = kSub * kD * 2;                  // FP8: K + V rows of a sub-tile as stored (4 KB)
+constexpr int kTop8 = 14, kMaxUp8 = 100;
+__device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // the two 16-bit halves of a word of e4m3 bytes -> two fp16 pairs
 __device__ __forceinline__ void fp8x4_to_half2x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -218,6 +224,7 @@ __global__ void __launch_bounds__(dec_warps(KV) * 32, 1) decode_attn_kernel(cons
 #pragma unroll
   for (int i = 0; i < 8; ++i) { o_acc[i][0] = o_acc[i][1] = o_acc[i][2] = o_acc[i][3] = 0.f; }
   float m_run[2] = {-INFINITY, -INFINITY}, l_part[2] = {0.f, 0.f};
+  int sv_up = kMaxUp8;                   // FP8: V's scales are taken times 2^sv_up
 
   for (int j = 0; j < my_count; ++j) {
     __syncwarp();                      // every lane is done with the buffer about to be refilled
@@ -289,18 +296,25 @@ __global__ void __launch_bounds__(dec_warps(KV) * 32, 1) decode_attn_kernel(cons
     l_part[0] = l_part[0] * alpha0 + (p0 + p2);
     l_part[1] = l_part[1] * alpha1 + (p1 + p3);
     if (HAS_V) {
+      float r0 = alpha0, r1 = alpha1;
       if (FP8) {                                 // P.V sees the stored values: the rows' scales go on the probabilities
-        const float va = __shfl_sync(FULL, sv0, grp), vb = __shfl_sync(FULL, sv0, grp + 8);
+        if (__any_sync(FULL, exponent(sv0) + sv_up > kTop8)) {       // (a first scale of 2^-85 or more: always)
+          const int to = max(min(sv_up, kTop8 - __reduce_max_sync(FULL, exponent(sv0))), -kMaxUp8);
+          const float r = pow2(max(to - sv_up, -126));
+          r0 *= r; r1 *= r;
+          sv_up = to;
+        }
+        const float sv = sv0 * pow2(sv_up), va = __shfl_sync(FULL, sv, grp), vb = __shfl_sync(FULL, sv, grp + 8);
         p0 *= va; p1 *= va; p2 *= vb; p3 *= vb;
       }
       // B operand P^T[key][head]: column = head grp, rows = keys 2q, 2q+1 (b0) and 2q+8, 2q+9 (b1)
       const uint32_t pb0 = movmatrix_trans(pack_half2<BF16>(p0, p1));
       const uint32_t pb1 = movmatrix_trans(pack_half2<BF16>(p2, p3));
       // ---- O^T = O^T * alpha + V^T P^T : 8 d-tiles of 16 -----------------------------------------
-      if (!__all_sync(FULL, alpha0 == 1.f && alpha1 == 1.f)) {         // a factor of exactly 1 changes nothing
+      if (!__all_sync(FULL, r0 == 1.f && r1 == 1.f)) {                 // a factor of exactly 1 changes nothing
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-          o_acc[t][0] *= alpha0; o_acc[t][1] *= alpha1; o_acc[t][2] *= alpha0; o_acc[t][3] *= alpha1;
+          o_acc[t][0] *= r0; o_acc[t][1] *= r1; o_acc[t][2] *= r0; o_acc[t][3] *= r1;
         }
       }
       if (FP8) {
@@ -356,8 +370,8 @@ __global__ void __launch_bounds__(dec_warps(KV) * 32, 1) decode_attn_kernel(cons
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
           const int d_lo = FP8 ? t * 16 + grp * 2 : t * 16 + grp;
-          dst[d_lo] = o_acc[t][e];
-          dst[d_lo + (FP8 ? 1 : 8)] = o_acc[t][2 + e];
+          dst[d_lo] = FP8 ? o_acc[t][e] * pow2(-sv_up) : o_acc[t][e];
+          dst[d_lo + (FP8 ? 1 : 8)] = FP8 ? o_acc[t][2 + e] * pow2(-sv_up) : o_acc[t][2 + e];
         }
       }
     }
