@@ -260,6 +260,29 @@ class EfficientKascadeStrategy(Strategy):
             self._map_dev[key] = m
         return m
 
+    def _decode_mapping(self, layer_idx: int, num_kv_heads: int, device) -> torch.Tensor:
+        """[G] int32: the row of a decode step's [B,G,k] index rows that each KV head of a reuse layer reads.  A sharded strategy's
+        steps hold the rows of this rank's heads only (prompts gather all), so its mapping must stay among them."""
+        key = (layer_idx, num_kv_heads, device)
+        m = self._map_dev.get(key)
+        if m is None:
+            row, first = [int(h) for h in self._head_mapping[layer_idx]], 0
+            if self._shard is not None and self._shard[1] > 1:
+                rank, world = self._shard
+                if len(row) != num_kv_heads * world:
+                    raise ValueError(f"layer {layer_idx}: the mapping has {len(row)} KV heads, {world} ranks of {num_kv_heads} were expected")
+                first = rank * num_kv_heads
+                row = row[first:first + num_kv_heads]
+                away = [h for h in row if not first <= h < first + num_kv_heads]
+                if away:
+                    raise NotImplementedError(f"layer {layer_idx} reads the index rows of KV heads {away}, which another rank selects: decode "
+                                              "steps of a sharded strategy do not exchange index rows")
+            row = [h - first for h in row]
+            if len(row) < num_kv_heads or not all(0 <= h < num_kv_heads for h in row[:num_kv_heads]):
+                raise ValueError(f"layer {layer_idx}: the mapping {row} does not fit a cache of {num_kv_heads} KV heads")
+            m = self._map_dev[key] = torch.tensor(row, dtype=torch.int32, device=device)
+        return m
+
     @staticmethod
     def _token_major(x: torch.Tensor) -> torch.Tensor:
         """[B, heads, L, D] -> a [B, L, heads, D] view with D contiguous and 16-byte aligned strides."""
@@ -602,7 +625,7 @@ class EfficientKascadeStrategy(Strategy):
         else:
             if self._dec_idx is None and index_rows is None:
                 raise RuntimeError("reuse layer called before any anchor layer")
-            head_map = self._mapping(layer, dev)
+            head_map = self._decode_mapping(layer, G, dev)
         rows, counts = (self._dec_idx, self._dec_count) if index_rows is None else index_rows
         kmax = rows.shape[2]
         splits = self._splits(B, G, kmax, 1.0 if int4 else ragged, dev)
@@ -714,9 +737,10 @@ class EfficientKascadeStrategy(Strategy):
         either type.  `attention_mass` [B, rows >= max_seq_len] fp32: anchor layers add to it, in place, the attention that each
         row draws, summed over the heads (reuse layers do not see all rows and leave it as it is); ``evict_kv`` chooses by it.
         `index_rows` = (rows [B,G,k] int32, counts [B,G] int32): a reuse layer attends to these rows (of the KV head its mapping
-        names) instead of the last anchor layer's, for a layer whose anchor runs elsewhere.  `mean_seq_len` is a hint of the
-        host for batches of very different lengths (the work is then cut into more, smaller pieces); results do not depend
-        on it beyond summation order.
+        names) instead of the last anchor layer's, for a layer whose anchor runs elsewhere.  In a sharded strategy key / value
+        cache, queries and index rows are those of this rank's KV heads, and a reuse layer whose mapping names another rank's
+        head is refused.  `mean_seq_len` is a hint of the host for batches of very different lengths (the work is then cut
+        into more, smaller pieces); results do not depend on it beyond summation order.
         The reference has no paged kernel (README.md:135); the nearest signature is
         kernels/flash_decoding/reuse_kascade_gqa_decode_with_kvcache.py:160-171."""
         if max_seq_len is None:
@@ -735,6 +759,8 @@ class EfficientKascadeStrategy(Strategy):
                     or rows.get_device() != where or counts.get_device() != where:
                 raise ValueError(f"index_rows must be int32 [{want[0]}, {want[1]}, k], the last dimension contiguous, and contiguous "
                                  f"int32 counts {want} on {query.device}, got {tuple(rows.shape)} and {tuple(counts.shape)}")
+        if self._shard is not None and not self.is_anchor(int(layer_idx)):
+            self._decode_mapping(int(layer_idx), key_cache.shape[2], query.device)       # refuses before anything is launched
         kv = nat.kv_layout_paged(key_cache, value_cache, block_table, k_scale, v_scale, query.dtype)
         return self._decode(int(layer_idx), query, kv, seq_lens, int(max_seq_len), scaling, key_cache.shape[2],
                             mean_len=mean_seq_len, mass=attention_mass, index_rows=index_rows)
