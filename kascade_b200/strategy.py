@@ -627,7 +627,9 @@ class EfficientKascadeStrategy(Strategy):
                 raise RuntimeError("reuse layer called before any anchor layer")
             head_map = self._decode_mapping(layer, G, dev)
         rows, counts = (self._dec_idx, self._dec_count) if index_rows is None else index_rows
-        kmax = rows.shape[2]
+        rows_b, rows_g, kmax = rows.shape
+        if rows_b != B or rows_g != G:
+            raise RuntimeError(f"the last anchor layer selected rows for {rows_b} sequences of {rows_g} KV heads, this layer has {B} of {G}")
         splits = self._splits(B, G, kmax, 1.0 if int4 else ragged, dev)
         ws = self._scratch("dec_ws_s", (nat.decode_workspace_bytes(B, H, splits),), torch.uint8, dev)
         nat.decode_sparse_paged(q, kv, rows, counts, kmax, head_map, scaling, out, None, ws, splits)

@@ -37,3 +37,15 @@ def test_reuse_layers_read_the_rows_of_the_ranks_own_heads(own_rows):
         for layer in range(2):
             want = whole[layer].view(2, G, 4, 128)[:, 2 * rank:2 * rank + 2].reshape(2, -1, 128)
             assert_close(part[layer], want.float(), what=f"rank {rank}, layer {layer}")
+
+
+def test_rows_of_a_smaller_batch_are_refused():
+    """A reuse layer whose anchor ran for fewer sequences or heads has no rows of its own."""
+    from kascade_b200 import EfficientKascadeStrategy
+    k, v, kp, vp, table, *_ = make_cache([200, 300, 250], 2, 16, seed=9)
+    strat = EfficientKascadeStrategy([0], "x/y", k=20, tile_size=32, head_mapping=[[0, 1]] * 2, register=False)
+    seq, q = torch.tensor([200, 300, 250], dtype=torch.int32, device="cuda"), torch.zeros(3, 8, 128, dtype=torch.float16, device="cuda")
+    strat.paged_decode_forward(0, q[:2], k, v, table[:2], seq[:2], 0.1, 300, kp, vp)
+    with pytest.raises(RuntimeError, match="2 sequences"):
+        strat.paged_decode_forward(1, q, k, v, table, seq, 0.1, 300, kp, vp)
+    strat.paged_decode_forward(1, q[:2], k, v, table[:2], seq[:2], 0.1, 300, kp, vp)
