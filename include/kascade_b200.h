@@ -454,10 +454,14 @@ int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t
                           int num_tiles, int n_rows, void* stream);
 
 /* Shortens every sequence of a cache to at most `budget` rows, in all layers alike: those with the largest mass[b, j] stay
- * (j < seq_lens[b] and j < n_rows; a NaN counts as 0, an infinite weight as the largest number; ties go to the lowest row), and in any case the rows whose token position is below
- * `sinks` or within the last `recent` of the sequence's positions.  Kept rows below the new length stay where they are, those
- * behind it fill the rows that were let go, the lowest into the lowest: the smallest number of moves, and no row is both source
- * and target.  (The order of rows in a cache has no meaning to attention: positions are in the keys' rotation.)
+ * (j < seq_lens[b] and j < n_rows; a NaN counts as 0, an infinite weight as the largest number; ties go to the lowest row), and in any
+ * case the protected rows, whose token position is in 0 .. `sinks` - 1 or within the last `recent` of the sequence's positions.
+ * Where rows share positions (images on several axes) more rows can be protected than the budget holds: then the lowest `sinks` rows
+ * of the first positions stay and the recent rows, the newest position first (ties: the lowest row), so that the last `recent`
+ * rows in the order of positions are among them.  (Where the newest position alone has more rows than the budget, the
+ * lowest of all protected rows stay.)  A negative position is no first one: -1 stands for rows whose position was never noted.
+ * Kept rows below the new length stay where they are, those behind it fill the rows that were let go, the lowest into the
+ * lowest: the smallest number of moves, and no row is both source and target.  (The order of rows in a cache has no meaning to attention: positions are in the keys' rotation.)
  *   layers     host array of n_layers layouts, fp16 / bf16 or INT4, of one type, block table and set of strides (an FP8 cache has
  *              one scale per page, so its rows cannot leave their page: refused); changed in place.  The pages below the new
  *              length must belong to one sequence alone

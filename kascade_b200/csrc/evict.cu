@@ -4,6 +4,7 @@
 #include <cooperative_groups.h>
 
 #include <cfloat>
+#include <climits>
 
 #include "common.cuh"
 
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kMassWarps * 32) mass_prompt_kernel(const Prom
 // 17.3).  32768 rows: 5.9 TB/s, 0.92 of the copy.  (A thread per four rows, over all heads and tiles: 1995 us.)
 static int mass_ctas(int64_t clusters) {
   int c = 1;
-    while (c < 8 && clusters * c <= sm_count()) c *= 2;
+  while (c < 8 && clusters * c <= sm_count()) c *= 2;
   return c;
 }
 
@@ -103,41 +104,107 @@ static int mass_ctas(int64_t clusters) {
 // largest number, so that it stays behind the protected rows).  A cluster of CTAs
 // takes a sequence: the newest position first, over all of it, then the keys of its piece.  Latency is what counts: 4 sequences of 32768
 // rows 20.6 us with one CTA each, 7.8 with eight.
+// Rows that share a position (images on several axes) can be more than the budget holds.  Then the lowest `sinks` rows of the first
+// positions get +inf, the recent ones a key that falls with their distance from the newest position, above all weights: the last
+// `recent` rows in the order of positions stay in any case.  Only where the newest position alone has more rows than
+// the budget do all protected rows count alike.
 constexpr int kKeyThreads = 1024;
 struct EvictKeysParams {
   const float* mass; int64_t mass_stride;
   const int32_t* seq_lens;
   const int32_t* positions; int64_t pos_stride;
   float* keys; int64_t key_stride;
-  int sinks, recent, n_rows;
+  int sinks, recent, budget, n_rows;
 };
+
+// Sums of N numbers of each thread over the cluster.  All its threads call it.
+template <int N>
+__device__ __forceinline__ void cluster_sums(int (&v)[N], int (*of_warp)[32], int* of_cta) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = __reduce_add_sync(0xFFFFFFFFu, v[i]);
+    if ((tid & 31) == 0) of_warp[i][tid >> 5] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = __reduce_add_sync(0xFFFFFFFFu, of_warp[i][tid & 31]);
+    if (tid == 0) of_cta[i] = v[i];
+  }
+  cluster.sync();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0;
+    for (int r = 0; r < (int)cluster.num_blocks(); ++r) v[i] += cluster.map_shared_rank(of_cta, r)[i];
+  }
+  cluster.sync();                                                 // the others have read this CTA's sums
+}
+
 __global__ void __launch_bounds__(kKeyThreads) evict_keys_kernel(const EvictKeysParams p) {
   namespace cg = cooperative_groups;
   pdl_begin();
-  __shared__ int newest_of[32], newest_s;
+  __shared__ int newest_of[32], newest_s, sums_of[2][32], sums_s[2];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x;
   const int b = blockIdx.x / ctas, n = min(p.seq_lens[b], p.n_rows);
+  const int j0 = rank * kKeyThreads + tid, step = ctas * kKeyThreads;
   const float* mass = p.mass + b * p.mass_stride;
   const int32_t* positions = p.positions ? p.positions + b * p.pos_stride : nullptr;
-  int newest = n - 1;
-  if (positions) {
-    newest = -1;
-    for (int j = rank * kKeyThreads + tid; j < n; j += ctas * kKeyThreads) newest = max(newest, positions[j]);
-    newest = __reduce_max_sync(0xFFFFFFFFu, newest);
-    if ((tid & 31) == 0) newest_of[tid >> 5] = newest;
-    __syncthreads();
-    newest = __reduce_max_sync(0xFFFFFFFFu, newest_of[tid & 31]);
-    if (tid == 0) newest_s = newest;
-    cluster.sync();
-    for (int r = 0; r < ctas; ++r) newest = max(newest, *cluster.map_shared_rank(&newest_s, r));
+  float* keys = p.keys + b * p.key_stride;
+  auto weight = [&](int j, float most) { const float m = mass[j]; return m == m ? fminf(m, most) + 0.f : 0.f; };   // (-0 is 0)
+  if (!positions) {
+    for (int j = j0; j < n; j += step) keys[j] = j < p.sinks || j >= n - p.recent ? INFINITY : weight(j, FLT_MAX);
+    return;
   }
-  for (int j = rank * kKeyThreads + tid; j < n; j += ctas * kKeyThreads) {
-    const int pos = positions ? positions[j] : j;
-    const float m = mass[j];
-    p.keys[b * p.key_stride + j] = pos < p.sinks || (int64_t)pos > (int64_t)newest - p.recent ? INFINITY : m == m ? fminf(m, FLT_MAX) : 0.f;
+  int newest = INT_MIN;
+  for (int j = j0; j < n; j += step) newest = max(newest, positions[j]);
+  newest = __reduce_max_sync(0xFFFFFFFFu, newest);
+  if ((tid & 31) == 0) newest_of[tid >> 5] = newest;
+  __syncthreads();
+  newest = __reduce_max_sync(0xFFFFFFFFu, newest_of[tid & 31]);
+  if (tid == 0) newest_s = newest;
+  cluster.sync();
+  for (int r = 0; r < ctas; ++r) newest = max(newest, *cluster.map_shared_rank(&newest_s, r));
+  auto is_first = [&](int pos) { return pos >= 0 && pos < p.sinks; };          // (a negative one was never noted)
+  auto is_recent = [&](int pos) { return (int64_t)pos > (int64_t)newest - p.recent; };
+  int kept[1] = {0};
+  for (int j = j0; j < n; j += step) {
+    const int pos = positions[j];
+    const bool stays = is_first(pos) || is_recent(pos);
+    keys[j] = stays ? INFINITY : weight(j, FLT_MAX);
+    kept[0] += stays;
   }
-  if (positions) cluster.sync();                                  // the other CTAs have read this one's newest position
+  cluster_sums(kept, sums_of, sums_s);
+  if (kept[0] <= p.budget) return;                                // (the same for the whole cluster)
+  int count[2] = {0, 0};                                          // rows of the newest position, of the first ones
+  for (int j = j0; j < n; j += step) {
+    count[0] += positions[j] == newest;
+    count[1] += is_first(positions[j]);
+  }
+  cluster_sums(count, sums_of, sums_s);
+  if (count[0] > p.budget) return;
+  int end = n;                                                    // below it lie the first `sinks` rows of the first positions
+  if (count[1] > p.sinks) {
+    int lo = 0;
+    while (lo < end) {
+      const int mid = lo + (end - lo) / 2;
+      int below[1] = {0};
+      for (int j = j0; j < mid; j += step) below[0] += is_first(positions[j]);
+      cluster_sums(below, sums_of, sums_s);
+      if (below[0] >= p.sinks) end = mid;
+      else lo = mid + 1;
+    }
+  }
+  constexpr int kMost = 0x7F7FFFFF, kSteps = 0x7FFFFF;            // the largest number, and the numbers above 2^127
+  for (int j = j0; j < n; j += step) {
+    const int pos = positions[j];
+    keys[j] = is_first(pos) && j < end ? INFINITY
+              : is_recent(pos)         ? __int_as_float(kMost - (int)min((int64_t)newest - pos, (int64_t)kSteps))
+                                       : weight(j, __int_as_float(kMost - kSteps - 1));
+  }
 }
 
 struct EvictPlanParams {
@@ -381,7 +448,7 @@ extern "C" int kb200_evict(const kb200_kv_layout* layers, int n_layers, const in
   while (ctas < 8 && n_rows > ctas * 2048 && batch * ctas <= sm_count() / 2) ctas *= 2;
   KB_LAUNCH("evict_keys_kernel",
             launch_pdl(evict_keys_kernel, dim3(batch * ctas), kKeyThreads, 0, st, ctas,
-                       EvictKeysParams{mass, mass_stride, seq_lens, token_positions, pos_stride, keys, at.keys_row, sinks, recent, n_rows}));
+                       EvictKeysParams{mass, mass_stride, seq_lens, token_positions, pos_stride, keys, at.keys_row, sinks, recent, budget, n_rows}));
   if (kb200_topk_select(keys, at.keys_row, n_rows, seq_lens, nullptr, budget, ws + at.keep, budget, ws + at.keep_count, batch, stream) != 0)
     return -1;
   int2* moves = reinterpret_cast<int2*>(ws + at.moves);

@@ -703,6 +703,14 @@ class EfficientKascadeStrategy(Strategy):
         that go are the same in all layers and heads, because anchor layers hand index rows to other layers and heads.  `rows`
         must be as long as the longest sequence: what lies behind is not kept.
 
+        `recent` has to cover at least the last 32 tokens after a prompt: the weight of a prompt leaves out what a tile of 32 queries pays
+        to the tile's own keys, so the last tile has drawn none yet.
+        Where rows share positions (``append_kv(token_positions=)`` notes the first axis, which is time for video: all patches of a
+        frame share it) more rows can be protected than the budget holds; then the lowest `sinks` rows of the first
+        positions stay and the recent ones, the newest position first, and where the newest position alone has more rows than the budget, the lowest of
+        all protected rows.  To have tokens counted one by one, give them running numbers on an axis of their own, the first,
+        that `rope_axes` does not name.  A negative position counts as not noted, never as one of the first.
+
         caches: the layers' (key_cache, value_cache) or (key_cache, value_cache, k_scale, v_scale); fp16, bf16 or 4-bit, changed in
         place.  Kept rows behind the new length move into the places before it that became free, no other row moves; so
         rows lose their order, which attention does not see, and `token_positions` [B, rows] int32 (None: rows in order, of a
