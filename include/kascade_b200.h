@@ -465,8 +465,8 @@ int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t
  *   layers     host array of n_layers layouts, fp16 / bf16 or INT4, of one type, block table and set of strides (an FP8 cache has
  *              one scale per page, so its rows cannot leave their page: refused); changed in place.  The pages below the new
  *              length must belong to one sequence alone
- *   mass       [B, n_rows] fp32, rows mass_stride apart
- *   token_positions  [B, n_rows] int32 (pos_stride apart), or NULL: the row's number (a cache that no row has left yet)
+ *   mass       [B, n_rows] fp32, rows mass_stride apart (n_rows at least, with more than one sequence)
+ *   token_positions  [B, n_rows] int32 (pos_stride apart, likewise), or NULL: the row's number (a cache that no row has left yet)
  *   new_lens   [B] receives min(seq_lens[b], budget)
  *   mass_out / pos_out  [B, n_rows] (out_stride apart): the rows' weight and token position after the moves, 0 and -1 behind
  *              new_lens[b]; neither may be its input

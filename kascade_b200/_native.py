@@ -819,6 +819,10 @@ def evict(mass, layers, seq_lens, budget: int, recent: int, sinks: int, token_po
     if seq_lens.shape != (B,) or not seq_lens.is_contiguous():
         raise KascadeNativeError("evict: seq_lens [B] must be contiguous")
     _same_device(mass, seq_lens=seq_lens, token_positions=token_positions)
+    if B > 1 and mass.stride(0) < rows:                        # the same row for several sequences
+        mass = mass.contiguous()
+    if B > 1 and token_positions is not None and token_positions.stride(0) < rows:
+        token_positions = token_positions.contiguous()
     where, shape = mass.get_device(), layers[0]._keep[0].shape
     for i, layer in enumerate(layers):
         if layer._keep[0].shape != shape:

@@ -429,6 +429,8 @@ extern "C" int kb200_evict(const kb200_kv_layout* layers, int n_layers, const in
   KB_REQUIRE(n_layers >= 1 && batch >= 0 && batch <= 65535 && num_kv_heads > 0 && n_rows >= 0, "evict: bad sizes");
   KB_REQUIRE(budget >= 1 && budget <= (n_rows > 1 ? n_rows : 1) && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget,
              "evict: a budget of %d rows of %d, %d first and %d last ones protected", budget, n_rows, sinks, recent);
+  KB_REQUIRE(batch <= 1 || (mass_stride >= n_rows && (!token_positions || pos_stride >= n_rows)),
+             "evict: rows of mass or token_positions overlap: %lld and %lld apart, %d long", (long long)mass_stride, (long long)pos_stride, n_rows);
   KB_REQUIRE(out_stride >= n_rows && mass_out != mass && pos_out != token_positions,
              "evict: outputs must hold %d rows and not be inputs", n_rows);
   if (check_layers(layers, n_layers) != 0) return -1;

@@ -120,3 +120,27 @@ def test_running_numbers_on_an_axis_of_their_own():
     _, _, left = S.evict_kv([caches[1]], table, torch.tensor([T], device="cuda"), torch.zeros(1, T, device="cuda"), 20, recent=10, sinks=2,
                             token_positions=noted[1])
     assert sorted(left[0, :20].tolist()) == [*range(10), *range(86, 96)]
+
+
+def test_rows_that_sequences_share():
+    """The same weight and positions for all sequences, as broadcast tensors; the C entry takes no overlapping rows."""
+    from kascade_b200 import EfficientKascadeStrategy as S, _native as nat
+    B, rows = 3, 70
+    mass, pos = torch.rand(1, rows, generator=torch.Generator().manual_seed(2)), torch.randperm(rows, generator=torch.Generator().manual_seed(3))
+    left = _run(mass.expand(B, -1), pos.to(torch.int32).expand(B, -1), 20, 5, 2)
+    assert left[0] == left[1] == left[2]
+    k, v = (torch.zeros(B * 5, 16, 1, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    table, lens = torch.arange(B * 5, dtype=torch.int32, device="cuda").view(B, 5), torch.full((B,), rows, dtype=torch.int32, device="cuda")
+    shared = mass.cuda().expand(B, -1)
+    assert S.evict_kv([(k, v)], table, lens, shared, 20)[0].tolist() == [20] * B
+    layout, lib = nat.kv_layout_paged(k, v, table), nat.load()
+    at = torch.zeros(B, rows, dtype=torch.int32, device="cuda")
+    new, out_m, out_p = torch.zeros_like(lens), torch.zeros(B, rows, device="cuda"), torch.zeros_like(at)
+    size = lib.kb200_evict_workspace_bytes(B, rows, 20)
+    ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    own = mass.cuda().expand(B, -1).contiguous()
+    for m, p in ((rows - 1, rows), (rows, rows - 1), (0, rows)):
+        rc = lib.kb200_evict((nat.KvLayout * 1)(layout), 1, lens.data_ptr(), own.data_ptr(), m, at.data_ptr(), p, 20, 0, 0, new.data_ptr(),
+                             out_m.data_ptr(), out_p.data_ptr(), rows, ws.data_ptr(), size, B, 1, rows, None)
+        assert rc != 0 and b"overlap" in lib.kb200_last_error()
+    assert not bool(new.any())
