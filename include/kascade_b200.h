@@ -53,8 +53,14 @@ int kb200_init(int device);
 /* Replaces `get_last_error()` (…_rolling.cu:245-247).  Thread-local, never NULL. */
 const char* kb200_last_error(void);
 
-/* ABI version of this header. */
+/* ABI version: how the fields of the layouts that every call reads lie (2: with a dtype).  It does not count fields that were added
+ * behind them, which only the calls and types read that came with them. */
 int kb200_abi_version(void);
+
+/* sizeof(kb200_kv_layout) as the library was built.  A caller whose header gives another size was built against an older or newer one:
+ * it may use the calls that take one layout, with the types that its header knows (an older one), but no array of layouts
+ * (kb200_evict). */
+size_t kb200_kv_layout_bytes(void);
 
 /* Every device-side wait of the tensor-core kernels is bounded; a kernel that gives up records a
  * non-zero code in a device status word, releases what it holds and returns.  This call copies

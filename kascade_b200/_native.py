@@ -32,7 +32,7 @@ EXPORTS = [
     "kb200_kv_write", "kb200_prefill_dense_ragged", "kb200_prefill_pool_scores_ragged", "kb200_prefill_sparse_ragged",
     "kb200_prefill_budgets_ragged", "kb200_zero_padding", "kb200_peer_push", "kb200_stream_wait_events", "kb200_selftest_wait_timeout", "kb200_tensor_map_encodes", "kb200_decode_noalloc_splits",
     "kb200_kv_write_at", "kb200_kv_read", "kb200_decode_anchor_paged_mass", "kb200_mass_add_prompt", "kb200_evict",
-    "kb200_evict_workspace_bytes",
+    "kb200_evict_workspace_bytes", "kb200_kv_layout_bytes",
 ]
 
 
@@ -121,6 +121,17 @@ def _launched(n: int):
     launch_count += n
 
 
+def _check_layout(lib):
+    """The library and this binding agree on the layout that calls take one or an array of."""
+    size = getattr(lib, "kb200_kv_layout_bytes", None)
+    if size is not None:
+        size.restype = C.c_size_t
+    if size is None or size() != C.sizeof(KvLayout):
+        raise KascadeNativeError(f"{LIB_PATH} was built from other sources than this binding (its kb200_kv_layout has "
+                                 f"{size() if size is not None else 'fewer'} bytes, {C.sizeof(KvLayout)} expected): build it again with "
+                                 "`python -m kascade_b200.build`")
+
+
 def load() -> C.CDLL:
     """dlopen the library (no CUDA call is made)."""
     global _lib
@@ -130,6 +141,7 @@ def load() -> C.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m kascade_b200.build` "
                 "(there is no fallback implementation)")
         lib = C.CDLL(LIB_PATH)
+        _check_layout(lib)
         lib.kb200_last_error.restype = C.c_char_p
         lib.kb200_decode_workspace_bytes.restype = C.c_size_t
         lib.kb200_decode_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]

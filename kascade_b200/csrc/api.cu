@@ -70,6 +70,7 @@ int check_int4(const kb200_kv_layout* kv, bool need_v, const char* what) {
 }  // namespace kb200
 
 extern "C" int kb200_abi_version(void) { return 2; }
+extern "C" size_t kb200_kv_layout_bytes(void) { return sizeof(kb200_kv_layout); }
 
 extern "C" const char* kb200_last_error(void) { return kb200::g_err; }
 
