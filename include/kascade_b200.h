@@ -432,6 +432,7 @@ int kb200_kv_write_at(const kb200_act_layout* q_in, void* q_out, const kb200_act
 
 /* Rows 0 .. seq_lens[b] - 1 of an INT4 cache in 16 bits (act_dtype of the layout), for a prompt that arrives in pieces: the
  * prefill kernels take fp16 / bf16.
+ * fp16 rows saturate at +-65504.
  *   k_out / v_out  [B, max_len, G, 128] contiguous; rows behind a sequence are written as zeros */
 int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens, void* k_out, void* v_out, int batch, int max_len,
                   int num_kv_heads, void* stream);

@@ -599,7 +599,9 @@ struct KvReadParams {
   int G, rows, chunks;                                                // rows of a sequence (T G), CTAs that share them
 };
 
-// the eight values of a word of codes, the lowest nibble first: a code in the low bits of 2^23 is that number and the code
+// the eight values of a word of codes, the lowest nibble first: a code in the low bits of 2^23 is that number and the code.  Code 15
+// of a group that reaches fp16's largest number can stand for more than that (s is rounded: 65536 for -65504 .. 65504): it
+// saturates, as the row did on its way in; a NaN stays one.
 template <bool BF16>
 __device__ __forceinline__ uint4 from_codes(uint32_t w, uint64_t s2, uint64_t z2) {
   using H2 = typename Pair<BF16>::T;
@@ -610,7 +612,8 @@ __device__ __forceinline__ uint4 from_codes(uint32_t w, uint64_t s2, uint64_t z2
     const uint64_t c = pack2(__uint_as_float(((w >> (8 * e)) & 15u) | 0x4B000000u),
                              __uint_as_float(((w >> (8 * e + 4)) & 15u) | 0x4B000000u));
     const float2 v = unpack2(fma2(add2(c, minus), s2, z2));
-    out[e] = from_f2<BF16>(v.x, v.y);
+    if constexpr (BF16) out[e] = from_f2<BF16>(v.x, v.y);
+    else out[e] = __hmax2_nan(__hmin2_nan(from_f2<BF16>(v.x, v.y), __half2half2(__ushort_as_half(0x7BFF))), __half2half2(__ushort_as_half(0xFBFF)));
   }
   return *reinterpret_cast<uint4*>(out);
 }
