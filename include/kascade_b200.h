@@ -430,8 +430,8 @@ int kb200_kv_write_at(const kb200_act_layout* q_in, void* q_out, const kb200_act
                       float norm_eps, const float* inv_freq, float rope_scale, const kb200_positions* at,
                       int batch, int max_new, int num_q_heads, int num_kv_heads, void* stream);
 
-/* Rows 0 .. seq_lens[b] - 1 of an INT4 cache in 16 bits (act_dtype of the layout), for a prompt that arrives in pieces: the
- * prefill kernels take fp16 / bf16.
+/* Rows 0 .. seq_lens[b] - 1 of an INT4 cache in 16 bits (act_dtype of the layout), for attention that takes 16-bit rows: a whole
+ * prompt again (the prefill kernels take as many queries as keys), or, by the caller's own attention, a later piece of one.
  * fp16 rows saturate at +-65504.
  *   k_out / v_out  [B, max_len, G, 128] contiguous; rows behind a sequence are written as zeros */
 int kb200_kv_read(const kb200_kv_layout* kv, const int32_t* seq_lens, void* k_out, void* v_out, int batch, int max_len,

@@ -673,7 +673,9 @@ class EfficientKascadeStrategy(Strategy):
     def read_kv(key_cache, value_cache, block_table, seq_lens, max_seq_len: int, *, k_scale, v_scale,
                 dtype: torch.dtype = torch.float16):
         """Rows 0 .. seq_lens[b] - 1 of a 4-bit cache as key, value [B, max_seq_len, G, D] in `dtype` (fp16 or bf16), zeros behind
-        a sequence: for a prompt that arrives in pieces, whose attention runs over 16-bit rows."""
+        a sequence: for attention that takes 16-bit rows.  ``attention_forward`` runs a whole prompt over them (as many queries as
+        keys); a later piece of a prompt, with fewer queries than keys, is refused there, so its attention over these rows is
+        the caller's.  fp16 rows saturate at +-65504."""
         if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous():
             seq_lens = seq_lens.to(torch.int32).contiguous()
         B, G = seq_lens.shape[0], key_cache.shape[2]
