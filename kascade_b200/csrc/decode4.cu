@@ -16,8 +16,8 @@
 //     not on the 128 values, and sum_k p_k z_gk as one product with the transposed parameters.
 // The orders of the codes in K and V rows are those in which a lane needs them: 16 bytes of a K row, 8 of a V row.
 // What bounds it: dense passes and rows in order, HBM (5.5-5.6 TB/s at 37 x 16384 and 64 x 32768 keys; 128 us of 144 for the
-// former with the cache in L2, with 57 % of the issue slots and 52 % of the integer pipe busy); reuse layers, lines: DRAM hands
-// out 128 bytes at a time, so random rows of 64 + 64 + 32 bytes move 304 bytes per key (64 x 3244 rows: 92 us, 5.4 TB/s of DRAM
+// former with the cache in L2, with 59 % of the issue slots and 52 % of the integer pipe busy); reuse layers, lines: DRAM hands
+// out 128 bytes at a time, so random rows of 64 + 64 + 32 bytes move 304 bytes per key (64 x 3244 rows: 95 us, 5.3 TB/s of DRAM
 // traffic).
 // Queries are brought to a largest element of 64..128 per head by a power of two, so that bf16 ones fit fp16 exactly.
 #include "decode.cuh"
@@ -38,7 +38,8 @@ constexpr float kBase4 = 11.f, kTop4 = 13.f;
 // below 2^15 and, like p, keeps its bits down to 2^-26 of the largest, whatever the size of V.  It moves as the reference does.
 // (Without it p s falls below 2^-14, where fp16 has steps of 2^-24, wherever V is small or one key dominates: for 8192 keys with
 // one 9 above the others and V of a standard deviation of 0.03 outputs were off by 17 %.)  Scales below 2^-15 are taken
-// times 2^15, the largest power of two in fp16.
+// times 2^15, the largest power of two in fp16.  It takes 1 % of a dense pass of K and V and of a reuse layer (16 ragged sequences of
+// up to 32768 keys 147.4 -> 149.3 us, 64 x 3244 rows 117.2 -> 118.7, whole layers, L2 flushed).
 constexpr int kMaxUp4 = 15;
 constexpr float kUnbase4 = 1.f / 2048.f;                   // 2^-kBase4: the results are relative to the largest logit again
 // The tensor core rounds its sums towards zero: by about 2^-24 of the accumulator per product, always the same way.  The codes' mean

@@ -103,7 +103,7 @@ static int mass_ctas(int64_t clusters) {
 // What the rows of a sequence are ranked by: +inf for protected ones, else their weight (a NaN counts as 0, an infinite one as the
 // largest number, so that it stays behind the protected rows).  A cluster of CTAs
 // takes a sequence: the newest position first, over all of it, then the keys of its piece.  Latency is what counts: 4 sequences of 32768
-// rows 20.6 us with one CTA each, 7.8 with eight.
+// rows 20.6 us with one CTA each, 7.8 with eight; counting the protected rows, where rows have positions of their own, takes 2 more.
 // Rows that share a position (images on several axes) can be more than the budget holds.  Then the lowest `sinks` rows of the first
 // positions get +inf, the recent ones a key that falls with their distance from the newest position, above all weights: the last
 // `recent` rows in the order of positions stay in any case.  Only where the newest position alone has more rows than
