@@ -468,7 +468,8 @@ int kb200_mass_add_prompt(const float* pooled, int64_t row_stride, const int32_t
  * rows in the order of positions are among them.  (Where the newest position alone has more rows than the budget, the
  * lowest of all protected rows stay.)  A negative position is no first one: -1 stands for rows whose position was never noted.
  * Kept rows below the new length stay where they are, those behind it fill the rows that were let go, the lowest into the
- * lowest: the smallest number of moves, and no row is both source and target.  (The order of rows in a cache has no meaning to attention: positions are in the keys' rotation.)
+ * lowest: the smallest number of moves, and no row is both source and target.  (The order of rows in a cache has no meaning to
+ * attention: positions are in the keys' rotation.)
  *   layers     host array of n_layers layouts, fp16 / bf16 or INT4, of one type, block table and set of strides (an FP8 cache has
  *              one scale per page, so its rows cannot leave their page: refused); changed in place.  The pages below the new
  *              length must belong to one sequence alone

@@ -709,9 +709,10 @@ class EfficientKascadeStrategy(Strategy):
         to the tile's own keys, so the last tile has drawn none yet.
         Where rows share positions (``append_kv(token_positions=)`` notes the first axis, which is time for video: all patches of a
         frame share it) more rows can be protected than the budget holds; then the lowest `sinks` rows of the first
-        positions stay and the recent ones, the newest position first, and where the newest position alone has more rows than the budget, the lowest of
-        all protected rows.  To have tokens counted one by one, give them running numbers on an axis of their own, the first,
-        that `rope_axes` does not name.  A negative position counts as not noted, never as one of the first.
+        positions stay and the recent ones, the newest position first, and where the newest position alone has more rows than the
+        budget, the lowest of all protected rows.  To have tokens counted one by one, give them running numbers on an axis of
+        their own, the first, that `rope_axes` does not name.  A negative position counts as not noted, never as one of the
+        first.
 
         caches: the layers' (key_cache, value_cache) or (key_cache, value_cache, k_scale, v_scale); fp16, bf16 or 4-bit, changed in
         place.  Kept rows behind the new length move into the places before it that became free, no other row moves; so
@@ -748,8 +749,8 @@ class EfficientKascadeStrategy(Strategy):
         [num_pages, G] fp32 and takes fp16 queries; a 4-bit cache (``int4_kv_cache``) with its k_scale / v_scale takes
         either type.  `attention_mass` [B, rows >= max_seq_len] fp32: anchor layers add to it, in place, the attention that each
         row draws, summed over the heads (reuse layers do not see all rows and leave it as it is); ``evict_kv`` chooses by it.
-        `index_rows` = (rows [B,G,k] int32, counts [B,G] int32): a reuse layer attends to these rows (of the KV head its mapping
-        names) instead of the last anchor layer's, for a layer whose anchor runs elsewhere.  In a sharded strategy key / value
+        `index_rows` = (rows [B,G,k] int32, counts [B,G] int32; rows of the sequence, below its length): a reuse layer attends to
+        these rows (of the KV head its mapping names) instead of the last anchor layer's, for a layer whose anchor runs elsewhere.  In a sharded strategy key / value
         cache, queries and index rows are those of this rank's KV heads, and a reuse layer whose mapping names another rank's
         head is refused.  `mean_seq_len` is a hint of the host for batches of very different lengths (the work is then cut
         into more, smaller pieces); results do not depend on it beyond summation order.
